@@ -46,7 +46,7 @@ def default_ref_root() -> str:
 def build(ref_root: str | None = None) -> None:
     ref_root = ref_root or default_ref_root()
     subprocess.run(["make", "-s", "-C", HERE, "all"], check=True)
-    if os.path.isdir(ref_root):
+    if os.path.isdir(os.path.join(ref_root, "src")):
         subprocess.run(["make", "-s", "-C", HERE, "ref", f"REF_ROOT={ref_root}"], check=True)
         # the reference's own test program over the GPU library (needs the library built first)
         subprocess.run(["make", "-s", "-C", HERE, "shimtest", f"REF_ROOT={ref_root}"], check=True)
