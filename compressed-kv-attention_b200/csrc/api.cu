@@ -7,6 +7,7 @@
 // host-resident blobs (the same walk the reference does in include/kvexp/scan.hpp), moves
 // buffers and launches kernels.
 #include "codec.cuh"
+#include "host.cuh"
 
 #include <algorithm>
 #include <cstdio>
@@ -17,21 +18,17 @@
 #include <vector>
 
 namespace kvx {
-namespace {
 
+namespace {
 thread_local std::string g_err;
+}
 
 int fail(int code, const std::string &msg) {
     g_err = msg;
     return code;
 }
 
-#define KVX_CUDA(call)                                                                         \
-    do {                                                                                       \
-        cudaError_t e_ = (call);                                                               \
-        if (e_ != cudaSuccess)                                                                 \
-            return fail(KVX_ERR_CUDA, std::string(#call) + ": " + cudaGetErrorString(e_));     \
-    } while (0)
+void clear_error() { g_err.clear(); }
 
 const char *detail_message(int code, int detail) {
     switch (detail) {
@@ -50,10 +47,15 @@ const char *detail_message(int code, int detail) {
     case DERR_RANGE: return "xkv block index entry outside its blob";
     case DERR_ESC_CAP:
         return "kvx_attention_decode_noalloc: the blobs' escape positions exceed the fixed scratch";
+    case DERR_POSITION: return "position outside the rotation tables";
+    case DERR_SLOT: return "slot outside the page pools";
+    case DERR_PAGE: return "page table entry outside the page pools";
+    case DERR_LENGTH: return "sequence length negative or above max_len";
     default: return "device error";
     }
 }
 
+namespace {
 
 // RAII device buffer (stream-ordered allocator).
 struct DevBuf {
@@ -101,6 +103,8 @@ bool is_device_ptr(const void *p) {
 
 constexpr int kMaxDevices = 64;
 
+}  // namespace
+
 int check_device() {
     int dev = 0;
     KVX_CUDA(cudaGetDevice(&dev));
@@ -122,6 +126,8 @@ int check_device() {
         });
     return KVX_OK;
 }
+
+namespace {
 
 // A pinned host buffer per device for the outputs of the host-buffer entry points: one
 // device -> host copy per chunk of units instead of one per unit; held (locked) by one call at a
@@ -150,12 +156,24 @@ int copy_stream(cudaStream_t *out) {
     return KVX_OK;
 }
 
+}  // namespace
+
 int sm_count() {
     int dev = 0, n = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
     return n;
 }
+
+int read_status(int *dev_status, bool reset) {
+    int st[2] = {0, 0};
+    KVX_CUDA(cudaMemcpy(st, dev_status, sizeof st, cudaMemcpyDeviceToHost));
+    if (st[0] == 0) return KVX_OK;
+    if (reset) cudaMemset(dev_status, 0, sizeof st);
+    return fail(st[0], detail_message(st[0], st[1]));
+}
+
+namespace {
 
 // ---- host header walk (include/kvexp/scan.hpp:28-66, :94-123) ----------------------------------
 
@@ -354,14 +372,6 @@ struct PlanGuard {
     kvx_plan_s *p;
     ~PlanGuard() { delete p; }
 };
-
-int read_status(int *dev_status, bool reset) {
-    int st[2] = {0, 0};
-    KVX_CUDA(cudaMemcpy(st, dev_status, sizeof st, cudaMemcpyDeviceToHost));
-    if (st[0] == 0) return KVX_OK;
-    if (reset) cudaMemset(dev_status, 0, sizeof st);
-    return fail(st[0], detail_message(st[0], st[1]));
-}
 
 }  // namespace
 

@@ -1,0 +1,279 @@
+// batch.cu -- host side of the serving-step operators (kvx_batch_*): argument checks, the cut of an
+// attention call into items, scratch, launches.
+#include <algorithm>
+#include <cmath>
+#include <new>
+
+#include "host.cuh"
+#include "paged.cuh"
+
+using namespace kvx;
+
+struct kvx_batch_s {
+    int max_batch = 0, n_q_heads = 0, n_kv_heads = 0, group = 0, dim = 0, dtype = 0;
+    int sms = 0;
+    int64_t cap_rows = 0;   // partial-state rows of the scratch
+    float *acc = nullptr;
+    float2 *ml = nullptr;
+    int *status = nullptr;
+    ~kvx_batch_s() {
+        cudaFree(acc);
+        cudaFree(ml);
+        cudaFree(status);
+    }
+};
+
+namespace {
+
+constexpr int kMaxTokens = 1 << 30;   // of a prefix or a tail (token arithmetic in 32 bits)
+constexpr int kMaxBatch = 65535;      // grid limit of the combine pass
+
+// Items of an attention call.  About kItemsPerSm CTAs an SM keep the loads of a streaming kernel in
+// flight and even out ragged tails; an item takes at least kMinChunk tokens, below which the join
+// of its warps and the write of its partial state weigh more than its loads.
+constexpr int kItemsPerSm = 16;
+constexpr int kMinChunk = 256;
+
+int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
+
+// Rows of an upper bound of the scratch an attention call of `batch` sequences takes.
+int64_t scratch_rows(const kvx_batch_s *h, int batch) {
+    const int64_t qg = ceil_div(h->group, 8), rg = ceil_div(int64_t(batch) * h->group, 8);
+    const int64_t items = int64_t(kItemsPerSm) * h->sms;
+    const int64_t prefix = (items + h->n_kv_heads * rg) * 8;
+    const int64_t tails = (items / qg + 1 + int64_t(batch) * h->n_kv_heads) * h->group;
+    return prefix + tails;
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool rows_aligned(const kvx_view &v) {
+    return aligned16(v.data) && v.token_stride % 8 == 0 && v.head_stride % 8 == 0;
+}
+
+PageSplit page_split(int tokens) {
+    PageSplit p{tokens, -1};
+    if ((tokens & (tokens - 1)) == 0)
+        for (p.shift = 0; (1 << p.shift) < tokens;) ++p.shift;
+    return p;
+}
+
+int pool_of(const char *who, const kvx_pages *p, PoolDev &out) {
+    if (p == nullptr || p->k == nullptr || p->v == nullptr || p->n_pages <= 0 || p->page_tokens <= 0 ||
+        p->page_stride < 0 || p->token_stride < 0 || p->head_stride < 0)
+        return fail(KVX_ERR_INVALID_ARGUMENT, std::string(who) + ": bad page pools");
+    out.k = static_cast<uint16_t *>(p->k);
+    out.v = static_cast<uint16_t *>(p->v);
+    out.page_stride = p->page_stride;
+    out.token_stride = p->token_stride;
+    out.head_stride = p->head_stride;
+    out.n_pages = p->n_pages;
+    out.split = page_split(p->page_tokens);
+    return KVX_OK;
+}
+
+int rope_of(const char *who, const kvx_batch_s *h, const kvx_rope *r, RotArgs &a) {
+    if (r->cos == nullptr || r->sin == nullptr || r->pos == nullptr || r->n_pos <= 0 || r->rot_dim <= 0 ||
+        r->rot_dim % 2 != 0 || r->rot_dim > h->dim || r->n_axes <= 0 || r->n_axes > 255 ||
+        (r->n_axes > 1 && r->axis == nullptr))
+        return fail(KVX_ERR_INVALID_ARGUMENT, std::string(who) + ": bad rotation");
+    a.cos = r->cos;
+    a.sin = r->sin;
+    a.pos = r->pos;
+    a.axis = r->axis;
+    a.pos_stride = r->pos_stride;
+    a.n_pos = r->n_pos;
+    a.rot_dim = r->rot_dim;
+    a.n_axes = r->n_axes;
+    a.interleaved = r->interleaved != 0;
+    return KVX_OK;
+}
+
+// Whether a launch may take 16 values a thread: every row it reads or writes starts on 16 bytes and
+// the rotated part and the rest are whole 16-value pieces.
+bool vector_path(const RotArgs &a, int n_seg) {
+    if (a.dim % 16 != 0 || a.rot_dim % 16 != 0) return false;
+    if (a.rot_dim > 0 && (!aligned16(a.cos) || !aligned16(a.sin) || (reinterpret_cast<uintptr_t>(a.axis) & 7u) != 0))
+        return false;
+    for (int i = 0; i < n_seg; ++i) {
+        const RotSeg &s = a.seg[i];
+        if (!aligned16(s.src) || s.src_token % 8 != 0 || s.src_head % 8 != 0) return false;
+        if (s.pool == 0 && (!aligned16(s.dst) || s.dst_token % 8 != 0 || s.dst_head % 8 != 0)) return false;
+        if (s.pool != 0 && (!aligned16(s.pool == 1 ? a.pool.k : a.pool.v) || a.pool.page_stride % 8 != 0 ||
+                            a.pool.token_stride % 8 != 0 || a.pool.head_stride % 8 != 0))
+            return false;
+    }
+    return true;
+}
+
+RotSeg seg_of(const kvx_view *src, const kvx_view *dst, int heads, bool rotated, int pool) {
+    RotSeg s{};
+    s.src = static_cast<const uint16_t *>(src->data);
+    s.src_token = src->token_stride;
+    s.src_head = src->head_stride;
+    if (dst != nullptr) {
+        s.dst = static_cast<uint16_t *>(dst->data);
+        s.dst_token = dst->token_stride;
+        s.dst_head = dst->head_stride;
+    }
+    s.heads = heads;
+    s.rotated = rotated;
+    s.pool = pool;
+    return s;
+}
+
+bool view_ok(const kvx_view *v) { return v != nullptr && v->data != nullptr; }
+
+}  // namespace
+
+extern "C" {
+
+int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int dtype, kvx_batch *out) {
+    if (out == nullptr || max_batch <= 0 || max_batch > kMaxBatch || n_q_heads <= 0 || n_kv_heads <= 0 ||
+        n_q_heads % n_kv_heads != 0 || dim <= 0 || dim % 2 != 0 || dim > kMaxHeadDim ||
+        (dtype != KVX_DTYPE_BF16 && dtype != KVX_DTYPE_FP16))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_create: bad argument");
+    *out = nullptr;
+    if (int rc = check_device()) return rc;
+    auto *h = new (std::nothrow) kvx_batch_s();
+    if (h == nullptr) return fail(KVX_ERR_RUNTIME, "kvx_batch_create: out of host memory");
+    h->max_batch = max_batch;
+    h->n_q_heads = n_q_heads;
+    h->n_kv_heads = n_kv_heads;
+    h->group = n_q_heads / n_kv_heads;
+    h->dim = dim;
+    h->dtype = dtype;
+    h->sms = sm_count();
+    h->cap_rows = scratch_rows(h, max_batch);
+    cudaError_t e = cudaMalloc(&h->status, 2 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(h->status, 0, 2 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&h->acc, size_t(h->cap_rows) * dim * sizeof(float));
+    if (e == cudaSuccess) e = cudaMalloc(&h->ml, size_t(h->cap_rows) * sizeof(float2));
+    if (e != cudaSuccess) {
+        delete h;
+        return fail(KVX_ERR_CUDA, std::string("kvx_batch_create: ") + cudaGetErrorString(e));
+    }
+    *out = h;
+    clear_error();
+    return KVX_OK;
+}
+
+void kvx_batch_destroy(kvx_batch h) { delete h; }
+
+int kvx_batch_check(kvx_batch h) {
+    if (h == nullptr) return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_check: null batch");
+    KVX_CUDA(cudaDeviceSynchronize());
+    if (int rc = read_status(h->status, true)) return rc;
+    clear_error();
+    return KVX_OK;
+}
+
+int kvx_batch_rotate(kvx_batch h, const kvx_view *x, const kvx_view *out, int n_tokens, int n_heads,
+                     const kvx_rope *rope, int inverse, void *stream) {
+    if (h != nullptr && n_tokens == 0) return KVX_OK;  // (an empty tensor's address is null)
+    if (h == nullptr || !view_ok(x) || !view_ok(out) || n_tokens < 0 || n_heads <= 0 || rope == nullptr)
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_rotate: bad argument");
+    RotArgs a{};
+    if (int rc = rope_of("kvx_batch_rotate", h, rope, a)) return rc;
+    a.seg[0] = seg_of(x, out, n_heads, true, 0);
+    a.inverse = inverse != 0;
+    a.status = h->status;
+    a.n_tokens = n_tokens;
+    a.dim = h->dim;
+    a.heads = n_heads;
+    KVX_CUDA(launch_rotate(h->dtype, vector_path(a, 1), a, static_cast<cudaStream_t>(stream)));
+    return KVX_OK;
+}
+
+int kvx_batch_append(kvx_batch h, const kvx_view *q, const kvx_view *k, const kvx_view *v, const kvx_view *q_out,
+                     int n_tokens, const kvx_rope *rope, const int64_t *slots, const kvx_pages *pages, void *stream) {
+    if (h != nullptr && n_tokens == 0) return KVX_OK;
+    const bool has_q = q != nullptr && q->data != nullptr;
+    if (h == nullptr || !view_ok(k) || !view_ok(v) || n_tokens < 0 || slots == nullptr ||
+        has_q != (q_out != nullptr && q_out->data != nullptr))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_append: bad argument");
+    RotArgs a{};
+    if (int rc = pool_of("kvx_batch_append", pages, a.pool)) return rc;
+    if (rope != nullptr)
+        if (int rc = rope_of("kvx_batch_append", h, rope, a)) return rc;
+    int n = 0;
+    if (has_q) a.seg[n++] = seg_of(q, q_out, h->n_q_heads, rope != nullptr, 0);
+    a.seg[n++] = seg_of(k, nullptr, h->n_kv_heads, rope != nullptr, 1);
+    a.seg[n++] = seg_of(v, nullptr, h->n_kv_heads, false, 2);
+    a.slots = slots;
+    a.status = h->status;
+    a.n_tokens = n_tokens;
+    a.dim = h->dim;
+    a.heads = (has_q ? h->n_q_heads : 0) + 2 * h->n_kv_heads;
+    KVX_CUDA(launch_rotate(h->dtype, vector_path(a, n), a, static_cast<cudaStream_t>(stream)));
+    return KVX_OK;
+}
+
+int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
+    if (h != nullptr && x != nullptr && x->batch == 0) return KVX_OK;
+    if (h == nullptr || x == nullptr || x->batch < 0 || x->batch > h->max_batch || !view_ok(&x->q) ||
+        !view_ok(&x->out) || x->prefix_len < 0 || x->max_len < 0 || x->prefix_len > kMaxTokens ||
+        x->max_len > kMaxTokens || !(x->scale >= 0.f))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: bad argument");
+    if (h->dim != 32 && h->dim != 64 && h->dim != 128 && h->dim != 256)
+        return fail(KVX_ERR_UNSUPPORTED, "kvx_batch_attend: head_dim must be 32, 64, 128 or 256");
+    const bool paged = x->prefix_table != nullptr && x->prefix_len > 0;
+    if (x->prefix_len > 0 && x->prefix_table == nullptr)
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: a prefix without its page table");
+    if (x->max_len > 0 && (x->table == nullptr || x->lens == nullptr))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: tails without page table or lengths");
+    if (!rows_aligned(x->q))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: query rows must be 16-byte aligned");
+    PagedArgs a{};
+    if (int rc = pool_of("kvx_batch_attend", x->pages, a.pool)) return rc;
+    if (!aligned16(a.pool.k) || !aligned16(a.pool.v) || a.pool.page_stride % 8 != 0 || a.pool.token_stride % 8 != 0 ||
+        a.pool.head_stride % 8 != 0)
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: page rows must be 16-byte aligned");
+    a.q = static_cast<const uint16_t *>(x->q.data);
+    a.q_token = x->q.token_stride;
+    a.q_head = x->q.head_stride;
+    a.out = static_cast<uint16_t *>(x->out.data);
+    a.out_token = x->out.token_stride;
+    a.out_head = x->out.head_stride;
+    a.lse = x->lse;
+    a.prefix_table = x->prefix_table;
+    a.table = x->table;
+    a.lens = x->lens;
+    a.table_stride = x->table_stride;
+    a.prefix_len = paged ? x->prefix_len : 0;
+    a.max_len = x->max_len;
+    a.batch = x->batch;
+    a.n_q_heads = h->n_q_heads;
+    a.n_kv_heads = h->n_kv_heads;
+    a.group = h->group;
+    a.scale_log2 = float((x->scale > 0.f ? double(x->scale) : 1.0 / std::sqrt(double(h->dim))) * 1.4426950408889634);
+    a.acc = h->acc;
+    a.ml = h->ml;
+    a.status = h->status;
+    const int items = kItemsPerSm * h->sms;
+    const int rows = x->batch * h->group;
+    a.q_groups = ceil_div(h->group, 8);
+    a.row_groups = ceil_div(rows, 8);
+    a.row_pad = 8 * a.row_groups;
+    if (paged) {
+        const int most = std::max(1, items / (h->n_kv_heads * a.row_groups));
+        a.split_tokens = std::max(kMinChunk, ceil_div(ceil_div(x->prefix_len, most), 128) * 128);
+        a.n_split = ceil_div(x->prefix_len, a.split_tokens);
+        a.prefix_items = h->n_kv_heads * a.n_split * a.row_groups;
+    }
+    a.tail_base = int64_t(h->n_kv_heads) * a.n_split * a.row_pad;
+    if (x->max_len > 0) {
+        const int most = std::max(1, items / (x->batch * h->n_kv_heads * a.q_groups));
+        a.chunk_tokens = std::max(kMinChunk, ceil_div(ceil_div(x->max_len, most), 128) * 128);
+        a.n_chunk = ceil_div(x->max_len, a.chunk_tokens);
+        a.tail_items = x->batch * h->n_kv_heads * a.n_chunk * a.q_groups;
+    }
+    const int64_t used = a.tail_base + int64_t(x->batch) * h->n_kv_heads * a.n_chunk * h->group;
+    if (used > h->cap_rows) return fail(KVX_ERR_RUNTIME, "kvx_batch_attend: scratch too small");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    KVX_CUDA(launch_paged_stream(h->dim, h->dtype, a, s));
+    KVX_CUDA(launch_paged_combine(h->dim, h->dtype, a, s));
+    return KVX_OK;
+}
+
+}  // extern "C"

@@ -32,6 +32,10 @@ enum DeviceError : int {
     DERR_INDEX_CAP = 10,    // more blocks than the index capacity
     DERR_RANGE = 11,        // an index entry points outside its blob
     DERR_ESC_CAP = 12,      // escape records do not fit the fixed scratch
+    DERR_POSITION = 13,     // a position outside the rotation tables
+    DERR_SLOT = 14,         // a slot outside the page pools
+    DERR_PAGE = 15,         // a page table entry outside the page pools
+    DERR_LENGTH = 16,       // a sequence length that is negative or above max_len
 };
 
 // Residual code bytes of a coded block: the reference's formula for 2 and 4 bits

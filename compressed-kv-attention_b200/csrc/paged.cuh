@@ -1,0 +1,94 @@
+// paged.cuh -- declarations shared by the serving-step kernels (rotation, append, attention over a
+// shared prefix and paged tails) and their host code.
+#pragma once
+
+#include "common.cuh"
+
+namespace kvx {
+
+// Page lookup: token -> (page of the table, place in it).
+struct PageSplit {
+    int32_t tokens;  // per page
+    int32_t shift;   // log2(tokens) when it is a power of two, else -1
+    __device__ __forceinline__ void at(int64_t t, int64_t &page, int32_t &place) const {
+        if (shift >= 0) {
+            page = t >> shift;
+            place = int32_t(t & (tokens - 1));
+        } else if (t < int64_t(1) << 31) {  // a 32-bit division is several times cheaper
+            const uint32_t p = uint32_t(t) / uint32_t(tokens);
+            page = p;
+            place = int32_t(uint32_t(t) - p * uint32_t(tokens));
+        } else {
+            page = t / tokens;
+            place = int32_t(t - page * tokens);
+        }
+    }
+};
+
+struct PoolDev {
+    uint16_t *k, *v;
+    int64_t page_stride, token_stride, head_stride;  // elements
+    int32_t n_pages;
+    PageSplit split;
+};
+
+// One kind of head of a rotate / append launch.
+struct RotSeg {
+    const uint16_t *src;
+    uint16_t *dst;          // null: into the pools
+    int64_t src_token, src_head, dst_token, dst_head;
+    int32_t heads;
+    int32_t rotated;        // 0: copied as it is
+    int32_t pool;           // 0: dst; 1: K pool; 2: V pool
+};
+
+struct RotArgs {
+    RotSeg seg[3];
+    const float *cos, *sin;
+    const int32_t *pos;
+    const uint8_t *axis;
+    int64_t pos_stride;
+    const int64_t *slots;
+    PoolDev pool;
+    int *status;
+    int32_t n_pos, rot_dim, n_axes, interleaved, inverse;
+    int32_t n_tokens, dim, heads;    // heads: of all segments together
+    int32_t tokens_per_cta;
+};
+
+cudaError_t launch_rotate(int dtype, bool vec, const RotArgs &a, cudaStream_t s);
+
+// One attention call (kvx_batch_attend) as its kernels see it.
+struct PagedArgs {
+    const uint16_t *q;
+    uint16_t *out;
+    float *lse;
+    int64_t q_token, q_head, out_token, out_head;
+    PoolDev pool;
+    const int32_t *prefix_table, *table, *lens;
+    int64_t table_stride;
+    int32_t prefix_len, max_len;
+    int32_t batch, n_q_heads, n_kv_heads, group;
+    float scale_log2;       // scale * log2(e)
+    // partial states: row r has dim accumulators at acc + r * dim and {m (log2 units), l} at ml[r]
+    float *acc;
+    float2 *ml;
+    int *status;
+    // prefix parts: row ((kv head * n_split + split) * row_pad + (sequence * group + g));
+    // n_split parts per row, each `split_tokens` tokens but the last
+    int32_t n_split, row_pad;
+    int32_t split_tokens;
+    // tail parts: row tail_base + ((sequence * kv heads + kv head) * n_chunk + chunk) * group + g
+    int64_t tail_base;
+    int32_t n_chunk, chunk_tokens;
+    // CTAs of the streaming kernel: prefix items first, then tail items
+    int32_t prefix_items, tail_items;
+    int32_t q_groups;       // 8-query groups of a tail item's heads
+    int32_t row_groups;     // 8-row groups of the prefix rows (streaming prefix)
+};
+
+// The streaming kernel over the items of `a` and the combine pass over every (sequence, head).
+cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
+cudaError_t launch_paged_combine(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
+
+}  // namespace kvx

@@ -1,0 +1,67 @@
+// paged_types.cuh -- the two 16-bit types of the serving-step attention kernels.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "paged.cuh"
+
+namespace kvx {
+
+constexpr float kPagedLog2e = 1.4426950408889634f;
+constexpr float kPagedLn2 = 0.6931471805599453f;
+
+// Softmax weights enter the tensor cores in the cache's type, rounded to nearest: 8 significant
+// bits in BF16, 11 in FP16, the same relative size as the output's own rounding (the normaliser l
+// sums them unrounded, in FP32, so the log-sum-exp does not see it).  kBias: weights are formed as
+// 2^(x - m + kBias); FP16's normal numbers end at 2^-14, so a bias of 10 keeps weights down to
+// 2^-24 of the largest at full precision (and its largest, 2^10 times the growth a kernel allows
+// before it rescales, below 65504).  The bias is part of the stored m, so it cancels.
+template <int DT> struct Elem;
+template <> struct Elem<KVX_DTYPE_BF16> {
+    static constexpr float kBias = 0.f;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ uint16_t one(float x) { return __bfloat16_as_ushort(__float2bfloat16_rn(x)); }
+};
+template <> struct Elem<KVX_DTYPE_FP16> {
+    static constexpr float kBias = 10.f;
+    static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    static __device__ __forceinline__ uint16_t one(float x) { return __half_as_ushort(__float2half_rn(x)); }
+};
+
+// 2^x by the SFU; results below 2^-126 flush to zero.
+__device__ __forceinline__ float exp2_sfu(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Row offset (elements, without the head) of token t of a page list, or -1 when the table's entry
+// is outside the pool (reported).
+__device__ __forceinline__ int64_t page_row(const PoolDev &p, const int32_t *table, int64_t t, int *status) {
+    int64_t i;
+    int32_t place;
+    p.split.at(t, i, place);
+    const int32_t page = __ldg(table + i);
+    if (unsigned(page) >= unsigned(p.n_pages)) {
+        report(status, KVX_ERR_RUNTIME, DERR_PAGE);
+        return -1;
+    }
+    return int64_t(page) * p.page_stride + int64_t(place) * p.token_stride;
+}
+
+// lens[b] clamped to [0, max_len] (reported when it was outside).
+__device__ __forceinline__ int tail_len(const PagedArgs &a, int b) {
+    const int n = __ldg(a.lens + b);
+    if (n >= 0 && n <= a.max_len) return n;
+    report(a.status, KVX_ERR_RUNTIME, DERR_LENGTH);
+    return n < 0 ? 0 : a.max_len;
+}
+
+}  // namespace kvx

@@ -250,6 +250,99 @@ KVX_API int kvx_attention_decode_noalloc(const uint16_t *q, const uint8_t *k_xkv
                                  const kvx_block *v_index, int n_blocks, float *out, int n_q,
                                  int dim, int seq, void *stream);
 
+/* ---- serving step: position rotation, paged cache, attention over a shared prefix ---------- */
+
+/* The operators of a batch's decode step beside the compressed cache: rotate queries and keys by
+ * their positions, append new keys and values to a paged cache (rotated on the way), and attend
+ * from every sequence of a batch to one shared prefix (read once for all of them) followed by the
+ * sequence's own pages.  All calls are asynchronous on `stream`, allocate nothing and do not
+ * synchronise, so they can be captured in a CUDA graph.  No counterpart in the reference. */
+#define KVX_DTYPE_BF16 0
+#define KVX_DTYPE_FP16 1
+
+typedef struct kvx_batch_s *kvx_batch;
+
+/* [n_tokens, n_heads, dim] values of the batch's type in device memory: dim contiguous, strides in
+ * elements.  Any strides and alignment work; 16-byte aligned rows take the vector path. */
+typedef struct kvx_view {
+    void *data;
+    int64_t token_stride;
+    int64_t head_stride;
+} kvx_view;
+
+/* One layer's K and V page pools: element (page, token, head, d) of either at page * page_stride +
+ * token * token_stride + head * head_stride + d (elements), whichever of tokens and heads is
+ * outside.  kvx_batch_attend needs 16-byte aligned rows. */
+typedef struct kvx_pages {
+    void *k;
+    void *v;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t n_pages;
+    int32_t page_tokens; /* any positive number */
+} kvx_pages;
+
+/* A rotation: pair i of a head's first rot_dim values (i < rot_dim / 2; values i and i + rot_dim /
+ * 2, or 2 i and 2 i + 1 when interleaved) turns by the angle whose cosine and sine are at
+ * cos / sin[p * rot_dim / 2 + i], p the token's position on the pair's axis: pos[axis[i] *
+ * pos_stride + token].  (a, b) becomes (a cos - b sin, b cos + a sin), in FP32, rounded once;
+ * values past rot_dim stay.  axis NULL: every pair on axis 0.  All pointers are device memory. */
+typedef struct kvx_rope {
+    const float *cos;     /* [n_pos, rot_dim / 2] */
+    const float *sin;
+    const int32_t *pos;   /* [n_axes, n_tokens], rows pos_stride apart */
+    const uint8_t *axis;  /* [rot_dim / 2], each < n_axes */
+    int64_t pos_stride;
+    int32_t n_pos;
+    int32_t rot_dim;      /* even, <= dim */
+    int32_t n_axes;
+    int32_t interleaved;
+} kvx_rope;
+
+/* One attention call. */
+typedef struct kvx_attend {
+    kvx_view q;                  /* token = sequence: [batch, n_q_heads, dim] */
+    kvx_view out;                /* the same shape and type */
+    float *lse;                  /* optional [batch, n_q_heads] FP32: log-sum-exp of the scaled scores */
+    const kvx_pages *pages;
+    const int32_t *prefix_table; /* pages of the shared prefix */
+    const int32_t *table;        /* pages of each sequence: rows table_stride apart */
+    const int32_t *lens;         /* [batch] tokens in each sequence's own pages */
+    int64_t table_stride;
+    int32_t prefix_len;
+    int32_t max_len;             /* >= every lens[b]; table rows hold that many tokens' pages */
+    int32_t batch;
+    float scale;                 /* of q . k; 0 means dim^-1/2 */
+} kvx_attend;
+
+/* A batch's handle: its head layout, its scratch for up to max_batch sequences and its device
+ * status word.  n_q_heads is a multiple of n_kv_heads (query head h reads KV head h / (n_q_heads /
+ * n_kv_heads)).  dim is even and at most 256; kvx_batch_attend takes 32, 64, 128 and 256.  One
+ * handle serves every layer; like a plan's steps, its attention calls run one after another (calls
+ * that overlap on two streams race on its scratch). */
+KVX_API int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int dtype,
+                             kvx_batch *batch);
+/* out = x rotated (inverse != 0: by the opposite angles, which is the gradient's rotation).  out
+ * may be x. */
+KVX_API int kvx_batch_rotate(kvx_batch batch, const kvx_view *x, const kvx_view *out, int n_tokens,
+                             int n_heads, const kvx_rope *rope, int inverse, void *stream);
+/* Store n_tokens new tokens: k rotated and v as it is at slots[token] = page * page_tokens + place
+ * in the page (negative: a padding token, not stored), and q rotated into q_out (both NULL: no
+ * queries).  rope NULL: nothing is rotated.  Slots are distinct. */
+KVX_API int kvx_batch_append(kvx_batch batch, const kvx_view *q, const kvx_view *k, const kvx_view *v,
+                             const kvx_view *q_out, int n_tokens, const kvx_rope *rope,
+                             const int64_t *slots, const kvx_pages *pages, void *stream);
+/* out[b, h] = softmax over the prefix's tokens and the first lens[b] tokens of the sequence's own
+ * pages.  A sequence with neither gets zeros and an lse of -inf.  What a page holds past the
+ * last token is never used, whatever its bits. */
+KVX_API int kvx_batch_attend(kvx_batch batch, const kvx_attend *args, void *stream);
+/* Synchronise and report device-side errors since the last check: a position outside the tables or
+ * a slot outside the pools (what they concern was not written), a table entry outside the pools (its tokens
+ * were left out) or a length outside [0, max_len] (clamped). */
+KVX_API int kvx_batch_check(kvx_batch batch);
+KVX_API void kvx_batch_destroy(kvx_batch batch);
+
 /* ---- benchmark support -------------------------------------------------------------------- */
 
 /* Fill [seq, dim] BF16 on the device with the seeded synthetic distribution `profile`
