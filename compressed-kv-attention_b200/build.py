@@ -15,7 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIB_DIR, "libkvexp_b200.so")
-SOURCES = ["api.cu", "attention.cu", "codec.cu", "batch.cu", "rotate.cu", "paged_stream.cu"]
+SOURCES = ["api.cu", "attention.cu", "codec.cu", "batch.cu", "rotate.cu", "paged_stream.cu",
+           "prefix_attention.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 FLAGS = [

@@ -36,11 +36,35 @@ constexpr int kMinChunk = 256;
 
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
+// A batch of at most this many rows a KV head streams its prefix like a tail; more rows go through
+// the tensor-core kernel.
+constexpr int kStreamRows = 8;
+
+// The cut of a prefix for the tensor-core kernel: tiles a split, the splits that end soonest when
+// `slots` CTAs run at a time and an item costs its tiles and about kItemTiles more (its queries,
+// the pipeline's fill and the write of its state).
+constexpr int kItemTiles = 4;
+int prefix_split_tiles(int tiles, int lists, int slots) {
+    int best = tiles;
+    int64_t least = INT64_MAX;
+    for (int waves = 1; waves <= 4; ++waves) {
+        const int splits = std::max(1, int(int64_t(waves) * slots / lists));
+        const int per = ceil_div(tiles, splits);
+        const int64_t items = int64_t(ceil_div(tiles, per)) * lists;
+        const int64_t cost = (items + slots - 1) / slots * (per + kItemTiles);
+        if (cost < least) least = cost, best = per;
+    }
+    return best;
+}
+
 // Rows of an upper bound of the scratch an attention call of `batch` sequences takes.
 int64_t scratch_rows(const kvx_batch_s *h, int batch) {
     const int64_t qg = ceil_div(h->group, 8), rg = ceil_div(int64_t(batch) * h->group, 8);
     const int64_t items = int64_t(kItemsPerSm) * h->sms;
-    const int64_t prefix = (items + h->n_kv_heads * rg) * 8;
+    const int64_t stream = (items + h->n_kv_heads * rg) * 8;
+    const int64_t tensor = (4 * int64_t(prefix_ctas_per_sm(h->dim)) * h->sms +
+                            h->n_kv_heads * int64_t(ceil_div(int64_t(batch) * h->group, kPrefixRows))) * kPrefixRows;
+    const int64_t prefix = std::max(stream, tensor);
     const int64_t tails = (items / qg + 1 + int64_t(batch) * h->n_kv_heads) * h->group;
     return prefix + tails;
 }
@@ -253,9 +277,16 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     const int items = kItemsPerSm * h->sms;
     const int rows = x->batch * h->group;
     a.q_groups = ceil_div(h->group, 8);
-    a.row_groups = ceil_div(rows, 8);
-    a.row_pad = 8 * a.row_groups;
-    if (paged) {
+    const bool tensor = paged && rows > kStreamRows;
+    a.row_groups = ceil_div(rows, tensor ? kPrefixRows : 8);
+    a.row_pad = (tensor ? kPrefixRows : 8) * a.row_groups;
+    if (tensor) {
+        const int per = prefix_split_tiles(ceil_div(x->prefix_len, kPrefixTile), h->n_kv_heads * a.row_groups,
+                                           prefix_ctas_per_sm(h->dim) * h->sms);
+        a.split_tokens = per * kPrefixTile;
+        a.n_split = ceil_div(x->prefix_len, a.split_tokens);
+        a.prefix_items = h->n_kv_heads * a.n_split * a.row_groups;
+    } else if (paged) {
         const int most = std::max(1, items / (h->n_kv_heads * a.row_groups));
         a.split_tokens = std::max(kMinChunk, ceil_div(ceil_div(x->prefix_len, most), 128) * 128);
         a.n_split = ceil_div(x->prefix_len, a.split_tokens);
@@ -271,6 +302,10 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     const int64_t used = a.tail_base + int64_t(x->batch) * h->n_kv_heads * a.n_chunk * h->group;
     if (used > h->cap_rows) return fail(KVX_ERR_RUNTIME, "kvx_batch_attend: scratch too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (tensor) {
+        KVX_CUDA(launch_paged_prefix(h->dim, h->dtype, a, s));
+        a.prefix_items = 0;
+    }
     KVX_CUDA(launch_paged_stream(h->dim, h->dtype, a, s));
     KVX_CUDA(launch_paged_combine(h->dim, h->dtype, a, s));
     return KVX_OK;

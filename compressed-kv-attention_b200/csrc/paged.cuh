@@ -81,12 +81,17 @@ struct PagedArgs {
     // tail parts: row tail_base + ((sequence * kv heads + kv head) * n_chunk + chunk) * group + g
     int64_t tail_base;
     int32_t n_chunk, chunk_tokens;
-    // CTAs of the streaming kernel: prefix items first, then tail items
-    int32_t prefix_items, tail_items;
+    int32_t prefix_items, tail_items;  // CTAs (of the streaming kernel: prefix items first)
     int32_t q_groups;       // 8-query groups of a tail item's heads
-    int32_t row_groups;     // 8-row groups of the prefix rows (streaming prefix)
+    int32_t row_groups;     // groups of the prefix rows: of 8 (streaming kernel) or kPrefixRows
 };
 
+// Query rows of an item and tokens of a tile of the tensor-core prefix kernel.
+constexpr int kPrefixRows = 128, kPrefixTile = 64;
+int prefix_ctas_per_sm(int dim);
+
+// The tensor-core kernel over the prefix items of `a`.
+cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
 // The streaming kernel over the items of `a` and the combine pass over every (sequence, head).
 cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
 cudaError_t launch_paged_combine(int dim, int dtype, const PagedArgs &a, cudaStream_t s);

@@ -306,43 +306,20 @@ __global__ void __launch_bounds__(512) combine_kernel(const PagedArgs a) {
         a.lse[int64_t(b) * a.n_q_heads + h] = l == 0.f ? -INFINITY : M * kPagedLn2 + logf(l);
 }
 
-template <class K> cudaError_t launch_pdl(K k, dim3 grid, int threads, int smem, cudaStream_t s, const PagedArgs &a) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(unsigned(threads));
-    cfg.dynamicSmemBytes = size_t(smem);
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, a);
-}
-
 template <int D, int DT> cudaError_t stream_d(const PagedArgs &a, cudaStream_t s) {
     static const cudaError_t attr = cudaFuncSetAttribute(
         stream_kernel<D, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem<D>());
     if (attr != cudaSuccess) return attr;
-    return launch_pdl(stream_kernel<D, DT>, dim3(unsigned(a.prefix_items + a.tail_items)), NW * 32, stream_smem<D>(), s, a);
+    return launch_paged(stream_kernel<D, DT>, dim3(unsigned(a.prefix_items + a.tail_items)), NW * 32, stream_smem<D>(), s, a);
 }
 
 template <int D, int DT> cudaError_t combine_d(const PagedArgs &a, cudaStream_t s) {
     // 16 warps only where a row has many parts
     const int warps = a.n_split + a.n_chunk > 16 ? 16 : 4;
-    return launch_pdl(combine_kernel<D, DT>, dim3(unsigned(a.n_q_heads), unsigned(a.batch)), 32 * warps, 0, s, a);
+    return launch_paged(combine_kernel<D, DT>, dim3(unsigned(a.n_q_heads), unsigned(a.batch)), 32 * warps, 0, s, a);
 }
 
 }  // namespace
-
-#define KVX_PAGED_DIM(fn)                                                                                  \
-    switch (dim) {                                                                                         \
-    case 32: return dtype == KVX_DTYPE_BF16 ? fn<32, KVX_DTYPE_BF16>(a, s) : fn<32, KVX_DTYPE_FP16>(a, s);    \
-    case 64: return dtype == KVX_DTYPE_BF16 ? fn<64, KVX_DTYPE_BF16>(a, s) : fn<64, KVX_DTYPE_FP16>(a, s);    \
-    case 128: return dtype == KVX_DTYPE_BF16 ? fn<128, KVX_DTYPE_BF16>(a, s) : fn<128, KVX_DTYPE_FP16>(a, s); \
-    case 256: return dtype == KVX_DTYPE_BF16 ? fn<256, KVX_DTYPE_BF16>(a, s) : fn<256, KVX_DTYPE_FP16>(a, s); \
-    default: return cudaErrorInvalidValue;                                                                 \
-    }
 
 cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, cudaStream_t s) {
     if (a.prefix_items + a.tail_items <= 0) return cudaSuccess;

@@ -64,4 +64,31 @@ __device__ __forceinline__ int tail_len(const PagedArgs &a, int b) {
     return n < 0 ? 0 : a.max_len;
 }
 
+// A launch that may be set up while the grid before it in the stream drains (programmatic dependent
+// launch; every kernel launched so waits for that grid itself).
+template <class K>
+cudaError_t launch_paged(K k, dim3 grid, int threads, int smem, cudaStream_t s, const PagedArgs &a) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(unsigned(threads));
+    cfg.dynamicSmemBytes = size_t(smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, a);
+}
+
 }  // namespace kvx
+
+// The instantiation of fn<D, type> for a head dim and type given at run time.
+#define KVX_PAGED_DIM(fn)                                                                                     \
+    switch (dim) {                                                                                            \
+    case 32: return dtype == KVX_DTYPE_BF16 ? fn<32, KVX_DTYPE_BF16>(a, s) : fn<32, KVX_DTYPE_FP16>(a, s);    \
+    case 64: return dtype == KVX_DTYPE_BF16 ? fn<64, KVX_DTYPE_BF16>(a, s) : fn<64, KVX_DTYPE_FP16>(a, s);    \
+    case 128: return dtype == KVX_DTYPE_BF16 ? fn<128, KVX_DTYPE_BF16>(a, s) : fn<128, KVX_DTYPE_FP16>(a, s); \
+    case 256: return dtype == KVX_DTYPE_BF16 ? fn<256, KVX_DTYPE_BF16>(a, s) : fn<256, KVX_DTYPE_FP16>(a, s); \
+    default: return cudaErrorInvalidValue;                                                                    \
+    }
