@@ -292,10 +292,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
         for (int i = 0; i < it.tiles && ok; ++i) {
             ok = __all_sync(FULL, wait(bar(B_S0 + (i & 1)), i >> 1));
             if (!ok) break;
-            // (phases of B_PV are taken one by one, so that its parity always tells)
-            if (i > 1) ok = __all_sync(FULL, wait(bar(B_PV), i - 2));
-            if (!ok) break;
             fence_after();
+            bool pv_seen = i == 0;  // PV(i - 1) has completed
             if (live) {
                 const uint32_t st = tm + lanes + uint32_t(D + (i & 1) * TT);
                 uint32_t x0[32], x1[32];
@@ -324,6 +322,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
                         // O is complete up to tile i - 1, and the next PV waits for this warp
                         ok = __all_sync(FULL, wait(bar(B_PV), i - 1));
                         if (!ok) break;
+                        pv_seen = true;
                         fence_after();
 #pragma unroll
                         for (int c = 0; c < D; c += 32) {
@@ -351,11 +350,15 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
                 tmem_st32(st, p);
                 tmem_wait_st();
             }
+            // B_PV is waited for once a tile, before the arrival that lets its next phase begin: a
+            // phase later its parity would not tell PV(i - 1) done from PV(i) to come
+            if (!pv_seen) ok = __all_sync(FULL, wait(bar(B_PV), i - 1));
+            if (!ok) break;
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_P0 + (i & 1)));
         }
-        for (int i = max(0, it.tiles - 2); i < it.tiles && ok; ++i) ok = __all_sync(FULL, wait(bar(B_PV), i));
+        if (ok) ok = __all_sync(FULL, wait(bar(B_PV), it.tiles - 1));
         if (ok && live) {
             // every copy and MMA of the CTA has completed: Q and the ring make room for the rows
             fence_after();
