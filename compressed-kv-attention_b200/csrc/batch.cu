@@ -15,10 +15,12 @@ struct kvx_batch_s {
     int64_t cap_rows = 0;   // partial-state rows of the scratch
     float *acc = nullptr;
     float2 *ml = nullptr;
+    int32_t *starts = nullptr;
     int *status = nullptr;
     ~kvx_batch_s() {
         cudaFree(acc);
         cudaFree(ml);
+        cudaFree(starts);
         cudaFree(status);
     }
 };
@@ -26,14 +28,6 @@ struct kvx_batch_s {
 namespace {
 
 constexpr int kMaxTokens = 1 << 30;   // of a prefix or a tail (token arithmetic in 32 bits)
-constexpr int kMaxBatch = 65535;      // grid limit of the combine pass
-
-// Items of an attention call.  About kItemsPerSm CTAs an SM keep the loads of a streaming kernel in
-// flight and even out ragged tails; an item takes at least kMinChunk tokens, below which the join
-// of its warps and the write of its partial state weigh more than its loads.
-constexpr int kItemsPerSm = 16;
-constexpr int kMinChunk = 256;
-
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
 // A batch of at most this many rows a KV head streams its prefix like a tail; more rows go through
@@ -57,16 +51,16 @@ int prefix_split_tiles(int tiles, int lists, int slots) {
     return best;
 }
 
+// CTAs of the streaming kernel that fill the device.
+int stream_ctas(const kvx_batch_s *h) { return (h->dim <= 128 ? 2 : 1) * h->sms; }
+
 // Rows of an upper bound of the scratch an attention call of `batch` sequences takes.
 int64_t scratch_rows(const kvx_batch_s *h, int batch) {
-    const int64_t qg = ceil_div(h->group, 8), rg = ceil_div(int64_t(batch) * h->group, 8);
-    const int64_t items = int64_t(kItemsPerSm) * h->sms;
-    const int64_t stream = (items + h->n_kv_heads * rg) * 8;
-    const int64_t tensor = (4 * int64_t(prefix_ctas_per_sm(h->dim)) * h->sms +
-                            h->n_kv_heads * int64_t(ceil_div(int64_t(batch) * h->group, kPrefixRows))) * kPrefixRows;
-    const int64_t prefix = std::max(stream, tensor);
-    const int64_t tails = (items / qg + 1 + int64_t(batch) * h->n_kv_heads) * h->group;
-    return prefix + tails;
+    const int64_t rows = int64_t(batch) * h->group;
+    const int64_t tensor = (4 * int64_t(prefix_ctas_per_sm(h->dim)) * h->sms + h->n_kv_heads * int64_t(ceil_div(rows, kPrefixRows))) *
+                           kPrefixRows;
+    const int64_t units = h->n_kv_heads * (int64_t(batch) * ceil_div(h->group, 8) + ceil_div(kStreamRows, 8));
+    return tensor + 8 * (int64_t(stream_ctas(h)) * kStreamWarps + units);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -153,7 +147,7 @@ bool view_ok(const kvx_view *v) { return v != nullptr && v->data != nullptr; }
 extern "C" {
 
 int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int dtype, kvx_batch *out) {
-    if (out == nullptr || max_batch <= 0 || max_batch > kMaxBatch || n_q_heads <= 0 || n_kv_heads <= 0 ||
+    if (out == nullptr || max_batch <= 0 || max_batch > kMaxStreamBatch || n_q_heads <= 0 || n_kv_heads <= 0 ||
         n_q_heads % n_kv_heads != 0 || dim <= 0 || dim % 2 != 0 || dim > kMaxHeadDim ||
         (dtype != KVX_DTYPE_BF16 && dtype != KVX_DTYPE_FP16))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_create: bad argument");
@@ -171,6 +165,7 @@ int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int 
     h->cap_rows = scratch_rows(h, max_batch);
     cudaError_t e = cudaMalloc(&h->status, 2 * sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(h->status, 0, 2 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&h->starts, (size_t(max_batch) + 1) * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMalloc(&h->acc, size_t(h->cap_rows) * dim * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&h->ml, size_t(h->cap_rows) * sizeof(float2));
     if (e != cudaSuccess) {
@@ -274,39 +269,29 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     a.acc = h->acc;
     a.ml = h->ml;
     a.status = h->status;
-    const int items = kItemsPerSm * h->sms;
+    a.starts = h->starts;
     const int rows = x->batch * h->group;
-    a.q_groups = ceil_div(h->group, 8);
     const bool tensor = paged && rows > kStreamRows;
-    a.row_groups = ceil_div(rows, tensor ? kPrefixRows : 8);
-    a.row_pad = (tensor ? kPrefixRows : 8) * a.row_groups;
     if (tensor) {
-        const int per = prefix_split_tiles(ceil_div(x->prefix_len, kPrefixTile), h->n_kv_heads * a.row_groups,
-                                           prefix_ctas_per_sm(h->dim) * h->sms);
-        a.split_tokens = per * kPrefixTile;
+        a.row_groups = ceil_div(rows, kPrefixRows);
+        a.row_pad = kPrefixRows * a.row_groups;
+        a.split_tokens = kPrefixTile * prefix_split_tiles(ceil_div(x->prefix_len, kPrefixTile), h->n_kv_heads * a.row_groups,
+                                                          prefix_ctas_per_sm(h->dim) * h->sms);
         a.n_split = ceil_div(x->prefix_len, a.split_tokens);
-        a.prefix_items = h->n_kv_heads * a.n_split * a.row_groups;
-    } else if (paged) {
-        const int most = std::max(1, items / (h->n_kv_heads * a.row_groups));
-        a.split_tokens = std::max(kMinChunk, ceil_div(ceil_div(x->prefix_len, most), 128) * 128);
-        a.n_split = ceil_div(x->prefix_len, a.split_tokens);
-        a.prefix_items = h->n_kv_heads * a.n_split * a.row_groups;
+        a.stream_base = int64_t(h->n_kv_heads) * a.n_split * a.row_pad;
     }
-    a.tail_base = int64_t(h->n_kv_heads) * a.n_split * a.row_pad;
-    if (x->max_len > 0) {
-        const int most = std::max(1, items / (x->batch * h->n_kv_heads * a.q_groups));
-        a.chunk_tokens = std::max(kMinChunk, ceil_div(ceil_div(x->max_len, most), 128) * 128);
-        a.n_chunk = ceil_div(x->max_len, a.chunk_tokens);
-        a.tail_items = x->batch * h->n_kv_heads * a.n_chunk * a.q_groups;
-    }
-    const int64_t used = a.tail_base + int64_t(x->batch) * h->n_kv_heads * a.n_chunk * h->group;
+    a.tail_groups = ceil_div(h->group, 8);
+    a.pre_groups = ceil_div(rows, 8);
+    if (paged && !tensor) a.stream_prefix = h->n_kv_heads * a.pre_groups;
+    const int64_t units = a.stream_prefix + int64_t(x->batch) * h->n_kv_heads * a.tail_groups;
+    const int64_t most_tiles = int64_t(a.stream_prefix) * ceil_div(x->prefix_len, kStreamTile) +
+                               int64_t(x->batch) * h->n_kv_heads * a.tail_groups * ceil_div(x->max_len, kStreamTile);
+    a.stream_ctas = int(std::min<int64_t>(stream_ctas(h), ceil_div(most_tiles, kStreamLeast * kStreamWarps)));
+    const int64_t used = a.stream_base + (a.stream_ctas > 0 ? 8 * (int64_t(a.stream_ctas) * kStreamWarps + units) : 0);
     if (used > h->cap_rows) return fail(KVX_ERR_RUNTIME, "kvx_batch_attend: scratch too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (tensor) {
-        KVX_CUDA(launch_paged_prefix(h->dim, h->dtype, a, s));
-        a.prefix_items = 0;
-    }
-    KVX_CUDA(launch_paged_stream(h->dim, h->dtype, a, s));
+    if (tensor) KVX_CUDA(launch_paged_prefix(h->dim, h->dtype, a, s));
+    KVX_CUDA(launch_paged_stream(h->dim, h->dtype, a, tensor, s));
     KVX_CUDA(launch_paged_combine(h->dim, h->dtype, a, s));
     return KVX_OK;
 }

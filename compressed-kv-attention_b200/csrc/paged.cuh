@@ -70,21 +70,38 @@ struct PagedArgs {
     int32_t prefix_len, max_len;
     int32_t batch, n_q_heads, n_kv_heads, group;
     float scale_log2;       // scale * log2(e)
-    // partial states: row r has dim accumulators at acc + r * dim and {m (log2 units), l} at ml[r]
+    int *status;
+    // Partial states: row r has dim accumulators at acc + r * dim and {m (log2 units), l} at ml[r].
     float *acc;
     float2 *ml;
-    int *status;
-    // prefix parts: row ((kv head * n_split + split) * row_pad + (sequence * group + g));
-    // n_split parts per row, each `split_tokens` tokens but the last
-    int32_t n_split, row_pad;
-    int32_t split_tokens;
-    // tail parts: row tail_base + ((sequence * kv heads + kv head) * n_chunk + chunk) * group + g
-    int64_t tail_base;
-    int32_t n_chunk, chunk_tokens;
-    int32_t prefix_items, tail_items;  // CTAs (of the streaming kernel: prefix items first)
-    int32_t q_groups;       // 8-query groups of a tail item's heads
-    int32_t row_groups;     // groups of the prefix rows: of 8 (streaming kernel) or kPrefixRows
+    // Tensor-core prefix parts: row ((kv head * n_split + split) * row_pad + row), n_split parts of
+    // split_tokens tokens (the last fewer) for each of the head's batch * group rows, in row_groups
+    // items of kPrefixRows rows.
+    int32_t n_split, row_pad, split_tokens, row_groups;
+    // Streamed units, laid end to end in 16-token tiles: first (a streamed prefix) KV head by KV
+    // head and group of 8 rows, prefix_len tokens each; then sequence by sequence, KV head by KV
+    // head, group of 8 heads by group, the sequence's own tokens.  The tiles are cut into as many
+    // equal runs as there are workers (warps), so worker w has tiles [w T / n, (w + 1) T / n); the
+    // part it leaves of unit u is in rows stream_base + 8 (w + u) .., which no other pair has (w + u
+    // grows along the line).
+    int64_t stream_base;
+    int32_t stream_prefix;  // units of a streamed prefix (0: the prefix is not streamed)
+    int32_t pre_groups;     // its groups of 8 rows
+    int32_t tail_groups;    // groups of 8 heads of a KV head
+    int32_t stream_ctas;    // of kStreamWarps workers
+    int32_t *starts;        // [batch + 1] tiles of the sequences before each, written for the combine
 };
+
+constexpr int kStreamWarps = 8;   // workers a CTA
+constexpr int kStreamTile = 16;   // tokens
+constexpr int kStreamLeast = 4;   // tiles a worker takes at least
+constexpr int kMaxStreamBatch = 4096;
+
+// Workers that share `tiles` tiles out of those launched.
+__device__ __forceinline__ int stream_workers(const PagedArgs &a, int64_t tiles) {
+    const int64_t n = (tiles + kStreamLeast - 1) / kStreamLeast, most = int64_t(a.stream_ctas) * kStreamWarps;
+    return int(n < most ? n : most);
+}
 
 // Query rows of an item and tokens of a tile of the tensor-core prefix kernel.
 constexpr int kPrefixRows = 128, kPrefixTile = 64;
@@ -92,8 +109,9 @@ int prefix_ctas_per_sm(int dim);
 
 // The tensor-core kernel over the prefix items of `a`.
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
-// The streaming kernel over the items of `a` and the combine pass over every (sequence, head).
-cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
+// The streaming kernel over the units of `a` and the combine pass over every (sequence, head).
+// beside: the launch before it on the stream is the same call's prefix kernel, which it may run beside.
+cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, bool beside, cudaStream_t s);
 cudaError_t launch_paged_combine(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
 
 }  // namespace kvx

@@ -1,10 +1,11 @@
 // paged_stream.cu -- single-token attention over paged keys and values, up to 8 query rows at a
 // time, and the combine pass that folds every row's partial states.
 //
-// One CTA takes one item: up to 8 query rows and a run of tokens of one KV head, either a chunk of
-// one sequence's own pages or (batches of few rows) a piece of the shared prefix.  Its 8 warps take
-// the run's 16-token tiles in turn, each with its own online softmax, and join their states in
-// shared memory; the CTA leaves one partial state per row.
+// A unit is up to 8 query rows and the tokens they share: the own pages of one sequence under one KV
+// head or (batches of few rows) the shared prefix.  All units' 16-token tiles form one line, cut
+// into equal runs, one for each warp of the grid, whatever the lengths are: a warp walks its run
+// with an online softmax of its own and leaves one partial state per row for each unit it met.  No
+// warp waits for another.
 //
 // The work is 4 bytes and 2 rows FMAs per K and V element, so it is bound by HBM; everything is
 // arranged to keep loads in flight and nothing else in the way.  K and V go from global memory to
@@ -22,7 +23,8 @@ namespace kvx {
 namespace {
 
 constexpr uint32_t FULL = 0xFFFFFFFFu;
-constexpr int NW = 8;  // warps per CTA
+constexpr int NW = kStreamWarps;
+constexpr int TT = kStreamTile;
 
 template <int DT>
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -52,277 +54,381 @@ __device__ __forceinline__ uint2 load8(const uint16_t *p) {
     return v;
 }
 
-// An item: query rows and a run of tokens.
-struct Item {
+__device__ __forceinline__ int tiles_of(int tokens) { return (tokens + TT - 1) / TT; }
+
+// A worker's stretch of one unit.
+struct Unit {
     const int32_t *table;
-    int64_t row0;       // first partial row
-    int t0, t1;         // tokens
-    int first, n;       // rows first .. first + n - 1 of the head's (sequence, g) list
+    int64_t end;        // tile of the line after the unit's last
+    int tokens;         // of the unit
+    int skip;           // its tiles before the stretch
+    int first, n;       // query rows first .. first + n - 1 of the head's (sequence, g) list
     int head;           // KV head
+    int index;          // in the line
 };
 
-__device__ __forceinline__ bool item_of(const PagedArgs &a, int i, Item &x) {
-    if (i < a.prefix_items) {
-        const int rg = i % a.row_groups;
-        i /= a.row_groups;
-        const int s = i % a.n_split;
-        x.head = i / a.n_split;
-        x.table = a.prefix_table;
-        x.t0 = s * a.split_tokens;
-        x.t1 = min(a.prefix_len, x.t0 + a.split_tokens);
-        x.first = 8 * rg;
-        x.n = min(8, a.batch * a.group - x.first);
-        x.row0 = int64_t(x.head * a.n_split + s) * a.row_pad + x.first;
-        return true;
+// The unit that tile f of the line belongs to.  starts[b]: tiles of one (head, group) of the
+// sequences before b.
+__device__ __forceinline__ Unit unit_at(const PagedArgs &a, const int32_t *starts, int64_t f) {
+    Unit u;
+    const int pt = tiles_of(a.prefix_len);
+    const int64_t pre = int64_t(a.stream_prefix) * pt;
+    if (f < pre) {
+        u.index = int(f / pt);
+        u.skip = int(f - int64_t(u.index) * pt);
+        u.end = int64_t(u.index + 1) * pt;
+        u.head = u.index / a.pre_groups;
+        u.first = 8 * (u.index - u.head * a.pre_groups);
+        u.n = min(8, a.batch * a.group - u.first);
+        u.tokens = a.prefix_len;
+        u.table = a.prefix_table;
+        return u;
     }
-    i -= a.prefix_items;
-    const int qg = i % a.q_groups;
-    i /= a.q_groups;
-    const int c = i % a.n_chunk;
-    i /= a.n_chunk;
-    x.head = i % a.n_kv_heads;
-    const int b = i / a.n_kv_heads;
-    x.t0 = c * a.chunk_tokens;
-    x.t1 = min(tail_len(a, b), x.t0 + a.chunk_tokens);
-    x.table = a.table + int64_t(b) * a.table_stride;
-    x.first = b * a.group + 8 * qg;
-    x.n = min(8, a.group - 8 * qg);
-    x.row0 = a.tail_base + (int64_t(b * a.n_kv_heads + x.head) * a.n_chunk + c) * a.group + 8 * qg;
-    return x.t0 < x.t1;  // a chunk past the sequence's end has no state; the combine does not look
+    f -= pre;
+    const int per = a.n_kv_heads * a.tail_groups;
+    int lo = 0, hi = a.batch;  // starts[lo] * per <= f < starts[hi] * per
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (int64_t(starts[mid]) * per <= f) lo = mid;
+        else hi = mid;
+    }
+    const int n = starts[lo + 1] - starts[lo];  // > 0: starts[lo + 1] * per > f
+    const int64_t at = f - int64_t(starts[lo]) * per;
+    const int k = int(at / n);
+    u.skip = int(at - int64_t(k) * n);
+    u.end = pre + int64_t(starts[lo]) * per + int64_t(k + 1) * n;
+    u.head = k / a.tail_groups;
+    const int qg = k - u.head * a.tail_groups;
+    u.first = lo * a.group + 8 * qg;
+    u.n = min(8, a.group - 8 * qg);
+    u.tokens = tail_len(a, lo);
+    u.table = a.table + int64_t(lo) * a.table_stride;
+    u.index = a.stream_prefix + lo * per + k;
+    return u;
 }
 
-template <int D> constexpr int stream_smem() { return NW * 8 * D * 4; }
-
-template <int D, int DT>
-__global__ void __launch_bounds__(NW * 32, D <= 128 ? 2 : 1) stream_kernel(const PagedArgs a) {
-    constexpr int KJ = D / 32;                 // 32-dim pieces of a K row
-    constexpr int VI = D >= 64 ? D / 64 : 1;   // pieces of a V row
-    constexpr int VW = D >= 64 ? 4 : 2;        // words a lane loads of each
-    extern __shared__ float sacc[];            // [NW][8][D]
-    __shared__ float2 sml[NW][8];
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    Item it;
-    if (!item_of(a, int(blockIdx.x), it)) return;
+// starts[b], b = 0 .. batch, from the lengths (every thread of the CTA).
+__device__ __forceinline__ void scan_starts(const PagedArgs &a, int32_t *starts) {
+    __shared__ int32_t part[NW];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = lane >> 2, t = lane & 3;
-
-    // Q rows as A fragments
-    uint4 qf[KJ];
-    {
-        const int r = it.first + (g < it.n ? g : 0), b = r / a.group;
-        const uint16_t *q = a.q + int64_t(b) * a.q_token + int64_t(it.head * a.group + r - b * a.group) * a.q_head + 8 * t;
+    int32_t base = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += NW * 32) {
+        const int b = b0 + int(threadIdx.x);
+        const int n = b < a.batch && a.max_len > 0 ? tiles_of(tail_len(a, b)) : 0;
+        int s = n;
 #pragma unroll
-        for (int j = 0; j < KJ; ++j) qf[j] = g < it.n ? load16(q + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
-    }
-    const uint16_t *kb = a.pool.k + int64_t(it.head) * a.pool.head_stride + 8 * t;
-    const uint16_t *vb = a.pool.v + int64_t(it.head) * a.pool.head_stride + 2 * VW * g;
-
-    float acc[VI * VW][4];
-#pragma unroll
-    for (int i = 0; i < VI * VW; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    float m = -INFINITY, l = 0.f;
-
-    // lanes 0-15 look up the rows of the next tile's tokens, a tile ahead (-1: no such token)
-    auto rows_of = [&](int tile) -> int64_t {
-        const int tok = tile + (lane & 15);
-        return tile < it.t1 && tok < it.t1 ? page_row(a.pool, it.table, tok, a.status) : -1;
-    };
-    int64_t nxt = rows_of(it.t0 + 16 * warp);
-    for (int tile = it.t0 + 16 * warp; tile < it.t1; tile += 16 * NW) {
-        const int64_t row = nxt;
-        uint4 kf[2][KJ];
-        bool live[2][2];  // tokens 8 n + 2 t, 8 n + 2 t + 1
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int64_t r = __shfl_sync(FULL, row, 8 * n + g);
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) kf[n][j] = r >= 0 ? load16(kb + r + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(FULL, s, o);
+            if (lane >= o) s += v;
         }
-        uint32_t vf[4][VI][VW];
-        auto load_v = [&]() {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int64_t r = __shfl_sync(FULL, row, 2 * t + (k & 1) + 8 * (k >> 1));
-                live[k >> 1][k & 1] = r >= 0;
-#pragma unroll
-                for (int i = 0; i < VI; ++i) {
-                    if constexpr (VW == 4) {
-                        const uint4 v = r >= 0 ? load16(vb + r + 64 * i) : make_uint4(0u, 0u, 0u, 0u);
-                        vf[k][i][0] = v.x, vf[k][i][1] = v.y, vf[k][i][2] = v.z, vf[k][i][3] = v.w;
-                    } else {
-                        const uint2 v = r >= 0 ? load8(vb + r) : make_uint2(0u, 0u);
-                        vf[k][i][0] = v.x, vf[k][i][1] = v.y;
-                    }
-                }
-            }
-        };
-        if constexpr (D <= 128) load_v();  // (at 256 the registers hold one of K and V at a time)
-        nxt = rows_of(tile + 16 * NW);
-
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < KJ; ++j) {
-                mma16<DT>(s[n], qf[j].x, 0u, qf[j].y, 0u, kf[n][j].x, kf[n][j].y);
-                mma16<DT>(s[n], qf[j].z, 0u, qf[j].w, 0u, kf[n][j].z, kf[n][j].w);
-            }
-        }
-        if constexpr (D > 128) load_v();
-        // online softmax of query g: this lane has 4 of the 16 tokens
-        float x[2][2];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) x[n][e] = live[n][e] ? s[n][e] * a.scale_log2 : -INFINITY;
-        float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-        if (__any_sync(FULL, mx > m)) {
-            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
-            const float mn = fmaxf(m, mx);
-            const float al = mn == -INFINITY ? 1.f : exp2_sfu(m - mn);
-            m = mn;
-            l *= al;
-            const float al0 = __shfl_sync(FULL, al, 8 * t), al1 = __shfl_sync(FULL, al, 8 * t + 4);
-#pragma unroll
-            for (int i = 0; i < VI * VW; ++i) acc[i][0] *= al0, acc[i][1] *= al1, acc[i][2] *= al0, acc[i][3] *= al1;
-        }
-        const float mu = m == -INFINITY ? 0.f : m - Elem<DT>::kBias;
-        float p[2][2];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) p[n][e] = exp2_sfu(x[n][e] - mu), l += p[n][e];
-        const uint32_t b0 = Elem<DT>::pack(p[0][0], p[0][1]), b1 = Elem<DT>::pack(p[1][0], p[1][1]);
-#pragma unroll
-        for (int i = 0; i < VI; ++i)
-#pragma unroll
-            for (int w = 0; w < VW; ++w)
-                mma16<DT>(acc[i * VW + w], prmt(vf[0][i][w], vf[1][i][w], 0x5410u), prmt(vf[0][i][w], vf[1][i][w], 0x7632u),
-                          prmt(vf[2][i][w], vf[3][i][w], 0x5410u), prmt(vf[2][i][w], vf[3][i][w], 0x7632u), b0, b1);
-    }
-
-    // join the warps' states
-    l += __shfl_xor_sync(FULL, l, 1);
-    l += __shfl_xor_sync(FULL, l, 2);
-    if (t == 0) sml[warp][g] = make_float2(m, l);
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, sml[w][g].x);
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const float2 z = sml[w][g];
-        L += z.x == -INFINITY ? z.y * 0.f : z.y * exp2_sfu(z.x - M);  // (l is 0, or NaN, without a maximum)
-    }
-    const float f = m == -INFINITY ? 0.f : exp2_sfu(m - M);
-    const float f0 = __shfl_sync(FULL, f, 8 * t), f1 = __shfl_sync(FULL, f, 8 * t + 4);
-#pragma unroll
-    for (int i = 0; i < VI; ++i)
-#pragma unroll
-        for (int w = 0; w < VW; ++w) {
-            const float(&c)[4] = acc[i * VW + w];
-            const int d = 64 * i + 2 * VW * g + 2 * w;
-            float *o = sacc + (warp * 8 + 2 * t) * D + d;
-            *reinterpret_cast<float2 *>(o) = make_float2(c[0] * f0, c[2] * f0);
-            *reinterpret_cast<float2 *>(o + D) = make_float2(c[1] * f1, c[3] * f1);
-        }
-    __syncthreads();
-    if (warp == 0 && t == 0 && g < it.n)
-        a.ml[it.row0 + g] = make_float2(M == -INFINITY ? M : M - Elem<DT>::kBias, L);
-    for (int i = threadIdx.x; i < it.n * (D / 4); i += NW * 32) {
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (lane == 31) part[warp] = s;
+        __syncthreads();
+        int before = base, all = 0;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            const float4 u = reinterpret_cast<const float4 *>(sacc + w * 8 * D)[i];
-            v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+            if (w < warp) before += part[w];
+            all += part[w];
         }
-        reinterpret_cast<float4 *>(a.acc + it.row0 * D)[i] = v;
+        if (b < a.batch) starts[b] = before + s - n;
+        base += all;
+        __syncthreads();
     }
+    if (threadIdx.x == 0) starts[a.batch] = base;
+    __syncthreads();
+}
+
+template <int D> struct Cfg {
+    static constexpr int KJ = D / 32;                 // 32-dim pieces of a K row
+    static constexpr int VI = D >= 64 ? D / 64 : 1;   // pieces of a V row
+    static constexpr int VW = D >= 64 ? 4 : 2;        // words a lane loads of each
+    static constexpr int NT = D <= 64 ? 128 / D : 1;  // tiles taken together: 8 KB in flight a warp
+    static constexpr int CTAS = D <= 128 ? 2 : 1;
+};
+
+// BESIDE: launched behind the same call's prefix kernel, beside which it may run: that kernel's CTAs
+// let it start once everything before them on the stream is complete, and it waits for them at its
+// end, so that the combine pass, which waits for this grid, has both.
+template <int D, int DT, bool BESIDE>
+__global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const PagedArgs a) {
+    using C = Cfg<D>;
+    constexpr int KJ = C::KJ, VI = C::VI, VW = C::VW, NT = C::NT;
+    extern __shared__ int32_t starts[];
+    if constexpr (!BESIDE) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    scan_starts(a, starts);
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= a.batch; b += NW * 32) a.starts[b] = starts[b];
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int worker = int(blockIdx.x) * NW + int(threadIdx.x >> 5);
+    const int64_t total = int64_t(a.stream_prefix) * tiles_of(a.prefix_len) +
+                          int64_t(starts[a.batch]) * a.n_kv_heads * a.tail_groups;
+    const int workers = stream_workers(a, total);
+    int64_t f = worker < workers ? worker * total / workers : 0;
+    const int64_t f_end = worker < workers ? (worker + 1) * total / workers : 0;
+    while (f < f_end) {
+        const Unit u = unit_at(a, starts, f);
+        const int t0 = u.skip * TT;
+        const int t1 = min(u.tokens, t0 + int(min(u.end, f_end) - f) * TT);
+        f = u.end;
+
+        // Q rows as A fragments
+        uint4 qf[KJ];
+        {
+            const int r = u.first + (g < u.n ? g : 0), b = r / a.group;
+            const uint16_t *q = a.q + int64_t(b) * a.q_token + int64_t(u.head * a.group + r - b * a.group) * a.q_head + 8 * t;
+#pragma unroll
+            for (int j = 0; j < KJ; ++j) qf[j] = g < u.n ? load16(q + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        const uint16_t *kb = a.pool.k + int64_t(u.head) * a.pool.head_stride + 8 * t;
+        const uint16_t *vb = a.pool.v + int64_t(u.head) * a.pool.head_stride + 2 * VW * g;
+        float acc[VI * VW][4];
+#pragma unroll
+        for (int i = 0; i < VI * VW; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+        float m = -INFINITY, l = 0.f;
+
+        // the lanes look up the rows of the next tiles' tokens ahead of their use (-1: no such token)
+        constexpr int LOOK = NT * TT > 32 ? 2 : 1;
+        int64_t nxt[LOOK];
+        auto look_up = [&](int tok0) {
+#pragma unroll
+            for (int i = 0; i < LOOK; ++i) {
+                const int tok = tok0 + 32 * i + (NT * TT >= 32 ? lane : lane & 15);
+                nxt[i] = tok < t1 ? page_row(a.pool, u.table, tok, a.status) : -1;
+            }
+        };
+        look_up(t0);
+        for (int tok = t0; tok < t1; tok += NT * TT) {
+            int64_t row[LOOK];
+#pragma unroll
+            for (int i = 0; i < LOOK; ++i) row[i] = nxt[i];
+            uint4 kf[NT][2][KJ];
+            uint32_t vf[NT][4][VI][VW];
+            bool live[NT][2][2];  // tokens 8 n + 2 t, 8 n + 2 t + 1
+            auto load_k = [&]() {
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        const int64_t r = __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 8 * n + g);
+#pragma unroll
+                        for (int j = 0; j < KJ; ++j) kf[k][n][j] = r >= 0 ? load16(kb + r + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+            };
+            auto load_v = [&]() {
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int64_t r = __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 2 * t + (e & 1) + 8 * (e >> 1));
+                        live[k][e >> 1][e & 1] = r >= 0;
+#pragma unroll
+                        for (int i = 0; i < VI; ++i) {
+                            if constexpr (VW == 4) {
+                                const uint4 v = r >= 0 ? load16(vb + r + 64 * i) : make_uint4(0u, 0u, 0u, 0u);
+                                vf[k][e][i][0] = v.x, vf[k][e][i][1] = v.y, vf[k][e][i][2] = v.z, vf[k][e][i][3] = v.w;
+                            } else {
+                                const uint2 v = r >= 0 ? load8(vb + r) : make_uint2(0u, 0u);
+                                vf[k][e][i][0] = v.x, vf[k][e][i][1] = v.y;
+                            }
+                        }
+                    }
+            };
+            load_k();
+            if constexpr (D <= 128) load_v();  // (at 256 the registers hold one of K and V at a time)
+            look_up(tok + NT * TT);
+
+            float s[NT][2][4];
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    s[k][n][0] = s[k][n][1] = s[k][n][2] = s[k][n][3] = 0.f;
+#pragma unroll
+                    for (int j = 0; j < KJ; ++j) {
+                        mma16<DT>(s[k][n], qf[j].x, 0u, qf[j].y, 0u, kf[k][n][j].x, kf[k][n][j].y);
+                        mma16<DT>(s[k][n], qf[j].z, 0u, qf[j].w, 0u, kf[k][n][j].z, kf[k][n][j].w);
+                    }
+                }
+            if constexpr (D > 128) load_v();
+            // online softmax of query g: this lane has 4 of each tile's 16 tokens
+            float mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        s[k][n][e] = live[k][n][e] ? s[k][n][e] * a.scale_log2 : -INFINITY;
+                        mx = fmaxf(mx, s[k][n][e]);
+                    }
+            if (__any_sync(FULL, mx > m)) {
+                mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
+                const float mn = fmaxf(m, mx);
+                const float al = mn == -INFINITY ? 1.f : exp2_sfu(m - mn);
+                m = mn;
+                l *= al;
+                const float al0 = __shfl_sync(FULL, al, 8 * t), al1 = __shfl_sync(FULL, al, 8 * t + 4);
+#pragma unroll
+                for (int i = 0; i < VI * VW; ++i) acc[i][0] *= al0, acc[i][1] *= al1, acc[i][2] *= al0, acc[i][3] *= al1;
+            }
+            const float mu = m == -INFINITY ? 0.f : m - Elem<DT>::kBias;
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                uint32_t b[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const float p0 = exp2_sfu(s[k][n][0] - mu), p1 = exp2_sfu(s[k][n][1] - mu);
+                    l += p0 + p1;
+                    b[n] = Elem<DT>::pack(p0, p1);
+                }
+#pragma unroll
+                for (int i = 0; i < VI; ++i)
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        const uint32_t(&v)[4][VI][VW] = vf[k];
+                        mma16<DT>(acc[i * VW + w], prmt(v[0][i][w], v[1][i][w], 0x5410u), prmt(v[0][i][w], v[1][i][w], 0x7632u),
+                                  prmt(v[2][i][w], v[3][i][w], 0x5410u), prmt(v[2][i][w], v[3][i][w], 0x7632u), b[0], b[1]);
+                    }
+            }
+        }
+
+        // the part's state
+        l += __shfl_xor_sync(FULL, l, 1);
+        l += __shfl_xor_sync(FULL, l, 2);
+        const int64_t out = a.stream_base + 8 * int64_t(worker + u.index);
+        if (t == 0 && g < u.n) a.ml[out + g] = make_float2(m == -INFINITY ? m : m - Elem<DT>::kBias, l);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (2 * t + e >= u.n) continue;
+            float *o = a.acc + (out + 2 * t + e) * D + 2 * VW * g;
+#pragma unroll
+            for (int i = 0; i < VI; ++i)
+#pragma unroll
+                for (int w = 0; w < VW; w += 2)
+                    *reinterpret_cast<float4 *>(o + 64 * i + 2 * w) =
+                        make_float4(acc[i * VW + w][e], acc[i * VW + w][2 + e], acc[i * VW + w + 1][e], acc[i * VW + w + 1][2 + e]);
+        }
+    }
+    if constexpr (BESIDE) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Folds the partial states of one (sequence, head): M = max m_i, l = sum l_i 2^(m_i - M), out =
-// (sum acc_i 2^(m_i - M)) / l.  One CTA per row, its warps take the parts in turn; sums run in a
-// fixed order.
+// (sum acc_i 2^(m_i - M)) / l.  One CTA per row; its warps take the parts in turn, each with a
+// running maximum, so that no load waits for another's value; sums run in a fixed order.
+constexpr int kCombineWarps = 8;
 template <int D, int DT>
-__global__ void __launch_bounds__(512) combine_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const PagedArgs a) {
     constexpr int V = D / 32;  // values per lane
-    __shared__ float sacc[16][D];
-    __shared__ float sl[16];
+    __shared__ float sacc[kCombineWarps][D];
+    __shared__ float2 sml[kCombineWarps];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int b = blockIdx.y, h = blockIdx.x, head = h / a.group, gi = h - head * a.group;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    const int np = a.n_split;
-    const int nt = a.n_chunk > 0 ? (tail_len(a, b) + a.chunk_tokens - 1) / a.chunk_tokens : 0;
-    const int64_t prow = int64_t(head) * a.n_split * a.row_pad + b * a.group + gi;
-    const int64_t trow = a.tail_base + int64_t(b * a.n_kv_heads + head) * a.n_chunk * a.group + gi;
-    auto row = [&](int i) -> int64_t {
-        return i < np ? prow + int64_t(i) * a.row_pad : trow + int64_t(i - np) * a.group;
-    };
-    float M = -INFINITY;
-    for (int i = lane; i < np + nt; i += 32) M = fmaxf(M, a.ml[row(i)].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, o));
-    float o[V], l = 0.f;
+    // the row's parts: of the prefix (np, from row prow, pstep apart), then of its own tokens (ns)
+    const int row = b * a.group + gi;
+    int np = a.n_split, ns = 0;
+    int64_t prow = int64_t(head) * a.n_split * a.row_pad + row, pstep = a.row_pad, srow = 0;
+    if (a.stream_ctas > 0) {
+        const int64_t pt = tiles_of(a.prefix_len), pre = a.stream_prefix * pt;
+        const int per = a.n_kv_heads * a.tail_groups;
+        const int64_t total = pre + int64_t(a.starts[a.batch]) * per;
+        const int workers = stream_workers(a, total);
+        // the workers that met tiles [f, f + n) of the line, and the first one's row of unit u;
+        // worker_of(f) = the largest w with floor(w total / workers) <= f
+        auto worker_of = [&](int64_t f) { return int(((f + 1) * workers - 1) / total); };
+        auto parts = [&](int64_t f, int64_t n, int u, int64_t &first) {
+            const int w = worker_of(f);
+            first = a.stream_base + 8 * int64_t(w + u);
+            return worker_of(f + n - 1) - w + 1;
+        };
+        if (a.stream_prefix > 0) {
+            const int u = head * a.pre_groups + (row >> 3);
+            np = parts(u * pt, pt, u, prow);
+            prow += row & 7;
+            pstep = 8;
+        }
+        const int n = a.starts[b + 1] - a.starts[b], k = head * a.tail_groups + (gi >> 3);
+        if (n > 0) {
+            ns = parts(pre + int64_t(a.starts[b]) * per + int64_t(k) * n, n, a.stream_prefix + b * per + k, srow);
+            srow += gi & 7;
+        }
+    }
+    float m = -INFINITY, l = 0.f, o[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) o[j] = 0.f;
 #pragma unroll 4
-    for (int i = warp; i < np + nt; i += nw) {
-        const int64_t r = row(i);
+    for (int i = warp; i < np + ns; i += nw) {
+        const int64_t r = i < np ? prow + i * pstep : srow + 8 * int64_t(i - np);
         const float2 z = a.ml[r];
-        const float w = z.x == -INFINITY ? 0.f : exp2_sfu(z.x - M);
-        l += z.y * w;
         const float *p = a.acc + r * D + V * lane;
-        if (z.x != -INFINITY || z.y != z.y) {
-            if constexpr (V == 1) o[0] += w * p[0];
-            else if constexpr (V == 2) {
-                const float2 u = *reinterpret_cast<const float2 *>(p);
-                o[0] += w * u.x, o[1] += w * u.y;
-            } else {
+        float v[V];
+        if constexpr (V == 1) v[0] = p[0];
+        else if constexpr (V == 2) {
+            const float2 x = *reinterpret_cast<const float2 *>(p);
+            v[0] = x.x, v[1] = x.y;
+        } else {
 #pragma unroll
-                for (int j = 0; j < V; j += 4) {
-                    const float4 u = *reinterpret_cast<const float4 *>(p + j);
-                    o[j] += w * u.x, o[j + 1] += w * u.y, o[j + 2] += w * u.z, o[j + 3] += w * u.w;
-                }
+            for (int j = 0; j < V; j += 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(p + j);
+                v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
             }
         }
+        const float mn = fmaxf(m, z.x);
+        // (a part without a maximum has l = 0, or NaN, which stays)
+        const float e = mn == -INFINITY ? 1.f : exp2_sfu(m - mn), w = z.x == -INFINITY ? 0.f : exp2_sfu(z.x - mn);
+        m = mn;
+        l = l * e + z.y * w;
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = o[j] * e + (z.x == -INFINITY ? 0.f : w * v[j]);
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) sacc[warp][V * lane + j] = o[j];
-    if (lane == 0) sl[warp] = l;
+    if (lane == 0) sml[warp] = make_float2(m, l);
     __syncthreads();
+    float M = -INFINITY;
+    for (int w = 0; w < nw; ++w) M = fmaxf(M, sml[w].x);
     l = 0.f;
-    for (int w = 0; w < nw; ++w) l += sl[w];
+    float f[kCombineWarps];
+#pragma unroll
+    for (int w = 0; w < kCombineWarps; ++w) {
+        if (w >= nw) break;
+        const float2 z = sml[w];
+        f[w] = z.x == -INFINITY ? 0.f : exp2_sfu(z.x - M);
+        l += z.y * f[w];
+    }
     uint16_t *out = a.out + int64_t(b) * a.out_token + int64_t(h) * a.out_head;
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
         float v = 0.f;
-        for (int w = 0; w < nw; ++w) v += sacc[w][d];
+#pragma unroll
+        for (int w = 0; w < kCombineWarps; ++w)
+            if (w < nw) v += sacc[w][d] * f[w];
         out[d] = Elem<DT>::one(l == 0.f ? 0.f : v / l);
     }
     if (threadIdx.x == 0 && a.lse != nullptr)
         a.lse[int64_t(b) * a.n_q_heads + h] = l == 0.f ? -INFINITY : M * kPagedLn2 + logf(l);
 }
 
-template <int D, int DT> cudaError_t stream_d(const PagedArgs &a, cudaStream_t s) {
-    static const cudaError_t attr = cudaFuncSetAttribute(
-        stream_kernel<D, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, stream_smem<D>());
-    if (attr != cudaSuccess) return attr;
-    return launch_paged(stream_kernel<D, DT>, dim3(unsigned(a.prefix_items + a.tail_items)), NW * 32, stream_smem<D>(), s, a);
+template <int D, int DT, bool BESIDE> cudaError_t stream_launch(const PagedArgs &a, cudaStream_t s) {
+    return launch_paged(stream_kernel<D, DT, BESIDE>, dim3(unsigned(a.stream_ctas)), NW * 32, 4 * (a.batch + 1), s, a);
 }
+template <int D, int DT> cudaError_t stream_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, false>(a, s); }
+template <int D, int DT> cudaError_t beside_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, true>(a, s); }
 
 template <int D, int DT> cudaError_t combine_d(const PagedArgs &a, cudaStream_t s) {
-    // 16 warps only where a row has many parts
-    const int warps = a.n_split + a.n_chunk > 16 ? 16 : 4;
-    return launch_paged(combine_kernel<D, DT>, dim3(unsigned(a.n_q_heads), unsigned(a.batch)), 32 * warps, 0, s, a);
+    // about this many parts a row: more warps where each would take several in turn
+    const int units = a.stream_prefix + a.batch * a.n_kv_heads * a.tail_groups;
+    const int parts = a.n_split + a.stream_ctas * NW / units;
+    return launch_paged(combine_kernel<D, DT>, dim3(unsigned(a.n_q_heads), unsigned(a.batch)),
+                        32 * (parts > 16 ? kCombineWarps : 4), 0, s, a);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, cudaStream_t s) {
-    if (a.prefix_items + a.tail_items <= 0) return cudaSuccess;
+cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, bool beside, cudaStream_t s) {
+    if (a.stream_ctas <= 0) return cudaSuccess;
+    if (beside) KVX_PAGED_DIM(beside_d)
     KVX_PAGED_DIM(stream_d)
 }
 

@@ -197,31 +197,42 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
 
     if (warp >= SW && warp < SW + LW) {
         // ---- loads ----
-        const int tid = threadIdx.x - 32 * SW;
-        constexpr int CH = D / 8, STEPS = (TT * CH + 32 * LW - 1) / (32 * LW);
-        const int64_t head = int64_t(it.head) * a.pool.head_stride;
-        bool ok = true;
-        int q = 0;
+        // Loader warp w copies rows w, w + LW, ... of every tile: lane k holds the offset of row w +
+        // LW k (-1: no such token), looked up a tile ahead of its use.
+        constexpr int CH = D / 8, RPS = 32 / CH;              // pieces a row, rows a step
+        constexpr int MINE = (TT + LW - 1) / LW, STEPS = (MINE + RPS - 1) / RPS;
+        const int w = warp - SW, c = lane % CH;
+        const int64_t head = int64_t(it.head) * a.pool.head_stride + 8 * c;
+        auto look_up = [&](int tile) -> int64_t {
+            const int r = w + LW * lane, tok = it.t0 + tile * TT + r;
+            return r < TT && tok < it.t1 ? page_row(a.pool, a.prefix_table, tok, a.status) : -1;
+        };
         auto announce = [&](int i) {
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(full(i));
         };
-        for (; q < 2 * it.tiles && ok; ++q) {
-            // tile of ring item q, and which of K and V
-            const bool is_v = q == 2 * it.tiles - 1 || (q > 0 && (q & 1) == 0);
-            const int tile = q == 0 ? 0 : (q == 2 * it.tiles - 1 ? it.tiles - 1 : (is_v ? q / 2 - 1 : (q + 1) / 2));
+        // rows of the latest K tile, of the one before it (V follows a tile behind) and of the next
+        int64_t r_k = -1, r_before = -1, r_next = look_up(0);
+        bool ok = true;
+        int q = 0;
+        for (; q < 2 * it.tiles; ++q) {
+            const bool last = q == 2 * it.tiles - 1, is_v = last || (q > 0 && (q & 1) == 0);
+            if (!is_v) {
+                r_before = r_k;
+                r_k = r_next;
+                r_next = look_up((q + 1) / 2 + 1);
+            }
             if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
             if (!ok) break;
             const uint16_t *src = (is_v ? a.pool.v : a.pool.k) + head;
             const uint32_t dst = sb + uint32_t(C::O_RING + (q % C::NSLOT) * C::SLOT);
-            const int tok0 = it.t0 + tile * TT;
+            const int64_t mine = is_v && !last ? r_before : r_k;
 #pragma unroll
             for (int j = 0; j < STEPS; ++j) {
-                const int idx = tid + j * 32 * LW, r = idx / CH, c = idx % CH;
-                if (TT * CH % (32 * LW) != 0 && idx >= TT * CH) break;
-                const int64_t row = tok0 + r < it.t1 ? page_row(a.pool, a.prefix_table, tok0 + r, a.status) : -1;
-                copy16(dst + tile_off<D, TT>(r, c), src + (row >= 0 ? row + 8 * c : 0), row >= 0);
+                const int k = j * RPS + lane / CH, r = w + LW * k;
+                const int64_t o = __shfl_sync(FULL, mine, k);
+                if (r < TT) copy16(dst + tile_off<D, TT>(r, c), src + (o >= 0 ? o : 0), o >= 0);
             }
             copy_commit();
             if (q >= C::LAG) {
@@ -392,7 +403,7 @@ template <int D, int DT> cudaError_t prefix_d(const PagedArgs &a, cudaStream_t s
     static const cudaError_t attr =
         cudaFuncSetAttribute(prefix_kernel<D, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
     if (attr != cudaSuccess) return attr;
-    return launch_paged(prefix_kernel<D, DT>, dim3(unsigned(a.prefix_items)), THREADS, Cfg<D>::SMEM, s, a);
+    return launch_paged(prefix_kernel<D, DT>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), THREADS, Cfg<D>::SMEM, s, a);
 }
 
 }  // namespace
@@ -400,7 +411,7 @@ template <int D, int DT> cudaError_t prefix_d(const PagedArgs &a, cudaStream_t s
 int prefix_ctas_per_sm(int dim) { return dim == 256 ? Cfg<256>::CTAS : Cfg<128>::CTAS; }
 
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s) {
-    if (a.prefix_items <= 0) return cudaSuccess;
+    if (a.n_split <= 0) return cudaSuccess;
     KVX_PAGED_DIM(prefix_d)
 }
 

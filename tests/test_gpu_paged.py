@@ -227,6 +227,21 @@ def test_attend_prefix_lengths(kvx, cuda, H, prefix, batch, hq, hkv, dim):
     H.assert_attends(out, lse, c.truth())
 
 
+@pytest.mark.parametrize("batch,hq,hkv,dim,dtype", [(7, 32, 8, 128, "fp16"), (9, 2, 2, 64, "bf16"), (40, 4, 1, 32, "bf16"),
+                                                    (3, 16, 4, 256, "bf16")])
+def test_attend_long_prefix_again_and_again(kvx, cuda, H, batch, hq, hkv, dim, dtype):
+    """Many tiles an item and warps with no rows of their own: every run is the same, and no wait runs out."""
+    torch = cuda
+    c = H.Paged(batch, hq, hkv, dim, 40000, [5] * batch, 48, "hnd", dtype)
+    b, pages = kvx.Batch(batch, hq, hkv, dim, dtype=dtype), kvx.Pages(c.k_pool, c.v_pool)
+    outs = [torch.empty((batch, hq, dim), device="cuda", dtype=c.q.dtype) for _ in range(2)]
+    for i in range(60):
+        b.attend(c.q, outs[i % 2], pages, c.table, c.lens, 5, prefix_table=c.prefix_table, prefix_len=40000)
+    b.check()
+    assert torch.equal(outs[0], outs[1])
+    H.assert_attends(outs[0], None, c.truth())
+
+
 @pytest.mark.parametrize("dim,dtype", [(32, "fp16"), (64, "bf16"), (128, "bf16"), (256, "bf16")])
 def test_attend_peaked_and_rising_scores(kvx, cuda, H, dim, dtype):
     """Scores that rise along the prefix (every tile raises the maximum) and differ by hundreds."""
