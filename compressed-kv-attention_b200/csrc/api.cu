@@ -8,11 +8,13 @@
 // buffers and launches kernels.
 #include "codec.cuh"
 #include "host.cuh"
+#include "prefix.cuh"
 
 #include <algorithm>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -299,6 +301,7 @@ struct kvx_plan_s {
     int n_ranges = 0;     // CTA ranges of the attention grid (one CTA each)
     int64_t n_rows = 0;   // partial-state rows (one per unit segment of a CTA range)
     int stages_per_block = 0;  // ring stages of every block in the attention kernel (0: by block)
+    int max_valid = 0;         // attended tokens of the longest block
     bool compact = false;      // every block is coded: the attention kernel's compact ring
     cudaStream_t s = nullptr;
     UnitDev *units = nullptr;
@@ -526,6 +529,7 @@ static int plan_create_impl(const kvx_unit *units, int n_units, int n_q, int dim
         const int tsb = attention_stage_tokens(dim);
         p->stages_per_block = max_valid[0] > 0 ? (max_valid[0] + tsb - 1) / tsb : 0;
         p->compact = !bf16 && max_valid[1] == 0;
+        p->max_valid = max_valid[0];
     }
     // escape records: offsets, then (with the array sized) the records
     unsigned long long esc_total = 0;
@@ -608,6 +612,71 @@ int kvx_plan_create(const kvx_unit *units, int n_units, int n_q, int dim, int bl
                     kvx_plan *out) {
     return plan_create_impl(units, n_units, n_q, dim, block_tokens, out, false, nullptr);
 }
+
+// A shared prefix is prepared like a plan over its heads (every check of the blobs, escape records,
+// merge words); it keeps the records, the merge words and its own group table.
+static int prefix_create_impl(const kvx_unit *heads, int n_kv_heads, int dim, kvx_prefix *out) {
+    if (out == nullptr || heads == nullptr || n_kv_heads <= 0)
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_prefix_create: bad argument");
+    *out = nullptr;
+    std::vector<kvx_unit> units(heads, heads + n_kv_heads);
+    for (kvx_unit &u : units) {
+        if (u.k_index == nullptr || u.v_index == nullptr)
+            return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_prefix_create: a prefix is made of xkv blobs with their indexes");
+        if (u.seq != heads[0].seq || u.n_blocks != heads[0].n_blocks)
+            return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_prefix_create: heads of different lengths or block counts");
+        u.q = reinterpret_cast<const uint16_t *>(u.k);  // a plan wants both; nothing is run
+        u.out = reinterpret_cast<float *>(const_cast<void *>(u.k));
+        u.lse = nullptr;
+    }
+    kvx_plan plan = nullptr;
+    if (int rc = plan_create_impl(units.data(), n_kv_heads, 1, dim, kDefaultBlock, &plan, false, nullptr)) return rc;
+    PlanGuard guard{plan};
+    auto p = std::make_unique<kvx_prefix_s>();
+    p->n_kv_heads = n_kv_heads;
+    p->dim = dim;
+    p->seq = heads[0].seq;
+    const int tpb = std::max(1, (plan->max_valid + kPrefixTile - 1) / kPrefixTile);
+    XkvGroup *groups = nullptr;
+    uint8_t *tokens = nullptr;
+    const size_t tiles = size_t(plan->n_blocks) * size_t(tpb);
+    if (tiles > size_t(0x7FFFFFFF) / 8 || size_t(plan->n_blocks) * size_t(dim) > 0xFFFFFFFFull)
+        return fail(KVX_ERR_UNSUPPORTED, "kvx_prefix_create: too many blocks");
+    KVX_CUDA(cudaMalloc(&groups, tiles * 2 * (kPrefixTile / 16) * sizeof(XkvGroup)));
+    p->owned.push_back(groups);
+    KVX_CUDA(cudaMalloc(&tokens, tiles));
+    p->owned.push_back(tokens);
+    KVX_CUDA(launch_xkv_groups(plan->desc, plan->n_blocks, tpb, dim, groups, tokens, nullptr));
+    std::vector<uint8_t> host_tokens(tiles);
+    KVX_CUDA(cudaMemcpy(host_tokens.data(), tokens, tiles, cudaMemcpyDeviceToHost));
+    const size_t per_head = tiles / size_t(n_kv_heads);
+    for (size_t i = 0; i < tiles; ++i)
+        if (host_tokens[i] != 0) p->dev.tiles = std::max(p->dev.tiles, int32_t(i % per_head) + 1);
+    // the records and merge words change hands
+    for (void *q : {static_cast<void *>(plan->esc), static_cast<void *>(plan->b7)}) {
+        plan->owned.erase(std::find(plan->owned.begin(), plan->owned.end(), q));
+        p->owned.push_back(q);
+    }
+    p->dev.groups = groups;
+    p->dev.tile_tokens = tokens;
+    p->dev.esc = plan->esc;
+    p->dev.b7 = plan->b7;
+    p->dev.blocks = heads[0].n_blocks;
+    p->dev.tiles_per_block = tpb;
+    *out = p.release();
+    g_err.clear();
+    return KVX_OK;
+}
+
+int kvx_prefix_create(const kvx_unit *heads, int n_kv_heads, int dim, kvx_prefix *out) {
+    try {
+        return prefix_create_impl(heads, n_kv_heads, dim, out);
+    } catch (const std::exception &e) {
+        return fail(KVX_ERR_RUNTIME, std::string("kvx_prefix_create: ") + e.what());
+    }
+}
+
+void kvx_prefix_destroy(kvx_prefix p) { delete p; }
 
 int kvx_plan_run(kvx_plan p, void *stream) {
     if (int rc = kvx_plan_run_part(p, 0, stream)) return rc;

@@ -6,6 +6,7 @@
 
 #include "host.cuh"
 #include "paged.cuh"
+#include "prefix.cuh"
 
 using namespace kvx;
 
@@ -236,8 +237,12 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: bad argument");
     if (h->dim != 32 && h->dim != 64 && h->dim != 128 && h->dim != 256)
         return fail(KVX_ERR_UNSUPPORTED, "kvx_batch_attend: head_dim must be 32, 64, 128 or 256");
-    const bool paged = x->prefix_table != nullptr && x->prefix_len > 0;
-    if (x->prefix_len > 0 && x->prefix_table == nullptr)
+    const bool coded = x->prefix != nullptr, paged = !coded && x->prefix_table != nullptr && x->prefix_len > 0;
+    if (coded && (x->prefix_table != nullptr || x->prefix_len > 0))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: one prefix, in pages or as blobs");
+    if (coded && (h->dtype != KVX_DTYPE_BF16 || x->prefix->dim != h->dim || x->prefix->n_kv_heads != h->n_kv_heads))
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: the prefix is BF16 and of other heads or another head_dim");
+    if (!coded && x->prefix_len > 0 && x->prefix_table == nullptr)
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: a prefix without its page table");
     if (x->max_len > 0 && (x->table == nullptr || x->lens == nullptr))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: tails without page table or lengths");
@@ -260,6 +265,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     a.lens = x->lens;
     a.table_stride = x->table_stride;
     a.prefix_len = paged ? x->prefix_len : 0;
+    if (coded) a.xkv = x->prefix->dev;
     a.max_len = x->max_len;
     a.batch = x->batch;
     a.n_q_heads = h->n_q_heads;
@@ -271,13 +277,13 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     a.status = h->status;
     a.starts = h->starts;
     const int rows = x->batch * h->group;
-    const bool tensor = paged && rows > kStreamRows;
+    const bool tensor = coded || (paged && rows > kStreamRows);
     if (tensor) {
         a.row_groups = ceil_div(rows, kPrefixRows);
         a.row_pad = kPrefixRows * a.row_groups;
-        a.split_tokens = kPrefixTile * prefix_split_tiles(ceil_div(x->prefix_len, kPrefixTile), h->n_kv_heads * a.row_groups,
-                                                          prefix_ctas_per_sm(h->dim) * h->sms);
-        a.n_split = ceil_div(x->prefix_len, a.split_tokens);
+        a.prefix_tiles = coded ? a.xkv.tiles : ceil_div(x->prefix_len, kPrefixTile);
+        a.split_tiles = prefix_split_tiles(a.prefix_tiles, h->n_kv_heads * a.row_groups, prefix_ctas_per_sm(h->dim) * h->sms);
+        a.n_split = ceil_div(a.prefix_tiles, a.split_tiles);
         a.stream_base = int64_t(h->n_kv_heads) * a.n_split * a.row_pad;
     }
     a.tail_groups = ceil_div(h->group, 8);

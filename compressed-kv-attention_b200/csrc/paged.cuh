@@ -58,6 +58,30 @@ struct RotArgs {
 
 cudaError_t launch_rotate(int dtype, bool vec, const RotArgs &a, cudaStream_t s);
 
+// 16 tokens of one tensor of an XKV prefix, as the loader warps of the prefix kernel take them
+// (built once by kvx_prefix_create; 32 bytes for 16 tokens).
+struct XkvGroup {
+    uint64_t rows;    // address of the first token's sign/mantissa bytes (raw block: BF16 values)
+    uint32_t codes;   // from there to its residual codes
+    uint32_t esc;     // first escape entry (index in XkvDev::esc)
+    uint32_t b7;      // the block's merge words (index in XkvDev::b7)
+    uint16_t n_esc;
+    uint8_t mode;     // 0 raw, 2, 3, 4
+    uint8_t n;        // tokens (0 past the block's end)
+    uint32_t pad[2];
+};
+static_assert(sizeof(XkvGroup) == 32, "XkvGroup is 32 bytes");
+
+// An XKV prefix: every block takes tiles_per_block tiles of kPrefixTile tokens (fewer or none in
+// the last ones), every tile four groups a tensor.
+struct XkvDev {
+    const XkvGroup *groups;      // [kv head][block][K, V][tiles_per_block][4]
+    const uint8_t *tile_tokens;  // [kv head][block][tiles_per_block]
+    const uint32_t *esc, *b7;
+    int32_t blocks, tiles_per_block;
+    int32_t tiles;               // up to the last with tokens
+};
+
 // One attention call (kvx_batch_attend) as its kernels see it.
 struct PagedArgs {
     const uint16_t *q;
@@ -68,6 +92,7 @@ struct PagedArgs {
     const int32_t *prefix_table, *table, *lens;
     int64_t table_stride;
     int32_t prefix_len, max_len;
+    XkvDev xkv;             // the prefix when xkv.blocks > 0
     int32_t batch, n_q_heads, n_kv_heads, group;
     float scale_log2;       // scale * log2(e)
     int *status;
@@ -75,9 +100,9 @@ struct PagedArgs {
     float *acc;
     float2 *ml;
     // Tensor-core prefix parts: row ((kv head * n_split + split) * row_pad + row), n_split parts of
-    // split_tokens tokens (the last fewer) for each of the head's batch * group rows, in row_groups
-    // items of kPrefixRows rows.
-    int32_t n_split, row_pad, split_tokens, row_groups;
+    // split_tiles tiles of kPrefixTile tokens (the last fewer) of prefix_tiles for each of the head's
+    // batch * group rows, in row_groups items of kPrefixRows rows.
+    int32_t n_split, row_pad, split_tiles, prefix_tiles, row_groups;
     // Streamed units, laid end to end in 16-token tiles: first (a streamed prefix) KV head by KV
     // head and group of 8 rows, prefix_len tokens each; then sequence by sequence, KV head by KV
     // head, group of 8 heads by group, the sequence's own tokens.  The tiles are cut into as many
@@ -109,6 +134,10 @@ int prefix_ctas_per_sm(int dim);
 
 // The tensor-core kernel over the prefix items of `a`.
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
+// The group table of an XKV prefix from its flat blocks' descriptors (heads * blocks of them).
+struct BlockDesc;
+cudaError_t launch_xkv_groups(const BlockDesc *desc, int64_t n_blocks, int tiles_per_block, int dim, XkvGroup *groups,
+                              uint8_t *tile_tokens, cudaStream_t s);
 // The streaming kernel over the units of `a` and the combine pass over every (sequence, head).
 // beside: the launch before it on the stream is the same call's prefix kernel, which it may run beside.
 cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, bool beside, cudaStream_t s);

@@ -16,11 +16,20 @@
 //    relative to is raised, and O rescaled in TMEM, only when some row's scores pass it by 2^8
 //    (2^5 for FP16 weights), which is rare after the first tile; l and O share it, so it cancels.
 //
+// An XKV prefix takes the same kernel with other loader warps: each takes the tiles' 16-token groups
+// in turn (every group's place, mode and escapes are in a table built with the prefix), brings a
+// group's sign/mantissa bytes and residual codes into a staging slot of its own by two bulk copies,
+// a few groups ahead, and rebuilds them into the ring's tile: BF16 words by byte permutes and one
+// multiply-add a pair, escapes stored over them, rows past the block's end as zeros.  The blocks are
+// decoded once for the item's 128 rows.
+//
 // What bounds it: per 64-token tile and 128 rows the SM's exponentials take 64 x 128 / 16 = 512
 // cycles, the MMAs 4 D (256 at D = 64, 512 at D = 128) and the tile's bytes from HBM 256 D / 23
 // (712 at D = 64, 1425 at D = 128, shared by all 128-row items of the head through L2).  Two CTAs
 // a SM (one at D = 256) overlap one's softmax with the other's waits.
+#include "attention.cuh"
 #include "paged_types.cuh"
+#include "xkv_decode.cuh"
 
 namespace kvx {
 namespace {
@@ -32,19 +41,29 @@ constexpr int SW = 4, LW = 3;           // softmax and loader warps
 constexpr int THREADS = 32 * (SW + LW + 1);
 constexpr uint32_t kWaitUs = 1000000;   // bounded waits
 
-template <int D> struct Cfg {
+template <int D, bool XKV> struct Cfg {
     static constexpr int ROWB = D >= 64 ? 128 : 64;         // bytes of a row of one panel of head dims
     static constexpr int SLOT = TT * D * 2;
-    static constexpr int NSLOT = D == 32 ? 12 : (D == 64 ? 10 : 5);
+    static constexpr int NSLOT = XKV ? (D == 32 ? 8 : (D == 64 ? 6 : 3)) : (D == 32 ? 12 : (D == 64 ? 10 : 5));
     static constexpr int LAG = NSLOT - 2;                   // tiles in flight before one is announced
     static constexpr int CTAS = D == 256 ? 1 : 2;           // per SM
     static constexpr int O_Q = 0;
     static constexpr int O_RING = ROWS * D * 2;
-    static constexpr int O_BAR = O_RING + NSLOT * SLOT;
-    static constexpr int SMEM = O_BAR + 16 * NSLOT + 64;
+    // staging slots of a loader warp (XKV): the group's table entry, 16 rows, their codes, each piece
+    // landing 0-15 bytes past its 16-byte aligned start
+    static constexpr int NSTAGE = XKV ? (D <= 64 ? 8 : 3) : 0;
+    static constexpr int S_ROWS = 32, S_CODES = S_ROWS + 16 * D + 32;
+    static constexpr int STAGE = S_CODES + 8 * D + 32;
+    static constexpr int O_STAGE = O_RING + NSLOT * SLOT;
+    static constexpr int O_BAR = O_STAGE + LW * NSTAGE * STAGE;
+    static constexpr int N_BAR = 2 * NSLOT + 6 + LW * NSTAGE;
+    static constexpr int SMEM = O_BAR + 8 * N_BAR + 16;
+    // arrivals that announce a tile: one of each loader warp, or one for each 16-token group
+    static constexpr int ARRIVE = XKV ? TT / 16 : LW;
     static constexpr int LDO = D + 4;                       // floats of a staged output row
     static constexpr int TMEM = D == 256 ? 512 : 256;       // columns: O at 0, S / P buffers at D, D + 64
     static constexpr uint64_t LAYOUT = D >= 64 ? 2 : 4;     // 128- / 64-byte swizzle
+    static_assert(LAG < NSLOT - 1, "the tile that frees the ring's next slot has been announced");
     static_assert(ROWS * LDO * 4 <= O_BAR, "the staged outputs fit where Q and the ring were");
     static_assert(D + 2 * TT <= TMEM && CTAS * TMEM <= 512, "TMEM columns");
     static_assert(CTAS * (SMEM + 1024) <= 233472, "shared memory");
@@ -130,13 +149,14 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live)
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Barriers of a CTA (8 bytes each): full and empty of every ring slot, then these.
+// Barriers of a CTA (8 bytes each): full and empty of every ring slot, these, then one for each
+// staging slot.
 enum { B_S0, B_S1, B_P0, B_P1, B_PV, B_Q, B_COUNT };
 
 // One item.
 struct Item {
     int head, first, n;   // KV head, first row, rows
-    int t0, t1, tiles;
+    int tile0, tiles;
     int64_t row0;
 };
 __device__ __forceinline__ Item item_of(const PagedArgs &a, int i) {
@@ -147,9 +167,8 @@ __device__ __forceinline__ Item item_of(const PagedArgs &a, int i) {
     x.head = i / a.n_split;
     x.first = mt * ROWS;
     x.n = min(ROWS, a.batch * a.group - x.first);
-    x.t0 = s * a.split_tokens;
-    x.t1 = min(a.prefix_len, x.t0 + a.split_tokens);
-    x.tiles = (x.t1 - x.t0 + TT - 1) / TT;
+    x.tile0 = s * a.split_tiles;
+    x.tiles = min(a.split_tiles, a.prefix_tiles - x.tile0);
     x.row0 = int64_t(x.head * a.n_split + s) * a.row_pad + x.first;
     return x;
 }
@@ -158,11 +177,47 @@ __device__ __forceinline__ Item item_of(const PagedArgs &a, int i) {
 __device__ __forceinline__ int k_item(int i) { return i == 0 ? 0 : 2 * i - 1; }
 __device__ __forceinline__ int v_item(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
 
-template <int D, int DT>
-__global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const PagedArgs a) {
-    using C = Cfg<D>;
+// Chunk steps of one 16-token group: rebuild them from the staged sections (coded modes) or the raw
+// rows into the tile at `dst` (rows j0 .. j0 + 15), rows at or past n as zeros.
+template <int D, int MODE>
+__device__ __forceinline__ void decode_group(uint32_t stage_rows, uint32_t stage_codes, uint64_t raw, const Lay &ly,
+                                             const uint32_t (&b7)[4], uint32_t dst, int j0, int n, int lane) {
+    constexpr int C8 = D / 8, RPI = 32 / C8, STEPS = 16 / RPI, G = STEPS < 4 ? STEPS : 4;
+    const int r0 = lane / C8, c8 = lane % C8;
+#pragma unroll
+    for (int k = 0; k < STEPS; k += G) {
+        uint32_t W[G][MODE == 0 ? 5 : 3], X[G][2];
+        if constexpr (MODE == 0) {
+            // straight from the blob (raw blocks are rare): row sections start 0 or 2 bytes past a
+            // word, and the word after the row's last is not read when it would be the blob's end
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(raw & ~uint64_t(3));
+            const bool odd = (raw & 2u) != 0;
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int r = r0 + RPI * (k + g);
+#pragma unroll
+                for (int i = 0; i < 5; ++i)
+                    W[g][i] = r < n && (i < 4 || odd) ? __ldg(p + r * (D / 2) + 4 * c8 + i) : 0u;
+            }
+        } else {
+            load_chunks<D, MODE, G, 0>(stage_rows + uint32_t(k * RPI * D), stage_codes + uint32_t(k * RPI * (D * MODE / 8)), W, X);
+        }
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            uint32_t w[4];
+            build_chunk<MODE>(ly, b7, W[g], X[g], w);
+            const int r = r0 + RPI * (k + g);
+            const bool in = r < n;
+            sts_v4(dst + tile_off<D, TT>(j0 + r, c8), in ? w[0] : 0u, in ? w[1] : 0u, in ? w[2] : 0u, in ? w[3] : 0u);
+        }
+    }
+}
+
+template <int D, int DT, bool XKV>
+__global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(const PagedArgs a) {
+    using C = Cfg<D, XKV>;
     extern __shared__ __align__(1024) uint8_t smem[];
-    volatile uint32_t *tmem_base = reinterpret_cast<volatile uint32_t *>(smem + C::O_BAR + 16 * C::NSLOT + 8 * B_COUNT);
+    volatile uint32_t *tmem_base = reinterpret_cast<volatile uint32_t *>(smem + C::O_BAR + 8 * C::N_BAR);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -179,13 +234,14 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
     };
 
     if (warp == SW + LW) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar(B_COUNT)),
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bars + uint32_t(8 * C::N_BAR)),
                      "n"(C::TMEM)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::NSLOT; ++i) mbar_init(full(i), LW), mbar_init(empty(i), 1);
+        for (int i = 0; i < C::NSLOT; ++i) mbar_init(full(i), C::ARRIVE), mbar_init(empty(i), 1);
+        for (int i = 0; i < LW * C::NSTAGE; ++i) mbar_init(bar(B_COUNT + i), 1);
         mbar_init(bar(B_S0), 1), mbar_init(bar(B_S1), 1), mbar_init(bar(B_P0), SW), mbar_init(bar(B_P1), SW);
         mbar_init(bar(B_PV), 1), mbar_init(bar(B_Q), SW);
         fence_mbar_init();
@@ -197,6 +253,107 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
 
     if (warp >= SW && warp < SW + LW) {
         // ---- loads ----
+        // tile of ring item q, and which of K and V: K of the next tile, then V of the one before
+        auto is_v_item = [&](int q) { return q == 2 * it.tiles - 1 || (q > 0 && (q & 1) == 0); };
+        if constexpr (XKV) {
+            // Loader warp w takes the 16-token groups w, w + LW, ... of the ring's items in order: each
+            // tile's four arrivals come from whichever warps had them.
+            constexpr int C8 = D / 8, NS = C::NSTAGE;
+            const int w = warp - SW, c8 = lane % C8, r0 = lane / C8;
+            const int total = 2 * it.tiles * (TT / 16), mine = (total - w + LW - 1) / LW;
+            const uint32_t stages = sb + uint32_t(C::O_STAGE + w * NS * C::STAGE);
+            auto entry = [&](int k) -> const uint4 * {
+                const int id = w + LW * k, q = id >> 2;
+                const bool v = is_v_item(q);
+                const int tile = it.tile0 + (q == 0 ? 0 : (q == 2 * it.tiles - 1 ? it.tiles - 1 : (v ? q / 2 - 1 : (q + 1) / 2)));
+                const int block = tile / a.xkv.tiles_per_block, sub = tile - block * a.xkv.tiles_per_block;
+                const int64_t i = ((int64_t(it.head) * a.xkv.blocks + block) * 2 + (v ? 1 : 0)) * a.xkv.tiles_per_block + sub;
+                return reinterpret_cast<const uint4 *>(a.xkv.groups + i * 4 + (id & 3));
+            };
+            auto staged = [&](int k) { return bar(B_COUNT + w * NS + k % NS); };
+            // group k into its staging slot: the table entry, and the copies of a coded group
+            auto issue = [&](int k, const uint4 &e0, const uint4 &e1) {
+                const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
+                if (lane == 0) {
+                    sts_v4(slot, e0.x, e0.y, e0.z, e0.w);
+                    sts_v4(slot + 16, e1.x, e1.y, e1.z, e1.w);
+                    const uint64_t rows = (uint64_t(e0.y) << 32) | e0.x;
+                    const uint32_t mode = (e1.y >> 16) & 0xFFu, n = e1.y >> 24;
+                    uint32_t len0 = 0, len1 = 0;
+                    const uint64_t codes = rows + e0.z;
+                    if (mode != 0 && n > 0) {
+                        len0 = (uint32_t(rows & 15u) + n * D + 15u) & ~15u;
+                        len1 = (uint32_t(codes & 15u) + n * D * mode / 8 + 15u) & ~15u;
+                    }
+                    mbar_arrive_expect_tx(staged(k), len0 + len1);
+                    if (len0 != 0) {
+                        bulk_g2s(slot + C::S_ROWS, reinterpret_cast<const void *>(rows & ~uint64_t(15)), len0, staged(k));
+                        bulk_g2s(slot + C::S_CODES, reinterpret_cast<const void *>(codes & ~uint64_t(15)), len1, staged(k));
+                    }
+                }
+            };
+            uint4 e0 = make_uint4(0u, 0u, 0u, 0u), e1 = e0;
+            int issued = 0;
+            for (; issued < NS && issued < mine; ++issued) {
+                const uint4 *p = entry(issued);
+                issue(issued, __ldg(p), __ldg(p + 1));
+            }
+            if (issued < mine) e0 = __ldg(entry(issued)), e1 = __ldg(entry(issued) + 1);
+            __syncwarp();
+            // what a group needs from global memory besides its copies, fetched a group ahead: the
+            // lane's merge words and escape entry
+            uint4 h0, h1, b7n = make_uint4(0u, 0u, 0u, 0u);
+            uint32_t escn = 0;
+            auto fetch = [&](int k) {
+                const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
+                lds_v4(slot, h0.x, h0.y, h0.z, h0.w);
+                lds_v4(slot + 16, h1.x, h1.y, h1.z, h1.w);
+                if (((h1.y >> 16) & 0xFFu) != 0) b7n = __ldg(reinterpret_cast<const uint4 *>(a.xkv.b7 + h1.x) + c8);
+                if (lane < int(h1.y & 0xFFFFu)) escn = __ldg(a.xkv.esc + h0.w + lane);
+            };
+            if (mine > 0) fetch(0);
+            bool ok = true;
+            int k = 0;
+            for (; k < mine; ++k) {
+                const int id = w + LW * k, q = id >> 2, j0 = 16 * (id & 3);
+                const uint4 g0 = h0, g1 = h1;
+                const uint32_t b7[4] = {b7n.x, b7n.y, b7n.z, b7n.w}, ent = escn;
+                if (k + 1 < mine) fetch(k + 1);
+                if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
+                if (ok) ok = __all_sync(FULL, wait(staged(k), k / NS));
+                if (!ok) break;
+                const uint64_t rows = (uint64_t(g0.y) << 32) | g0.x;
+                const int n_esc = int(g1.y & 0xFFFFu), mode = int((g1.y >> 16) & 0xFFu), n = int(g1.y >> 24);
+                const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
+                const uint32_t dst = sb + uint32_t(C::O_RING + (q % C::NSLOT) * C::SLOT);
+                const Lay ly = make_lay<D>(uint32_t(rows) & 15u, uint32_t(rows + g0.z) & 15u, mode, c8, false, C::S_CODES - C::S_ROWS);
+                const uint32_t sr = slot + C::S_ROWS + ly.rows + uint32_t(r0 * D), sc = slot + C::S_ROWS + ly.codes;
+                if (mode == 4) decode_group<D, 4>(sr, sc + uint32_t(r0 * (D / 2)), 0, ly, b7, dst, j0, n, lane);
+                else if (mode == 2) decode_group<D, 2>(sr, sc + uint32_t(r0 * (D / 4)), 0, ly, b7, dst, j0, n, lane);
+                else if (mode == 3) decode_group<D, 3>(sr, sc + uint32_t(r0 * (D * 3 / 8)), 0, ly, b7, dst, j0, n, lane);
+                else decode_group<D, 0>(0, 0, rows, ly, b7, dst, j0, n, lane);
+                __syncwarp();
+                // escapes: the entry's element by its byte in a 16-row tile (swizzled like this one's rows)
+                for (int i = lane; i < n_esc; i += 32) {
+                    const uint32_t e = i == lane ? ent : __ldg(a.xkv.esc + g0.w + i);
+                    const uint32_t at = e & 0xFFFEu, r = at / (2 * D), in_row = at % (2 * D);
+                    if (int(r) < n)
+                        sts_u16(dst + (in_row / C::ROWB) * (TT * C::ROWB) + (uint32_t(j0) + r) * C::ROWB + in_row % C::ROWB, e >> 16);
+                }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full(q));
+                if (issued < mine) {
+                    issue(issued, e0, e1);
+                    ++issued;
+                    if (issued < mine) e0 = __ldg(entry(issued)), e1 = __ldg(entry(issued) + 1);
+                    __syncwarp();
+                }
+            }
+            // after a wait that ran out: let the copies in flight land before the memory goes away
+            if (!ok)
+                for (; k < issued; ++k) mbar_wait_bounded(staged(k), uint32_t((k / NS) & 1), kWaitUs);
+        } else {
         // Loader warp w copies rows w, w + LW, ... of every tile: lane k holds the offset of row w +
         // LW k (-1: no such token), looked up a tile ahead of its use.
         constexpr int CH = D / 8, RPS = 32 / CH;              // pieces a row, rows a step
@@ -204,8 +361,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
         const int w = warp - SW, c = lane % CH;
         const int64_t head = int64_t(it.head) * a.pool.head_stride + 8 * c;
         auto look_up = [&](int tile) -> int64_t {
-            const int r = w + LW * lane, tok = it.t0 + tile * TT + r;
-            return r < TT && tok < it.t1 ? page_row(a.pool, a.prefix_table, tok, a.status) : -1;
+            const int r = w + LW * lane, tok = (it.tile0 + tile) * TT + r;
+            return r < TT && tok < a.prefix_len && tile < it.tiles ? page_row(a.pool, a.prefix_table, tok, a.status) : -1;
         };
         auto announce = [&](int i) {
             proxy_fence();
@@ -217,7 +374,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
         bool ok = true;
         int q = 0;
         for (; q < 2 * it.tiles; ++q) {
-            const bool last = q == 2 * it.tiles - 1, is_v = last || (q > 0 && (q & 1) == 0);
+            const bool last = q == 2 * it.tiles - 1, is_v = is_v_item(q);
             if (!is_v) {
                 r_before = r_k;
                 r_k = r_next;
@@ -243,6 +400,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
         copy_wait<0>();
         if (ok)
             for (int i = max(0, q - C::LAG); i < q; ++i) announce(i);
+        }
     } else if (warp == SW + LW) {
         // ---- MMAs ----
         if (lane == 0 && wait(bar(B_Q), 0)) {
@@ -301,6 +459,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int i = 0; i < it.tiles && ok; ++i) {
+            int valid = a.prefix_len - (it.tile0 + i) * TT;  // tokens of the tile
+            if constexpr (XKV)
+                valid = __ldg(a.xkv.tile_tokens + int64_t(it.head) * a.xkv.blocks * a.xkv.tiles_per_block + it.tile0 + i);
             ok = __all_sync(FULL, wait(bar(B_S0 + (i & 1)), i >> 1));
             if (!ok) break;
             fence_after();
@@ -312,7 +473,6 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
                 tmem_ld32(st + 32, x1);
                 tmem_wait_ld(x0);
                 tmem_wait_ld(x1);
-                const int valid = it.t1 - (it.t0 + i * TT);
                 if (valid < TT) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
@@ -399,16 +559,64 @@ __global__ void __launch_bounds__(THREADS, Cfg<D>::CTAS) prefix_kernel(const Pag
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(C::TMEM) : "memory");
 }
 
-template <int D, int DT> cudaError_t prefix_d(const PagedArgs &a, cudaStream_t s) {
+template <int D, int DT, bool XKV> cudaError_t prefix_launch(const PagedArgs &a, cudaStream_t s) {
+    using C = Cfg<D, XKV>;
     static const cudaError_t attr =
-        cudaFuncSetAttribute(prefix_kernel<D, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+        cudaFuncSetAttribute(prefix_kernel<D, DT, XKV>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (attr != cudaSuccess) return attr;
-    return launch_paged(prefix_kernel<D, DT>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), THREADS, Cfg<D>::SMEM, s, a);
+    return launch_paged(prefix_kernel<D, DT, XKV>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), THREADS, C::SMEM, s, a);
+}
+template <int D, int DT> cudaError_t prefix_d(const PagedArgs &a, cudaStream_t s) {
+    if constexpr (DT == KVX_DTYPE_BF16)
+        if (a.xkv.blocks > 0) return prefix_launch<D, DT, true>(a, s);
+    return prefix_launch<D, DT, false>(a, s);
+}
+
+// One thread per (flat block, tile): its eight groups and its token count.
+__global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int dim, XkvGroup *groups, uint8_t *tokens) {
+    const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+    if (i >= n * tpb) return;
+    const int64_t b = i / tpb;
+    const int sub = int(i - b * tpb);
+    const BlockDesc &d = desc[b];
+    const int left = int(d.valid) - sub * TT;
+    tokens[i] = uint8_t(left < 0 ? 0 : (left < TT ? left : TT));
+    for (int T = 0; T < 2; ++T) {
+        const uint64_t blk = T ? d.v : d.k;
+        const int mode = T ? d.v_mode : d.k_mode, nesc = T ? d.v_nesc : d.k_nesc;
+        for (int j = 0; j < TT / 16; ++j) {
+            const int g16 = sub * (TT / 16) + j, t0 = 16 * g16;
+            XkvGroup g{};
+            g.mode = uint8_t(mode);
+            const int m = int(d.valid) - t0;
+            g.n = uint8_t(m < 0 ? 0 : (m < 16 ? m : 16));
+            g.b7 = uint32_t(d.b7_block) * uint32_t(dim) + uint32_t(T * (dim / 2));
+            if (g.n > 0) {
+                const uint64_t rows = blk + kHeaderBytes + (mode != 0 ? dim : 0);
+                g.rows = rows + uint64_t(t0) * dim * (mode != 0 ? 1 : 2);
+                g.codes = mode != 0 ? uint32_t(int(d.n_tok) * dim + t0 * dim * mode / 8 - t0 * dim) : 0u;
+                if (mode != 0 && nesc != 0) {
+                    const int e0 = g16 == 0 ? 0 : d.em[T][g16 - 1], e1 = d.em[T][g16];
+                    g.esc = (T ? d.v_rec : d.k_rec) + uint32_t(kEscRecHead + e0);
+                    g.n_esc = uint16_t(e1 - e0);
+                }
+            }
+            groups[((b * 2 + T) * tpb + sub) * (TT / 16) + j] = g;
+        }
+    }
 }
 
 }  // namespace
 
-int prefix_ctas_per_sm(int dim) { return dim == 256 ? Cfg<256>::CTAS : Cfg<128>::CTAS; }
+int prefix_ctas_per_sm(int dim) { return dim == 256 ? Cfg<256, false>::CTAS : Cfg<128, false>::CTAS; }
+
+cudaError_t launch_xkv_groups(const BlockDesc *desc, int64_t n_blocks, int tiles_per_block, int dim, XkvGroup *groups,
+                              uint8_t *tile_tokens, cudaStream_t s) {
+    const int64_t n = n_blocks * tiles_per_block;
+    if (n <= 0) return cudaSuccess;
+    xkv_groups_kernel<<<unsigned((n + 127) / 128), 128, 0, s>>>(desc, n_blocks, tiles_per_block, dim, groups, tile_tokens);
+    return cudaGetLastError();
+}
 
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s) {
     if (a.n_split <= 0) return cudaSuccess;

@@ -148,7 +148,7 @@ class kvx_rope(C.Structure):
 
 class kvx_attend(C.Structure):
     _fields_ = [("q", kvx_view), ("out", kvx_view), ("lse", _vp), ("pages", C.POINTER(kvx_pages)),
-                ("prefix_table", _vp), ("table", _vp), ("lens", _vp), ("table_stride", C.c_int64),
+                ("prefix_table", _vp), ("prefix", _vp), ("table", _vp), ("lens", _vp), ("table_stride", C.c_int64),
                 ("prefix_len", C.c_int32), ("max_len", C.c_int32), ("batch", C.c_int32),
                 ("scale", C.c_float)]
 
@@ -165,6 +165,8 @@ _batch_append = _sig("kvx_batch_append", C.c_int,
 _batch_attend = _sig("kvx_batch_attend", C.c_int, [_vp, C.POINTER(kvx_attend), _vp])
 _batch_check = _sig("kvx_batch_check", C.c_int, [_vp])
 _batch_destroy = _sig("kvx_batch_destroy", None, [_vp])
+_prefix_create = _sig("kvx_prefix_create", C.c_int, [_vp, C.c_int, C.c_int, C.POINTER(_vp)])
+_prefix_destroy = _sig("kvx_prefix_destroy", None, [_vp])
 
 # Every symbol the C header declares, for load/export checks.
 EXPORTED = [
@@ -175,7 +177,7 @@ EXPORTED = [
     "kvx_synth_bf16", "kvx_hbm_read_probe", "kvx_attention_decode_noalloc", "kvx_fold_shards",
     "kvx_exponent_stats", "kvx_encode_bf16_bits", "kvx_encode_batch_bits", "kvx_cache_append_bits",
     "kvx_batch_create", "kvx_batch_rotate", "kvx_batch_append", "kvx_batch_attend",
-    "kvx_batch_check", "kvx_batch_destroy",
+    "kvx_batch_check", "kvx_batch_destroy", "kvx_prefix_create", "kvx_prefix_destroy",
 ]
 
 # Residual code widths the encoder may use (include/kvexp_b200.h KVX_CODE_BITS_*): the reference's
@@ -532,6 +534,62 @@ class Pages:
         self._ref = C.pointer(self._c)
 
 
+class Prefix:
+    """A shared prefix kept as XKV blobs (kvx_prefix): one kvx_unit (make_unit without queries) for
+    each KV head.  `keep` holds what the units point into."""
+
+    def __init__(self, units, dim, keep=None):
+        self._h = None
+        self._keep = keep
+        self.dim, self.n_heads = int(dim), len(units)
+        self.seq = int(units[0].seq) if units else 0
+        self.nbytes = sum(int(u.k_bytes) + int(u.v_bytes) for u in units)
+        arr = (kvx_unit * len(units))(*units)
+        h = _vp()
+        _check(_prefix_create(C.cast(arr, _vp), len(units), self.dim, C.byref(h)))
+        self._h = h
+
+    @classmethod
+    def encode(cls, k, v, block_tokens=K_ENCODE_BLOCK, code_bits=CODE_BITS_REFERENCE):
+        """Encodes k and v (BF16 CUDA tensors [n_kv_heads, tokens, dim], contiguous) on the GPU."""
+        import torch
+        for name, x in (("k", k), ("v", v)):
+            _device_tensor(x, name, "torch.bfloat16", 3)
+            if not x.is_contiguous() or x.shape != k.shape:
+                raise ValueError("k and v must be contiguous and of one shape")
+        heads, seq, dim = (int(n) for n in k.shape)
+        if heads == 0 or seq == 0:
+            raise ValueError("an empty prefix")
+        bound, entries = encode_batch_bounds(2 * heads, seq, dim, block_tokens)
+        arena = torch.empty(bound, dtype=torch.uint8, device=k.device)
+        index = torch.empty(entries * C.sizeof(kvx_block), dtype=torch.uint8, device=k.device)
+        torch.cuda.current_stream(k.device).synchronize()
+        off, nb = encode_batch([x for h in range(heads) for x in (k[h], v[h])], seq, dim, arena, index,
+                               block_tokens, code_bits=code_bits)
+        blobs = arena[:int(off[-1] + nb[-1] + 31) & ~15].clone()  # the bound is of incompressible data
+        blocks = -(-seq // block_tokens)
+        torch.cuda.current_stream(k.device).synchronize()
+
+        def unit(h):
+            at = [blobs.data_ptr() + int(off[2 * h + i]) for i in (0, 1)]
+            ix = [index.data_ptr() + (2 * h + i) * blocks * C.sizeof(kvx_block) for i in (0, 1)]
+            return make_unit(at[0], at[1], None, None, k_index=ix[0], v_index=ix[1], k_bytes=nb[2 * h],
+                             v_bytes=nb[2 * h + 1], n_blocks=blocks, seq=seq)
+
+        return cls([unit(h) for h in range(heads)], dim, keep=(blobs, index))
+
+    def close(self):
+        if self._h:
+            _prefix_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Batch:
     """The operators of a batch's serving step (kvx_batch) for one head layout and type ("bf16" or
     "fp16"), with scratch for up to max_batch sequences."""
@@ -582,10 +640,10 @@ class Batch:
             None if q is None else self._view(q_out, "q_out", n, self.n_q_heads), n,
             None if rope is None else rope._at(pos, n), slots.data_ptr(), self._pages(pages), stream))
 
-    def attend(self, q, out, pages, table, lens, max_len, *, prefix_table=None, prefix_len=0, scale=None,
-               lse=None, stream=None):
+    def attend(self, q, out, pages, table, lens, max_len, *, prefix_table=None, prefix_len=0, prefix=None,
+               scale=None, lse=None, stream=None):
         """out[b, h] = attention of q [batch, n_q_heads, dim] over the shared prefix (prefix_len
-        tokens in the pages of prefix_table, int32) and then the first lens[b] tokens of row b of
+        tokens in the pages of prefix_table, int32, or a Prefix) and then the first lens[b] tokens of row b of
         table (int32 [batch, pages]); max_len bounds lens.  lse [batch, n_q_heads] FP32 receives
         the log-sum-exp of the scaled scores."""
         n = int(q.shape[0])
@@ -612,8 +670,8 @@ class Batch:
         if scale is not None and not scale > 0:
             raise ValueError("scale must be positive")
         a = kvx_attend(self._view(q, "q", n, self.n_q_heads), self._view(out, "out", n, self.n_q_heads),
-                       None if lse is None else lse.data_ptr(), self._pages(pages), at_prefix, at_table,
-                       at_lens, stride, prefix_len, max_len, n, 0.0 if scale is None else scale)
+                       None if lse is None else lse.data_ptr(), self._pages(pages), at_prefix,
+                       None if prefix is None else prefix._h, at_table, at_lens, stride, prefix_len, max_len, n, 0.0 if scale is None else scale)
         _check(_batch_attend(self._h, a, stream))
 
     def check(self):

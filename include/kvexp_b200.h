@@ -261,6 +261,7 @@ KVX_API int kvx_attention_decode_noalloc(const uint16_t *q, const uint8_t *k_xkv
 #define KVX_DTYPE_FP16 1
 
 typedef struct kvx_batch_s *kvx_batch;
+typedef struct kvx_prefix_s *kvx_prefix;
 
 /* [n_tokens, n_heads, dim] values of the batch's type in device memory: dim contiguous, strides in
  * elements.  Any strides and alignment work; 16-byte aligned rows take the vector path. */
@@ -300,13 +301,15 @@ typedef struct kvx_rope {
     int32_t interleaved;
 } kvx_rope;
 
-/* One attention call. */
+/* One attention call.  The shared prefix in one of two forms, or neither: prefix_table with
+ * prefix_len tokens in pages, or `prefix` (XKV blobs, kvx_prefix_create; a BF16 batch). */
 typedef struct kvx_attend {
     kvx_view q;                  /* token = sequence: [batch, n_q_heads, dim] */
     kvx_view out;                /* the same shape and type */
     float *lse;                  /* optional [batch, n_q_heads] FP32: log-sum-exp of the scaled scores */
     const kvx_pages *pages;
     const int32_t *prefix_table; /* pages of the shared prefix */
+    kvx_prefix prefix;           /* or its XKV blobs */
     const int32_t *table;        /* pages of each sequence: rows table_stride apart */
     const int32_t *lens;         /* [batch] tokens in each sequence's own pages */
     int64_t table_stride;
@@ -338,10 +341,18 @@ KVX_API int kvx_batch_append(kvx_batch batch, const kvx_view *q, const kvx_view 
  * last token is never used, whatever its bits. */
 KVX_API int kvx_batch_attend(kvx_batch batch, const kvx_attend *args, void *stream);
 /* Synchronise and report device-side errors since the last check: a position outside the tables or
- * a slot outside the pools (what they concern was not written), a table entry outside the pools (its tokens
- * were left out) or a length outside [0, max_len] (clamped). */
+ * a slot outside the pools (what they concern was not written), a table entry outside the pools (it is
+ * not read: the outputs that need it mean nothing) or a length outside [0, max_len] (clamped). */
 KVX_API int kvx_batch_check(kvx_batch batch);
 KVX_API void kvx_batch_destroy(kvx_batch batch);
+
+/* A shared prefix kept as XKV blobs: heads[h] gives KV head h's k, v, k_index, v_index, k_bytes,
+ * v_bytes, n_blocks and seq (the same n_blocks and seq for every head; q, out and lse are not used).
+ * Synchronous; checks the blobs like kvx_plan_create.  Holds a table of the blobs' 16-token groups,
+ * escape records and merge words (about 4 % of the blobs' bytes at dim 64); the blobs themselves
+ * stay the caller's and are read by every kvx_batch_attend. */
+KVX_API int kvx_prefix_create(const kvx_unit *heads, int n_kv_heads, int dim, kvx_prefix *prefix);
+KVX_API void kvx_prefix_destroy(kvx_prefix prefix);
 
 /* ---- benchmark support -------------------------------------------------------------------- */
 

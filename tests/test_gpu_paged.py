@@ -333,6 +333,96 @@ def test_attend_in_a_graph_on_a_stream(kvx, cuda, H):
     b.check()
 
 
+# ---- a prefix kept as XKV blobs ---------------------------------------------------------------------
+
+def _modes(torch, seq, heads, dim, block, seed, special=0.01):
+    """[heads, seq, dim] BF16 whose blocks favour raw, 2-, 3- and 4-bit residuals in turn, with escapes."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    spread = torch.tensor([3, 7, 15, 60], device="cuda")[(torch.arange(seq, device="cuda") // block + seed) % 4]
+    e = 126 - (torch.rand((heads, seq, dim), generator=g, device="cuda") * spread[None, :, None]).long()
+    far = torch.rand(e.shape, generator=g, device="cuda") < special
+    e = torch.where(far, torch.randint(60, 127, e.shape, generator=g, device="cuda"), e)
+    bits = (torch.randint(0, 2, e.shape, generator=g, device="cuda") << 15) | (e << 7) | torch.randint(
+        0, 128, e.shape, generator=g, device="cuda")
+    bits = torch.where(bits >= 32768, bits - 65536, bits).to(torch.int16)
+    return bits.view(torch.bfloat16)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,seq,lens,block,bits", [
+    (1, 1, 64, 1, [0], 128, 0x14), (14, 2, 64, 1000, [3, 0, 40], 128, 0x14), (14, 2, 64, 1000, [3, 0, 40], 128, 0x1C),
+    (8, 2, 128, 700, [0] * 40, 128, 0x1C), (32, 8, 128, 2111, [100] * 9, 128, 0x14), (6, 3, 32, 999, [70] * 70, 128, 0x1C),
+    (4, 2, 256, 515, [17, 0, 5], 128, 0x1C), (8, 4, 64, 777, [9] * 4, 32, 0x1C), (4, 1, 128, 900, [1] * 40, 255, 0x1C),
+    (4, 4, 64, 300, [0] * 3, 7, 0x14), (12, 2, 64, 20000, [64] * 12, 128, 0x1C),
+])
+def test_attend_xkv(kvx, cuda, H, hq, hkv, dim, seq, lens, block, bits):
+    torch = cuda
+    k, v = _modes(torch, seq, hkv, dim, block, 0), _modes(torch, seq, hkv, dim, block, 1, special=0.1)
+    c = H.Paged(len(lens), hq, hkv, dim, 0, lens, 16, paged_prefix=False, q_scale=0.7)
+    c.prefix = (k.transpose(0, 1), v.transpose(0, 1))
+    prefix = kvx.Prefix.encode(k, v, block_tokens=block, code_bits=bits)
+    b, pages = kvx.Batch(len(lens), hq, hkv, dim), kvx.Pages(c.k_pool, c.v_pool)
+    out = torch.full((len(lens), hq, dim), 7.0, device="cuda", dtype=torch.bfloat16)
+    lse = torch.full((len(lens), hq), 7.0, device="cuda")
+    for _ in range(2):
+        b.attend(c.q, out, pages, c.table, c.lens, c.max_len, prefix=prefix, lse=lse)
+    b.check()
+    H.assert_attends(out, lse, c.truth())
+    if block == 128 and len(lens) * (hq // hkv) > 8:
+        # the same tiles reach the tensor cores as from pages: the same bits
+        page = 16
+        n = -(-seq // page)
+        kp = torch.full((n + c.k_pool.shape[0], page, hkv, dim), math.nan, device="cuda", dtype=torch.bfloat16)
+        vp = kp.clone()
+        table = torch.arange(n, device="cuda", dtype=torch.int32)
+        t = torch.arange(seq, device="cuda")
+        kp[t // page, t % page], vp[t // page, t % page] = c.prefix
+        kp[n:], vp[n:] = c.k_pool, c.v_pool
+        same = torch.empty_like(out)
+        b.attend(c.q, same, kvx.Pages(kp, vp), c.table + n, c.lens, c.max_len, prefix_table=table, prefix_len=seq)
+        b.check()
+        assert torch.equal(same, out)
+
+
+def test_xkv_prefix_special_values(kvx, cuda, H):
+    """Every BF16 class goes through the decoder: V columns of zeros, subnormals and a NaN or infinity."""
+    torch = cuda
+    k, v = _modes(torch, 200, 1, 64, 128, 2), _modes(torch, 200, 1, 64, 128, 3)
+    v[0, :, 0], v[0, :, 1], v[0, 150, 2], v[0, 20, 3] = 0.0, 1e-40, math.nan, math.inf
+    c = H.Paged(10, 1, 1, 64, 0, [0] * 10, 16, paged_prefix=False)
+    out = torch.empty((10, 1, 64), device="cuda", dtype=torch.bfloat16)
+    b = kvx.Batch(10, 1, 1, 64)
+    b.attend(c.q, out, kvx.Pages(c.k_pool, c.v_pool), None, None, 0, prefix=kvx.Prefix.encode(k, v))
+    b.check()
+    assert bool((out[..., 0] == 0).all()) and bool(out[..., 2].isnan().all()) and bool((out[..., 3] == math.inf).all())
+    assert bool((out[..., 1].abs() < 1e-38).all()) and bool(out[..., 4:].isfinite().all())
+
+
+def test_xkv_prefix_refusals(kvx, cuda, H):
+    torch = cuda
+    k = _modes(torch, 300, 2, 64, 128, 0)
+    p = kvx.Prefix.encode(k, k)
+    c = H.Paged(2, 4, 2, 64, 16, [4, 4], 16)
+    pages, out = kvx.Pages(c.k_pool, c.v_pool), torch.empty((2, 4, 64), device="cuda", dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="one prefix"):
+        kvx.Batch(2, 4, 2, 64).attend(c.q, out, pages, c.table, c.lens, 4, prefix=p, prefix_table=c.prefix_table, prefix_len=16)
+    one = H.Paged(2, 4, 1, 64, 16, [4, 4], 16)
+    with pytest.raises(ValueError, match="other heads"):
+        kvx.Batch(2, 4, 1, 64).attend(one.q, out, kvx.Pages(one.k_pool, one.v_pool), one.table, one.lens, 4, prefix=p)
+    half = H.Paged(2, 4, 2, 64, 16, [4, 4], 16, dtype="fp16")
+    with pytest.raises(ValueError, match="BF16"):
+        kvx.Batch(2, 4, 2, 64, dtype="fp16").attend(half.q, out.half(), kvx.Pages(half.k_pool, half.v_pool), half.table,
+                                                    half.lens, 4, prefix=p)
+    blobs, index = p._keep
+    at = blobs.data_ptr()
+    short = kvx.make_unit(at, at, None, None, k_index=index, v_index=index, k_bytes=100, v_bytes=100, n_blocks=3, seq=300)
+    with pytest.raises(RuntimeError, match="xkv"):  # blobs shorter than their index says
+        kvx.Prefix([short], 64)
+    with pytest.raises(ValueError, match="index"):
+        kvx.Prefix([kvx.make_unit(at, at, None, None, seq=300)], 64)
+    with pytest.raises(ValueError, match="empty"):
+        kvx.Prefix.encode(k[:, :0].contiguous(), k[:, :0].contiguous())
+
+
 # ---- refusals and device-side reports ---------------------------------------------------------------
 
 def test_reports(kvx, cuda, H):
