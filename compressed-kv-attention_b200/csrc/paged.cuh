@@ -53,7 +53,7 @@ struct RotArgs {
     int *status;
     int32_t n_pos, rot_dim, n_axes, interleaved, inverse;
     int32_t n_tokens, dim, heads;    // heads: of all segments together
-    int32_t tokens_per_cta;
+    int32_t tokens_per_cta, head_slots;
 };
 
 cudaError_t launch_rotate(int dtype, bool vec, const RotArgs &a, cudaStream_t s);
@@ -103,6 +103,7 @@ struct PagedArgs {
     // split_tiles tiles of kPrefixTile tokens (the last fewer) of prefix_tiles for each of the head's
     // batch * group rows, in row_groups items of kPrefixRows rows.
     int32_t n_split, row_pad, split_tiles, prefix_tiles, row_groups;
+    int32_t box_tokens, heads_inside;   // TMA boxes of the pools (see the kernel)
     // Streamed units, laid end to end in 16-token tiles: first (a streamed prefix) KV head by KV
     // head and group of 8 rows, prefix_len tokens each; then sequence by sequence, KV head by KV
     // head, group of 8 heads by group, the sequence's own tokens.  The tiles are cut into as many

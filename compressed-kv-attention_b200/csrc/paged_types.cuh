@@ -66,8 +66,8 @@ __device__ __forceinline__ int tail_len(const PagedArgs &a, int b) {
 
 // A launch that may be set up while the grid before it in the stream drains (programmatic dependent
 // launch; every kernel launched so waits for that grid itself).
-template <class K>
-cudaError_t launch_paged(K k, dim3 grid, int threads, int smem, cudaStream_t s, const PagedArgs &a) {
+template <class K, class... More>
+cudaError_t launch_paged(K k, dim3 grid, int threads, int smem, cudaStream_t s, const PagedArgs &a, const More &...more) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(unsigned(threads));
@@ -78,7 +78,7 @@ cudaError_t launch_paged(K k, dim3 grid, int threads, int smem, cudaStream_t s, 
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, k, a);
+    return cudaLaunchKernelEx(&cfg, k, a, more...);
 }
 
 }  // namespace kvx

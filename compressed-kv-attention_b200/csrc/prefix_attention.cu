@@ -5,11 +5,13 @@
 // to 128 rows a CTA, so a piece of the prefix is read once for 128 rows.  One CTA takes one item:
 // a KV head, 128 of its rows and a run of 64-token tiles; it leaves one partial state per row.
 //
-//  * Warps 4-6 load: each K or V tile goes by 16-byte asynchronous copies into a slot of a
-//    shared-memory ring in the layout the tensor cores read (rows of 128 bytes, 16-byte pieces
-//    XOR-swizzled by the row; 64-byte rows at D = 32).  Copies by row take pages of any length and
-//    strides, and fill the rows past the run's end with zeros.
-//  * Warp 7 issues the MMAs (one thread): S(i) = Q K(i)^T into one of two TMEM buffers, then
+//  * The loader warps bring each K or V tile into a slot of a shared-memory ring in the layout the
+//    tensor cores read (rows of 128 bytes, 16-byte pieces XOR-swizzled by the row; 64-byte rows at
+//    D = 32).  From pages whose length is a multiple of 8 one warp does it with TMA: a tile is
+//    64 / R boxes of R tokens (R the power of two, at most 64, that divides the page) a panel.  For
+//    other lengths three warps copy row by row, 16 bytes a thread.  (TMA for the long pages is what
+//    lets the other roles run: the row copies take about 1600 cycles a tile of 128 dims.)
+//  * One more warp issues the MMAs (one thread): S(i) = Q K(i)^T into one of two TMEM buffers, then
 //    O += P(i - 1) V(i - 1) with P read from TMEM (it replaces S there), so that S(i) is computed
 //    while the softmax of tile i - 1 runs.  V is the N-major operand: the same rows as stored.
 //  * Warps 0-3 do the softmax, a thread to a row: no shuffles.  The maximum that weights are
@@ -27,6 +29,10 @@
 // cycles, the MMAs 4 D (256 at D = 64, 512 at D = 128) and the tile's bytes from HBM 256 D / 23
 // (712 at D = 64, 1425 at D = 128, shared by all 128-row items of the head through L2).  Two CTAs
 // a SM (one at D = 256) overlap one's softmax with the other's waits.
+#include <cuda.h>
+
+#include <utility>
+
 #include "attention.cuh"
 #include "paged_types.cuh"
 #include "xkv_decode.cuh"
@@ -37,15 +43,26 @@ namespace {
 constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int TT = kPrefixTile;         // tokens per tile
 constexpr int ROWS = kPrefixRows;       // query rows per item
-constexpr int SW = 4, LW = 3;           // softmax and loader warps
-constexpr int THREADS = 32 * (SW + LW + 1);
+constexpr int SW = 4;                   // softmax warps
 constexpr uint32_t kWaitUs = 1000000;   // bounded waits
 
-template <int D, bool XKV> struct Cfg {
+// Tensor maps of the K and V pools (LOAD_TMA).
+struct alignas(64) PrefixMaps {
+    CUtensorMap k, v;
+};
+
+// How the loader warps get the tiles: TMA boxes of whole page pieces, copies by row, or XKV blobs.
+enum { LOAD_TMA, LOAD_ROWS, LOAD_XKV };
+
+template <int D, int LOAD> struct Cfg {
+    static constexpr bool XKV = LOAD == LOAD_XKV;
+    static constexpr int LW = LOAD == LOAD_TMA ? 1 : 3;     // loader warps
+    static constexpr int THREADS = 32 * (SW + LW + 1);
     static constexpr int ROWB = D >= 64 ? 128 : 64;         // bytes of a row of one panel of head dims
     static constexpr int SLOT = TT * D * 2;
     static constexpr int NSLOT = XKV ? (D == 32 ? 8 : (D == 64 ? 6 : 3)) : (D == 32 ? 12 : (D == 64 ? 10 : 5));
-    static constexpr int LAG = NSLOT - 2;                   // tiles in flight before one is announced
+    static constexpr int LAG = NSLOT / 2;                   // row copies: tiles in flight before one is announced
+    static constexpr int PANELS = D >= 64 ? D / 64 : 1;
     static constexpr int CTAS = D == 256 ? 1 : 2;           // per SM
     static constexpr int O_Q = 0;
     static constexpr int O_RING = ROWS * D * 2;
@@ -56,13 +73,14 @@ template <int D, bool XKV> struct Cfg {
     static constexpr int STAGE = S_CODES + 8 * D + 32;
     static constexpr int O_STAGE = O_RING + NSLOT * SLOT;
     static constexpr int O_BAR = O_STAGE + LW * NSTAGE * STAGE;
-    static constexpr int N_BAR = 2 * NSLOT + 6 + LW * NSTAGE;
+    static constexpr int N_BAR = 2 * NSLOT + 7 + LW * NSTAGE;
     static constexpr int SMEM = O_BAR + 8 * N_BAR + 16;
     // arrivals that announce a tile: one of each loader warp, or one for each 16-token group
-    static constexpr int ARRIVE = XKV ? TT / 16 : LW;
+    static constexpr int ARRIVE = XKV ? TT / 16 : LW;  // (TMA: with the bytes)
     static constexpr int LDO = D + 4;                       // floats of a staged output row
     static constexpr int TMEM = D == 256 ? 512 : 256;       // columns: O at 0, S / P buffers at D, D + 64
     static constexpr uint64_t LAYOUT = D >= 64 ? 2 : 4;     // 128- / 64-byte swizzle
+    static_assert(PANELS * (TT / 8) <= 32, "a lane for each TMA box");
     static_assert(LAG < NSLOT - 1, "the tile that frees the ring's next slot has been announced");
     static_assert(ROWS * LDO * 4 <= O_BAR, "the staged outputs fit where Q and the ring were");
     static_assert(D + 2 * TT <= TMEM && CTAS * TMEM <= 512, "TMEM columns");
@@ -149,9 +167,17 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live)
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// One TMA box global -> shared, completing its bytes on `bar`.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+
 // Barriers of a CTA (8 bytes each): full and empty of every ring slot, these, then one for each
 // staging slot.
-enum { B_S0, B_S1, B_P0, B_P1, B_PV, B_Q, B_COUNT };
+enum { B_S0, B_S1, B_P0, B_P1, B_PV, B_Q, B_END, B_COUNT };
 
 // One item.
 struct Item {
@@ -213,9 +239,12 @@ __device__ __forceinline__ void decode_group(uint32_t stage_rows, uint32_t stage
     }
 }
 
-template <int D, int DT, bool XKV>
-__global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(const PagedArgs a) {
-    using C = Cfg<D, XKV>;
+template <int D, int DT, int LOAD>
+__global__ void __launch_bounds__(Cfg<D, LOAD>::THREADS, Cfg<D, LOAD>::CTAS)
+prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
+    using C = Cfg<D, LOAD>;
+    constexpr bool XKV = C::XKV;
+    constexpr int LW = C::LW;
     extern __shared__ __align__(1024) uint8_t smem[];
     volatile uint32_t *tmem_base = reinterpret_cast<volatile uint32_t *>(smem + C::O_BAR + 8 * C::N_BAR);
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -243,7 +272,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
         for (int i = 0; i < C::NSLOT; ++i) mbar_init(full(i), C::ARRIVE), mbar_init(empty(i), 1);
         for (int i = 0; i < LW * C::NSTAGE; ++i) mbar_init(bar(B_COUNT + i), 1);
         mbar_init(bar(B_S0), 1), mbar_init(bar(B_S1), 1), mbar_init(bar(B_P0), SW), mbar_init(bar(B_P1), SW);
-        mbar_init(bar(B_PV), 1), mbar_init(bar(B_Q), SW);
+        mbar_init(bar(B_PV), 1), mbar_init(bar(B_Q), SW), mbar_init(bar(B_END), 1);
         fence_mbar_init();
     }
     fence_before();
@@ -353,6 +382,68 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
             // after a wait that ran out: let the copies in flight land before the memory goes away
             if (!ok)
                 for (; k < issued; ++k) mbar_wait_bounded(staged(k), uint32_t((k / NS) & 1), kWaitUs);
+        } else if constexpr (LOAD == LOAD_TMA) {
+            // Lane i loads box i of a tile: box_tokens tokens of one panel of 64 head dims.  pages of the
+            // latest K tile, of the one before it (V follows a tile behind) and of the next; -1: no
+            // tokens there.
+            const int box = a.box_tokens, per = TT / box;
+            const int p = lane / per, t = (lane - p * per) * box;
+            const uint32_t at = uint32_t(p * (TT * C::ROWB) + t * C::ROWB), bytes = uint32_t(box * C::ROWB);
+            int place_k = 0, place_before = 0, place_next = 0;
+            // (nothing looks at the entry before the next K tile: its load is not waited for here)
+            auto look_up = [&](int tile, int &place) -> int32_t {
+                const int tok = (it.tile0 + tile) * TT + t;
+                place = -1;
+                if (tile >= it.tiles || p >= C::PANELS || tok >= a.prefix_len) return 0;
+                int64_t i;
+                a.pool.split.at(tok, i, place);
+                return __ldg(a.prefix_table + i);
+            };
+            int32_t pg_k = 0, pg_before = 0, pg_next = look_up(0, place_next);
+            bool ok = true;
+            int q = 0;
+            for (; q < 2 * it.tiles; ++q) {
+                const bool last = q == 2 * it.tiles - 1, is_v = is_v_item(q);
+                if (!is_v) {
+                    pg_before = pg_k, place_before = place_k;
+                    pg_k = pg_next, place_k = place_next;
+                    pg_next = look_up((q + 1) / 2 + 1, place_next);
+                }
+                if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
+                if (!ok) break;
+                const bool before = is_v && !last;
+                const int32_t pg = before ? pg_before : pg_k;
+                const int place = before ? place_before : place_k;
+                bool live = place >= 0;
+                if (live && unsigned(pg) >= unsigned(a.pool.n_pages)) {
+                    report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
+                    live = false;
+                }
+                const uint32_t dst = sb + uint32_t(C::O_RING + (q % C::NSLOT) * C::SLOT);
+                // V rows past the prefix's end meet weights of 0 and must be finite: that tile's boxes
+                // are waited for here and the rows zeroed before the tile is announced
+                const int valid = a.prefix_len - (it.tile0 + (last ? it.tiles : q / 2) - 1) * TT;
+                const bool ends = is_v && valid < TT;
+                const uint32_t to = ends ? bar(B_END) : full(q);
+                const uint32_t boxes = uint32_t(__popc(__ballot_sync(FULL, live)));
+                if (lane == 0) mbar_arrive_expect_tx(to, boxes * bytes);
+                __syncwarp();
+                if (live)
+                    tma_load(dst + at, is_v ? &maps.v : &maps.k, p * 64, a.heads_inside ? it.head : place,
+                             a.heads_inside ? place : it.head, pg, to);
+                if (ends) {
+                    ok = __all_sync(FULL, wait(to, 0));
+                    if (!ok) break;
+                    for (int i = lane; i < (TT - valid) * (D / 8); i += 32)
+                        sts_v4(dst + tile_off<D, TT>(valid + i / (D / 8), i % (D / 8)), 0u, 0u, 0u, 0u);
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full(q));
+                }
+            }
+            // after a wait that ran out: let the boxes in flight land before the memory goes away
+            if (!ok)
+                for (int i = max(0, q - C::NSLOT); i < q; ++i) mbar_wait_bounded(full(i), uint32_t((i / C::NSLOT) & 1), kWaitUs);
         } else {
         // Loader warp w copies rows w, w + LW, ... of every tile: lane k holds the offset of row w +
         // LW k (-1: no such token), looked up a tile ahead of its use.
@@ -360,9 +451,21 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
         constexpr int MINE = (TT + LW - 1) / LW, STEPS = (MINE + RPS - 1) / RPS;
         const int w = warp - SW, c = lane % CH;
         const int64_t head = int64_t(it.head) * a.pool.head_stride + 8 * c;
-        auto look_up = [&](int tile) -> int64_t {
+        // (nothing looks at the entry before the next K tile: its load is not waited for here)
+        int place_next = -1;
+        auto look_up = [&](int tile) -> int32_t {
             const int r = w + LW * lane, tok = (it.tile0 + tile) * TT + r;
-            return r < TT && tok < a.prefix_len && tile < it.tiles ? page_row(a.pool, a.prefix_table, tok, a.status) : -1;
+            place_next = -1;
+            if (r >= TT || tok >= a.prefix_len || tile >= it.tiles) return 0;
+            int64_t i;
+            a.pool.split.at(tok, i, place_next);
+            return __ldg(a.prefix_table + i);
+        };
+        auto row_of = [&](int32_t page, int place) -> int64_t {
+            if (place < 0) return -1;
+            if (unsigned(page) < unsigned(a.pool.n_pages)) return int64_t(page) * a.pool.page_stride + int64_t(place) * a.pool.token_stride;
+            report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
+            return -1;
         };
         auto announce = [&](int i) {
             proxy_fence();
@@ -370,15 +473,16 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
             if (lane == 0) mbar_arrive(full(i));
         };
         // rows of the latest K tile, of the one before it (V follows a tile behind) and of the next
-        int64_t r_k = -1, r_before = -1, r_next = look_up(0);
+        int64_t r_k = -1, r_before = -1;
+        int32_t pg_next = look_up(0);
         bool ok = true;
         int q = 0;
         for (; q < 2 * it.tiles; ++q) {
             const bool last = q == 2 * it.tiles - 1, is_v = is_v_item(q);
             if (!is_v) {
                 r_before = r_k;
-                r_k = r_next;
-                r_next = look_up((q + 1) / 2 + 1);
+                r_k = row_of(pg_next, place_next);
+                pg_next = look_up((q + 1) / 2 + 1);
             }
             if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
             if (!ok) break;
@@ -406,17 +510,20 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
         if (lane == 0 && wait(bar(B_Q), 0)) {
             constexpr uint32_t qk = instr_desc<DT>(TT, false), pv = instr_desc<DT>(D, true);
             constexpr uint32_t K8 = 8 * C::ROWB;  // bytes of 8 rows
+            // descriptors of a tile are its base's plus steps of the start address
+            const uint64_t q0 = smem_desc(sb + C::O_Q, 16, K8, C::LAYOUT), k0 = smem_desc(sb + C::O_RING, 16, K8, C::LAYOUT),
+                           v0 = smem_desc(sb + C::O_RING, TT * C::ROWB, K8, C::LAYOUT);
             for (int i = 0; i <= it.tiles; ++i) {
                 if (i < it.tiles) {
                     const int x = k_item(i);
                     if (!wait(full(x), x / C::NSLOT)) break;
                     fence_after();
-                    const uint32_t kq = sb + C::O_Q, kk = sb + uint32_t(C::O_RING + (x % C::NSLOT) * C::SLOT);
+                    const uint64_t kk = k0 + uint32_t(x % C::NSLOT) * uint32_t(C::SLOT / 16);
 #pragma unroll
                     for (int s = 0; s < D / 16; ++s) {
                         const uint32_t p = uint32_t(s / (C::ROWB / 32)), o = uint32_t(s % (C::ROWB / 32)) * 32;
-                        mma_ss(tm + D + (i & 1) * TT, smem_desc(kq + p * (ROWS * C::ROWB) + o, 16, K8, C::LAYOUT),
-                               smem_desc(kk + p * (TT * C::ROWB) + o, 16, K8, C::LAYOUT), qk, s > 0);
+                        mma_ss(tm + D + (i & 1) * TT, q0 + (p * (ROWS * C::ROWB) + o) / 16, kk + (p * (TT * C::ROWB) + o) / 16, qk,
+                               s > 0);
                     }
                     mma_commit(empty(x));
                     mma_commit(bar(B_S0 + (i & 1)));
@@ -425,10 +532,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
                     const int j = i - 1, x = v_item(j, it.tiles);
                     if (!wait(full(x), x / C::NSLOT) || !wait(bar(B_P0 + (j & 1)), j >> 1)) break;
                     fence_after();
-                    const uint32_t vv = sb + uint32_t(C::O_RING + (x % C::NSLOT) * C::SLOT);
+                    const uint64_t vv = v0 + uint32_t(x % C::NSLOT) * uint32_t(C::SLOT / 16);
 #pragma unroll
                     for (int s = 0; s < TT / 16; ++s)
-                        mma_ts(tm, tm + D + (j & 1) * TT + 8 * s, smem_desc(vv + 2 * s * K8, TT * C::ROWB, K8, C::LAYOUT),
+                        mma_ts(tm, tm + D + (j & 1) * TT + 8 * s, vv + 2 * s * K8 / 16,
                                pv, j > 0 || s > 0);
                     mma_commit(empty(x));
                     mma_commit(bar(B_PV));
@@ -559,17 +666,71 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, XKV>::CTAS) prefix_kernel(cons
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tm), "n"(C::TMEM) : "memory");
 }
 
-template <int D, int DT, bool XKV> cudaError_t prefix_launch(const PagedArgs &a, cudaStream_t s) {
-    using C = Cfg<D, XKV>;
+template <int D, int DT, int LOAD>
+cudaError_t prefix_launch(const PagedArgs &a, const PrefixMaps &maps, cudaStream_t s) {
+    using C = Cfg<D, LOAD>;
     static const cudaError_t attr =
-        cudaFuncSetAttribute(prefix_kernel<D, DT, XKV>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaFuncSetAttribute(prefix_kernel<D, DT, LOAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (attr != cudaSuccess) return attr;
-    return launch_paged(prefix_kernel<D, DT, XKV>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), THREADS, C::SMEM, s, a);
+    return launch_paged(prefix_kernel<D, DT, LOAD>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), C::THREADS, C::SMEM, s, a, maps);
 }
-template <int D, int DT> cudaError_t prefix_d(const PagedArgs &a, cudaStream_t s) {
+
+// The driver's tensor map encoder (found at run time: the library links no libcuda).
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn tensor_map_encoder() {
+    static const EncodeFn fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        cudaGetLastError();
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// Maps of one layer's pools with boxes of a.box_tokens tokens of 64 (32) head dims; the nearer of
+// tokens and heads inside (a.heads_inside).  false: the driver takes no such map.
+bool encode_maps(int dim, int dtype, PagedArgs &a, PrefixMaps &maps) {
+    const EncodeFn encode = tensor_map_encoder();
+    if (encode == nullptr) return false;
+    const PoolDev &p = a.pool;
+    // (a dimension of one element has no stride of its own: any will do)
+    const int64_t row = int64_t(dim) * 2;
+    const int64_t token = p.split.tokens > 1 ? p.token_stride * 2 : row, head = a.n_kv_heads > 1 ? p.head_stride * 2 : row,
+                  page = p.n_pages > 1 ? p.page_stride * 2 : row;
+    a.heads_inside = a.n_kv_heads > 1 && p.head_stride < p.token_stride;
+    if (token <= 0 || head <= 0 || page <= 0) return false;
+    const cuuint64_t tokens = cuuint64_t(p.split.tokens), heads = cuuint64_t(a.n_kv_heads), pages = cuuint64_t(p.n_pages);
+    const cuuint32_t b = cuuint32_t(a.box_tokens), inner = dim >= 64 ? 64u : 32u;
+    cuuint64_t dims[4] = {cuuint64_t(dim), tokens, heads, pages}, strides[3] = {cuuint64_t(token), cuuint64_t(head), cuuint64_t(page)};
+    cuuint32_t box[4] = {inner, b, 1u, 1u}, step[4] = {1u, 1u, 1u, 1u};
+    if (a.heads_inside) {
+        std::swap(dims[1], dims[2]);
+        std::swap(strides[0], strides[1]);
+        std::swap(box[1], box[2]);
+    }
+    const CUtensorMapDataType type = dtype == KVX_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapSwizzle swizzle = dim >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    for (int T = 0; T < 2; ++T)
+        if (encode(T ? &maps.v : &maps.k, type, 4, T ? p.v : p.k, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    return true;
+}
+
+template <int D, int DT> cudaError_t prefix_d(const PagedArgs &args, cudaStream_t s) {
+    PagedArgs a = args;
+    PrefixMaps maps{};
     if constexpr (DT == KVX_DTYPE_BF16)
-        if (a.xkv.blocks > 0) return prefix_launch<D, DT, true>(a, s);
-    return prefix_launch<D, DT, false>(a, s);
+        if (a.xkv.blocks > 0) return prefix_launch<D, DT, LOAD_XKV>(a, maps, s);
+    // boxes of fewer than 8 tokens would not fill a swizzle pattern
+    for (a.box_tokens = TT; a.pool.split.tokens % a.box_tokens != 0;) a.box_tokens >>= 1;
+    if (a.box_tokens >= 8 && encode_maps(D, DT, a, maps)) return prefix_launch<D, DT, LOAD_TMA>(a, maps, s);
+    return prefix_launch<D, DT, LOAD_ROWS>(a, maps, s);
 }
 
 // One thread per (flat block, tile): its eight groups and its token count.
@@ -608,7 +769,7 @@ __global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int
 
 }  // namespace
 
-int prefix_ctas_per_sm(int dim) { return dim == 256 ? Cfg<256, false>::CTAS : Cfg<128, false>::CTAS; }
+int prefix_ctas_per_sm(int dim) { return dim == 256 ? Cfg<256, LOAD_TMA>::CTAS : Cfg<128, LOAD_TMA>::CTAS; }
 
 cudaError_t launch_xkv_groups(const BlockDesc *desc, int64_t n_blocks, int tiles_per_block, int dim, XkvGroup *groups,
                               uint8_t *tile_tokens, cudaStream_t s) {

@@ -58,28 +58,26 @@ __device__ __forceinline__ int table_row(const RotArgs &a, int token, int axis) 
     return -1;
 }
 
-// Cosines and sines of pairs [8 c, 8 c + 8) of a token.
-__device__ __forceinline__ bool load_angles(const RotArgs &a, int token, int c, float (&co)[8], float (&si)[8]) {
+// Cosines and sines of pairs p .. p + 3 of a token (p a multiple of 4).
+__device__ __forceinline__ bool load_angles(const RotArgs &a, int token, int p, float *co, float *si) {
     const int half = a.rot_dim >> 1;
-    uint2 ax = make_uint2(0u, 0u);
-    if (a.axis != nullptr) ax = __ldg(reinterpret_cast<const uint2 *>(a.axis + 8 * c));
-    const uint32_t first = ax.x & 0xFFu;
-    if (ax.x == first * 0x01010101u && ax.y == ax.x) {  // the eight pairs turn about one axis
-        const int p = table_row(a, token, int(first));
-        if (p < 0) return false;
-        const float4 *pc = reinterpret_cast<const float4 *>(a.cos + int64_t(p) * half + 8 * c);
-        const float4 *ps = reinterpret_cast<const float4 *>(a.sin + int64_t(p) * half + 8 * c);
-        const float4 c0 = __ldg(pc), c1 = __ldg(pc + 1), s0 = __ldg(ps), s1 = __ldg(ps + 1);
-        co[0] = c0.x, co[1] = c0.y, co[2] = c0.z, co[3] = c0.w, co[4] = c1.x, co[5] = c1.y, co[6] = c1.z, co[7] = c1.w;
-        si[0] = s0.x, si[1] = s0.y, si[2] = s0.z, si[3] = s0.w, si[4] = s1.x, si[5] = s1.y, si[6] = s1.z, si[7] = s1.w;
+    const uint32_t ax = a.axis != nullptr ? __ldg(reinterpret_cast<const uint32_t *>(a.axis + p)) : 0u;
+    const uint32_t first = ax & 0xFFu;
+    if (ax == first * 0x01010101u) {  // the four pairs turn about one axis
+        const int row = table_row(a, token, int(first));
+        if (row < 0) return false;
+        const float4 c = __ldg(reinterpret_cast<const float4 *>(a.cos + int64_t(row) * half + p));
+        const float4 s = __ldg(reinterpret_cast<const float4 *>(a.sin + int64_t(row) * half + p));
+        co[0] = c.x, co[1] = c.y, co[2] = c.z, co[3] = c.w;
+        si[0] = s.x, si[1] = s.y, si[2] = s.z, si[3] = s.w;
         return true;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int p = table_row(a, token, int(((i < 4 ? ax.x : ax.y) >> (8 * (i & 3))) & 0xFFu));
-        if (p < 0) return false;
-        co[i] = __ldg(a.cos + int64_t(p) * half + 8 * c + i);
-        si[i] = __ldg(a.sin + int64_t(p) * half + 8 * c + i);
+    for (int i = 0; i < 4; ++i) {
+        const int row = table_row(a, token, int((ax >> (8 * i)) & 0xFFu));
+        if (row < 0) return false;
+        co[i] = __ldg(a.cos + int64_t(row) * half + p + i);
+        si[i] = __ldg(a.sin + int64_t(row) * half + p + i);
     }
     return true;
 }
@@ -91,63 +89,134 @@ __device__ __forceinline__ void turn(float &x, float &y, float c, float s) {
     x = u;
 }
 
-// One thread per (token, head, 16 values): eight pairs -- two 16-byte pieces rot_dim / 2 apart, or
-// adjacent when interleaved -- or 16 values copied.  The operator moves four bytes a value and
-// computes three operations, so it is bound by HBM (and by the launch for a few tokens); the
-// tables' rows are shared by all heads of a token, which are neighbours in a CTA, and come from L1.
-template <int DT>
-__global__ void __launch_bounds__(256) rotate_vec_kernel(const RotArgs a) {
+// 16 bytes that are read or written once: past L1, which the tables' rows are to stay in.
+__device__ __forceinline__ uint4 load_once(const uint16_t *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ void store_once(uint16_t *p, const uint4 &v) {
+    asm volatile("st.global.L1::no_allocate.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Eight pairs of a head, their two pieces in x and y: pairs (x[i], y[i]), or the adjacent values of x
+// and then of y.
+template <int DT, bool INTER>
+__device__ __forceinline__ void turn8(uint4 &x, uint4 &y, const float (&co)[8], const float (&si)[8]) {
+    uint32_t *xw = &x.x, *yw = &y.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float2 u = Half2<DT>::up(xw[j]), w = Half2<DT>::up(yw[j]);
+        if constexpr (INTER) {
+            turn(u.x, u.y, co[j], si[j]);
+            turn(w.x, w.y, co[4 + j], si[4 + j]);
+        } else {
+            turn(u.x, w.x, co[2 * j], si[2 * j]);
+            turn(u.y, w.y, co[2 * j + 1], si[2 * j + 1]);
+        }
+        xw[j] = Half2<DT>::down(u.x, u.y);
+        yw[j] = Half2<DT>::down(w.x, w.y);
+    }
+}
+
+// Where a thread's two pieces of a head are (elements): half the rotated part apart, or half the rest,
+// or half of a head that is copied whole, so that a warp's accesses are whole lines either way.
+struct Pieces {
+    int first, apart;
+    bool turned;
+};
+__device__ __forceinline__ Pieces pieces_of(const RotArgs &a, const RotSeg &sg, int c) {
+    const int nr = sg.rotated ? a.rot_dim >> 4 : 0;  // pieces of the rotated part come first
+    if (c < nr) return {8 * c, a.rot_dim >> 1, true};
+    return {16 * nr + 8 * (c - nr), (a.dim - 16 * nr) >> 1, false};
+}
+template <bool INTER> __device__ __forceinline__ bool load_angles8(const RotArgs &a, int token, int c, float (&co)[8], float (&si)[8]) {
+    const bool ok = INTER ? load_angles(a, token, 4 * c, co, si) && load_angles(a, token, (a.rot_dim >> 2) + 4 * c, co + 4, si + 4)
+                          : load_angles(a, token, 8 * c, co, si) && load_angles(a, token, 8 * c + 4, co + 4, si + 4);
+    if (a.inverse) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) si[j] = -si[j];
+    }
+    return ok;
+}
+
+// Many tokens.  One thread per (token, 16 values of a head, head slot): it turns or copies them in
+// every head_slots-th head.  The operator moves four bytes a value and computes three operations: HBM
+// bounds it as long as a head's piece costs few instructions, so the angles are loaded and every
+// division is done once a thread.  On one B200: 16384 tokens of 32 + 2 x 8 heads of 128 into pages
+// 65.5 us (6.15 TB/s), 32768 tokens of 32 heads of 128 84 us (6.4 TB/s); with one thread a head and
+// piece 115 and 152 us, with four heads a thread instead of eight 67.5 and 85.
+template <int DT, bool INTER>
+__global__ void __launch_bounds__(256, 4) rotate_many_kernel(const __grid_constant__ RotArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int nc = a.dim >> 4, per = a.heads * nc;
-    const int t0 = blockIdx.x * a.tokens_per_cta;
-    const int n = min(a.tokens_per_cta, a.n_tokens - t0) * per;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const int token = t0 + i / per;
-        int r = i % per;
-        int head = r / nc, sgi = 0;
-        const int c = r - head * nc;
-        if (head >= a.seg[0].heads) {
-            head -= a.seg[0].heads;
-            sgi = 1;
-            if (head >= a.seg[1].heads) head -= a.seg[1].heads, sgi = 2;
-        }
-        const RotSeg &sg = a.seg[sgi];
-        uint16_t *out;
-        if (!dest(a, sg, token, head, out)) continue;
-        const uint16_t *in = sg.src + int64_t(token) * sg.src_token + int64_t(head) * sg.src_head;
-        const bool rot = sg.rotated && 16 * c < a.rot_dim;
-        int o0 = 16 * c, o1 = 16 * c + 8;
-        if (rot && !a.interleaved) o0 = 8 * c, o1 = 8 * c + (a.rot_dim >> 1);
-        uint4 x = *reinterpret_cast<const uint4 *>(in + o0);
-        uint4 y = *reinterpret_cast<const uint4 *>(in + o1);
-        if (rot) {
-            float co[8], si[8];
-            if (!load_angles(a, token, c, co, si)) continue;
-            uint32_t *xw = &x.x, *yw = &y.x;
-            const float sign = a.inverse ? -1.f : 1.f;
+    constexpr int G = 2;  // heads whose loads are in flight together
+    const int nc = a.dim >> 4;
+    const int c = int(threadIdx.x) % nc, r = int(threadIdx.x) / nc;
+    const int slot = r % a.head_slots, token = int(blockIdx.x) * a.tokens_per_cta + r / a.head_slots;
+    if (r >= a.tokens_per_cta * a.head_slots || token >= a.n_tokens) return;
+    float co[8], si[8];
+    const bool angles = 16 * c >= a.rot_dim || load_angles8<INTER>(a, token, c, co, si);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float2 u = Half2<DT>::up(xw[j]), w = Half2<DT>::up(yw[j]);
-                if (a.interleaved) {
-                    turn(u.x, u.y, co[j], sign * si[j]);
-                    turn(w.x, w.y, co[4 + j], sign * si[4 + j]);
-                } else {
-                    turn(u.x, w.x, co[2 * j], sign * si[2 * j]);
-                    turn(u.y, w.y, co[2 * j + 1], sign * si[2 * j + 1]);
+    for (int g = 0; g < 3; ++g) {
+        const RotSeg &sg = a.seg[g];
+        const Pieces p = pieces_of(a, sg, c);
+        uint16_t *out;
+        if (slot >= sg.heads || (p.turned && !angles) || !dest(a, sg, token, slot, out)) continue;
+        const uint16_t *in = sg.src + int64_t(token) * sg.src_token + int64_t(slot) * sg.src_head + p.first;
+        out += p.first;
+        const int64_t in_step = int64_t(a.head_slots) * sg.src_head,
+                      out_step = int64_t(a.head_slots) * (sg.pool != 0 ? a.pool.head_stride : sg.dst_head);
+        for (int h = slot; h < sg.heads; h += G * a.head_slots) {
+            uint4 x[G], y[G];
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+                if (h + k * a.head_slots < sg.heads) x[k] = load_once(in + k * in_step), y[k] = load_once(in + k * in_step + p.apart);
+#pragma unroll
+            for (int k = 0; k < G; ++k)
+                if (h + k * a.head_slots < sg.heads) {
+                    if (p.turned) turn8<DT, INTER>(x[k], y[k], co, si);
+                    store_once(out + k * out_step, x[k]);
+                    store_once(out + k * out_step + p.apart, y[k]);
                 }
-                xw[j] = Half2<DT>::down(u.x, u.y);
-                yw[j] = Half2<DT>::down(w.x, w.y);
-            }
+            in += G * in_step;
+            out += G * out_step;
         }
-        *reinterpret_cast<uint4 *>(out + o0) = x;
-        *reinterpret_cast<uint4 *>(out + o1) = y;
     }
+}
+
+// Few tokens: one thread per (token, head of any kind, 16 values), so that nothing follows anything but
+// the chain position -> angles.  One token of 14 + 2 x 2 heads of 64: 2 us, the launch.
+template <int DT, bool INTER>
+__global__ void __launch_bounds__(256) rotate_few_kernel(const __grid_constant__ RotArgs a) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const unsigned nc = unsigned(a.dim) >> 4, i = blockIdx.x * 256u + threadIdx.x, r = i / nc;
+    const int c = int(i - r * nc), token = int(r / unsigned(a.heads));
+    if (token >= a.n_tokens) return;
+    int head = int(r) - token * a.heads, g = 0;
+    if (head >= a.seg[0].heads) {
+        head -= a.seg[0].heads, g = 1;
+        if (head >= a.seg[1].heads) head -= a.seg[1].heads, g = 2;
+    }
+    const RotSeg &sg = a.seg[g];
+    const Pieces p = pieces_of(a, sg, c);
+    const uint16_t *in = sg.src + int64_t(token) * sg.src_token + int64_t(head) * sg.src_head + p.first;
+    uint4 x = load_once(in), y = load_once(in + p.apart);
+    uint16_t *out;
+    if (!dest(a, sg, token, head, out)) return;
+    if (p.turned) {
+        float co[8], si[8];
+        if (!load_angles8<INTER>(a, token, c, co, si)) return;
+        turn8<DT, INTER>(x, y, co, si);
+    }
+    store_once(out + p.first, x);
+    store_once(out + p.first + p.apart, y);
 }
 
 // The same for any even width, stride and alignment: one thread per (token, head, pair of values).
 template <int DT>
-__global__ void __launch_bounds__(256) rotate_any_kernel(const RotArgs a) {
+__global__ void __launch_bounds__(256) rotate_any_kernel(const __grid_constant__ RotArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int nc = a.dim >> 1, per = a.heads * nc, half = a.rot_dim >> 1;
@@ -186,14 +255,37 @@ __global__ void __launch_bounds__(256) rotate_any_kernel(const RotArgs a) {
 
 }  // namespace
 
+namespace {
+template <int DT> void (*kernel_of(const RotArgs &a, bool vec, bool many))(const RotArgs) {
+    if (!vec) return rotate_any_kernel<DT>;
+    if (many) return a.interleaved ? rotate_many_kernel<DT, true> : rotate_many_kernel<DT, false>;
+    return a.interleaved ? rotate_few_kernel<DT, true> : rotate_few_kernel<DT, false>;
+}
+}  // namespace
+
 cudaError_t launch_rotate(int dtype, bool vec, const RotArgs &args, cudaStream_t s) {
     if (args.n_tokens <= 0 || args.heads <= 0) return cudaSuccess;
     RotArgs a = args;
-    const int per = a.heads * (vec ? a.dim >> 4 : a.dim >> 1);
-    a.tokens_per_cta = per >= 256 ? 1 : 256 / per;
+    const int nc = a.dim >> 4;
+    // a thread for every piece while they fill the device only a few times over
+    const int64_t pieces = int64_t(a.n_tokens) * a.heads * nc;
+    const bool many = vec && pieces > int64_t(1) << 20;
+    int64_t ctas = (pieces + 255) / 256;
+    if (many || !vec) {
+        const int slots = vec ? 256 / nc : 0, per = a.heads * (a.dim >> 1);
+        if (many) {
+            int most = 0;
+            for (const RotSeg &sg : a.seg) most = sg.heads > most ? sg.heads : most;
+            a.head_slots = (most + 7) / 8 < slots ? (most + 7) / 8 : slots;
+            a.tokens_per_cta = slots / a.head_slots;
+        } else {
+            a.tokens_per_cta = per >= 256 ? 1 : 256 / per;
+        }
+        ctas = (a.n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta;
+    }
     // programmatic dependent launch: the kernel waits for the grid before it
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned((a.n_tokens + a.tokens_per_cta - 1) / a.tokens_per_cta));
+    cfg.gridDim = dim3(unsigned(ctas));
     cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -201,9 +293,7 @@ cudaError_t launch_rotate(int dtype, bool vec, const RotArgs &args, cudaStream_t
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (dtype == KVX_DTYPE_BF16)
-        return cudaLaunchKernelEx(&cfg, vec ? rotate_vec_kernel<KVX_DTYPE_BF16> : rotate_any_kernel<KVX_DTYPE_BF16>, a);
-    return cudaLaunchKernelEx(&cfg, vec ? rotate_vec_kernel<KVX_DTYPE_FP16> : rotate_any_kernel<KVX_DTYPE_FP16>, a);
+    return cudaLaunchKernelEx(&cfg, dtype == KVX_DTYPE_BF16 ? kernel_of<KVX_DTYPE_BF16>(a, vec, many) : kernel_of<KVX_DTYPE_FP16>(a, vec, many), a);
 }
 
 }  // namespace kvx

@@ -47,6 +47,15 @@ def test_rotate(kvx, cuda, H, tokens, heads, dim, rot, axes, interleaved, dtype,
         assert torch.equal(y, out)
 
 
+@pytest.mark.parametrize("tokens,heads,dim,rot,axes,interleaved,dtype", [
+    (4500, 40, 128, 128, 1, False, "bf16"), (9001, 17, 128, 96, 2, True, "fp16"), (2100, 33, 256, 64, 3, False, "bf16"),
+    (33000, 3, 224, 192, 1, True, "bf16"), (2500, 300, 32, 32, 1, False, "bf16"),
+])
+def test_rotate_many(kvx, cuda, H, tokens, heads, dim, rot, axes, interleaved, dtype):
+    """Over a million pieces: the kernel that turns several heads a thread."""
+    test_rotate(kvx, cuda, H, tokens, heads, dim, rot, axes, interleaved, dtype, False)
+
+
 @pytest.mark.parametrize("offset,pad", [(0, 0), (1, 0), (8, 8), (0, 1), (0, 4)])
 def test_rotate_strides_and_alignment(kvx, cuda, H, offset, pad):
     """Rows anywhere: odd starts and odd strides take the general kernel, with the same values."""
@@ -106,6 +115,7 @@ def test_rotate_gradient(kvx, cuda, H):
     (300, 8, 2, 128, 128, 1, 16, "hnd", "bf16"), (123, 6, 3, 64, 32, 3, 48, "nhd", "fp16"),
     (61, 4, 4, 256, 256, 1, 7, "nhd", "bf16"), (40, 3, 1, 32, 24, 2, 5, "hnd", "bf16"),
     (9, 2, 2, 64, 0, 1, 16, "nhd", "bf16"),
+    (4097, 32, 4, 128, 64, 1, 16, "hnd", "bf16"), (9000, 9, 9, 128, 128, 1, 48, "nhd", "fp16"),  # over a million pieces
 ])
 def test_append(kvx, cuda, H, tokens, hq, hkv, dim, rot, axes, page, layout, dtype):
     torch = cuda
