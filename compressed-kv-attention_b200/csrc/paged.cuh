@@ -120,7 +120,7 @@ struct PagedArgs {
 
 constexpr int kStreamWarps = 8;   // workers a CTA
 constexpr int kStreamTile = 16;   // tokens
-constexpr int kStreamLeast = 4;   // tiles a worker takes at least
+constexpr int kStreamLeast = 1;   // tiles a worker takes at least
 constexpr int kMaxStreamBatch = 4096;
 
 // Workers that share `tiles` tiles out of those launched.

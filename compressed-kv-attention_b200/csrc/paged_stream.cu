@@ -41,6 +41,7 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// 16 (8) bytes that are read once.
 __device__ __forceinline__ uint4 load16(const uint16_t *p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
             const int r = u.first + (g < u.n ? g : 0), b = r / a.group;
             const uint16_t *q = a.q + int64_t(b) * a.q_token + int64_t(u.head * a.group + r - b * a.group) * a.q_head + 8 * t;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) qf[j] = g < u.n ? load16(q + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < KJ; ++j) qf[j] = load16(q + 32 * j);  // (rows past n repeat the first)
         }
         const uint16_t *kb = a.pool.k + int64_t(u.head) * a.pool.head_stride + 8 * t;
         const uint16_t *vb = a.pool.v + int64_t(u.head) * a.pool.head_stride + 2 * VW * g;
@@ -186,32 +187,46 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
         for (int i = 0; i < VI * VW; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
         float m = -INFINITY, l = 0.f;
 
-        // the lanes look up the rows of the next tiles' tokens ahead of their use (-1: no such token)
+        // The lanes look up the pages of the next tiles' tokens ahead of their use; nothing looks at an
+        // entry before then, so its load is not waited for.  place -1: no such token.
         constexpr int LOOK = NT * TT > 32 ? 2 : 1;
-        int64_t nxt[LOOK];
+        int32_t page[LOOK], place[LOOK];
         auto look_up = [&](int tok0) {
 #pragma unroll
             for (int i = 0; i < LOOK; ++i) {
                 const int tok = tok0 + 32 * i + (NT * TT >= 32 ? lane : lane & 15);
-                nxt[i] = tok < t1 ? page_row(a.pool, u.table, tok, a.status) : -1;
+                page[i] = 0, place[i] = -1;
+                if (tok < t1) {
+                    int64_t at;
+                    a.pool.split.at(tok, at, place[i]);
+                    page[i] = __ldg(u.table + at);
+                }
             }
         };
         look_up(t0);
         for (int tok = t0; tok < t1; tok += NT * TT) {
+            // Rows of the tiles' tokens.  Where there is no token (the run's end, a bad entry) the pool's
+            // first row is loaded in its place and then replaced by zeros: loads that depend on a
+            // condition would be waited for one by one (3200 cycles an iteration).
             int64_t row[LOOK];
+            uint32_t dead[LOOK];
 #pragma unroll
-            for (int i = 0; i < LOOK; ++i) row[i] = nxt[i];
+            for (int i = 0; i < LOOK; ++i) {
+                const bool in = place[i] >= 0, good = in && unsigned(page[i]) < unsigned(a.pool.n_pages);
+                if (in && !good) report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
+                row[i] = good ? int64_t(page[i]) * a.pool.page_stride + int64_t(place[i]) * a.pool.token_stride : 0;
+                dead[i] = __ballot_sync(FULL, !good);  // (NT = 1: lanes 16-31 repeat lanes 0-15)
+            }
             uint4 kf[NT][2][KJ];
             uint32_t vf[NT][4][VI][VW];
-            bool live[NT][2][2];  // tokens 8 n + 2 t, 8 n + 2 t + 1
             auto load_k = [&]() {
 #pragma unroll
                 for (int k = 0; k < NT; ++k)
 #pragma unroll
                     for (int n = 0; n < 2; ++n) {
-                        const int64_t r = __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 8 * n + g);
+                        const uint16_t *r = kb + __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 8 * n + g);
 #pragma unroll
-                        for (int j = 0; j < KJ; ++j) kf[k][n][j] = r >= 0 ? load16(kb + r + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+                        for (int j = 0; j < KJ; ++j) kf[k][n][j] = load16(r + 32 * j);
                     }
             };
             auto load_v = [&]() {
@@ -219,15 +234,14 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
                 for (int k = 0; k < NT; ++k)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int64_t r = __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 2 * t + (e & 1) + 8 * (e >> 1));
-                        live[k][e >> 1][e & 1] = r >= 0;
+                        const uint16_t *r = vb + __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 2 * t + (e & 1) + 8 * (e >> 1));
 #pragma unroll
                         for (int i = 0; i < VI; ++i) {
                             if constexpr (VW == 4) {
-                                const uint4 v = r >= 0 ? load16(vb + r + 64 * i) : make_uint4(0u, 0u, 0u, 0u);
+                                const uint4 v = load16(r + 64 * i);
                                 vf[k][e][i][0] = v.x, vf[k][e][i][1] = v.y, vf[k][e][i][2] = v.z, vf[k][e][i][3] = v.w;
                             } else {
-                                const uint2 v = r >= 0 ? load8(vb + r) : make_uint2(0u, 0u);
+                                const uint2 v = load8(r);
                                 vf[k][e][i][0] = v.x, vf[k][e][i][1] = v.y;
                             }
                         }
@@ -251,16 +265,32 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
                 }
             if constexpr (D > 128) load_v();
             // online softmax of query g: this lane has 4 of each tile's 16 tokens
-            float mx = -INFINITY;
 #pragma unroll
             for (int k = 0; k < NT; ++k)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        s[k][n][e] = live[k][n][e] ? s[k][n][e] * a.scale_log2 : -INFINITY;
-                        mx = fmaxf(mx, s[k][n][e]);
+                    for (int e = 0; e < 2; ++e) s[k][n][e] *= a.scale_log2;
+            if (LOOK == 2 ? (dead[0] | dead[LOOK - 1]) != 0u : dead[0] != 0u) {
+#pragma unroll
+                for (int k = 0; k < NT; ++k)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int at = TT * (k & 1) + 2 * t + (e & 1) + 8 * (e >> 1);
+                        if ((dead[k / 2] >> at) & 1u) {
+                            s[k][e >> 1][e & 1] = -INFINITY;
+#pragma unroll
+                            for (int i = 0; i < VI; ++i)
+#pragma unroll
+                                for (int w = 0; w < VW; ++w) vf[k][e][i][w] = 0u;
+                        }
                     }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < NT; ++k)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) mx = fmaxf(mx, fmaxf(s[k][n][0], s[k][n][1]));
             if (__any_sync(FULL, mx > m)) {
                 mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
