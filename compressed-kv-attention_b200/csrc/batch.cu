@@ -292,7 +292,9 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     const int64_t units = a.stream_prefix + int64_t(x->batch) * h->n_kv_heads * a.tail_groups;
     const int64_t most_tiles = int64_t(a.stream_prefix) * ceil_div(x->prefix_len, kStreamTile) +
                                int64_t(x->batch) * h->n_kv_heads * a.tail_groups * ceil_div(x->max_len, kStreamTile);
-    a.stream_ctas = int(std::min<int64_t>(stream_ctas(h), ceil_div(most_tiles, kStreamLeast * kStreamWarps)));
+    if (most_tiles + units * kUnitTiles > INT32_MAX - (1 << 20))  // (positions are counted in 32 bits)
+        return fail(KVX_ERR_UNSUPPORTED, "kvx_batch_attend: more than 2^31 tiles of 16 tokens in one call");
+    a.stream_ctas = int(std::min<int64_t>(stream_ctas(h), ceil_div(most_tiles, kStreamWarps)));
     const int64_t used = a.stream_base + (a.stream_ctas > 0 ? 8 * (int64_t(a.stream_ctas) * kStreamWarps + units) : 0);
     if (used > h->cap_rows) return fail(KVX_ERR_RUNTIME, "kvx_batch_attend: scratch too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -106,28 +106,24 @@ struct PagedArgs {
     int32_t box_tokens, heads_inside;   // TMA boxes of the pools (see the kernel)
     // Streamed units, laid end to end in 16-token tiles: first (a streamed prefix) KV head by KV
     // head and group of 8 rows, prefix_len tokens each; then sequence by sequence, KV head by KV
-    // head, group of 8 heads by group, the sequence's own tokens.  The tiles are cut into as many
-    // equal runs as there are workers (warps), so worker w has tiles [w T / n, (w + 1) T / n); the
-    // part it leaves of unit u is in rows stream_base + 8 (w + u) .., which no other pair has (w + u
-    // grows along the line).
+    // head, group of 8 heads by group, the sequence's own tokens; each unit's tiles are followed by
+    // kUnitTiles empty positions.  The line is cut into equal runs, one for each worker (warp); the part that worker w leaves of unit u is in rows stream_base + 8
+    // (w + u) .., which no other pair has (w + u grows along the line).
     int64_t stream_base;
     int32_t stream_prefix;  // units of a streamed prefix (0: the prefix is not streamed)
     int32_t pre_groups;     // its groups of 8 rows
     int32_t tail_groups;    // groups of 8 heads of a KV head
     int32_t stream_ctas;    // of kStreamWarps workers
-    int32_t *starts;        // [batch + 1] tiles of the sequences before each, written for the combine
+    int32_t *starts;        // [batch + 1] positions of a unit of each sequence before, for the combine
 };
 
-constexpr int kStreamWarps = 8;   // workers a CTA
+constexpr int kStreamWarps = 4;   // workers a CTA
 constexpr int kStreamTile = 16;   // tokens
-constexpr int kStreamLeast = 1;   // tiles a worker takes at least
-constexpr int kMaxStreamBatch = 4096;
-
-// Workers that share `tiles` tiles out of those launched.
-__device__ __forceinline__ int stream_workers(const PagedArgs &a, int64_t tiles) {
-    const int64_t n = (tiles + kStreamLeast - 1) / kStreamLeast, most = int64_t(a.stream_ctas) * kStreamWarps;
-    return int(n < most ? n : most);
-}
+// Positions a unit takes besides its tiles: its queries' loads, the walk to it and the write of its
+// state take a worker about as long as three tiles.  (Without them a worker whose run met a dozen
+// short sequences ended 40 us after the others.)
+constexpr int kUnitTiles = 3;
+constexpr int kMaxStreamBatch = 2048;
 
 // Query rows of an item and tokens of a tile of the tensor-core prefix kernel.
 constexpr int kPrefixRows = 128, kPrefixTile = 64;

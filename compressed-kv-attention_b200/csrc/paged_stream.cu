@@ -2,21 +2,20 @@
 // time, and the combine pass that folds every row's partial states.
 //
 // A unit is up to 8 query rows and the tokens they share: the own pages of one sequence under one KV
-// head or (batches of few rows) the shared prefix.  All units' 16-token tiles form one line, cut
-// into equal runs, one for each warp of the grid, whatever the lengths are: a warp walks its run
-// with an online softmax of its own and leaves one partial state per row for each unit it met.  No
-// warp waits for another.
+// head or (batches of few rows) the shared prefix.  All units' 16-token tiles form one line, with a
+// margin after each for what a unit costs besides its tiles, cut into equal runs, one for each warp of
+// the grid, whatever the lengths are: a warp walks its run with an online softmax of its own and
+// leaves one partial state per row for each unit it met.  No warp waits for another.
 //
 // The work is 4 bytes and 2 rows FMAs per K and V element, so it is bound by HBM; everything is
-// arranged to keep loads in flight and nothing else in the way.  K and V go from global memory to
-// the tensor cores' fragments without shared memory: the MMAs may take head dims (of QK) and output
-// columns (of PV) in any order as long as both operands agree, so each lane loads 16 contiguous
-// bytes of a token's row and calls them its fragment.
-//   S = Q K^T (m16n8k16, rows 8-15 zero): lane (g, t) loads K token g, dims 32 j + 8 t .. + 7: words
-//   0, 1 are the B fragment of k-step 2 j, words 2, 3 that of 2 j + 1; Q's A fragment is loaded the
-//   same way.  The C fragment (query g, tokens 2 t, 2 t + 1) is already the B fragment of
-//   O^T += V^T P^T, whose A fragment (dims x tokens) pairs two tokens' words by byte permutes:
-//   lane (g, t) loads V tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9 at dims 64 i + 8 g .. + 7.
+// arranged to keep loads in flight.  Each warp has a ring of stages of its own in shared memory (NT
+// tiles of K and V rows, filled row by row with 16-byte asynchronous copies, the pages looked up one
+// stage further ahead), so the copies of the next stages, the next unit's included, are in flight while
+// one is computed.  (With the rows loaded into registers instead, a warp's tile took its load latency
+// and its arithmetic in turn: 2.2 us on an idle device, and 16 warps a SM read 134 MB at 4.3 TB/s.)
+// S^T = K Q^T (m16n8k16, tokens x queries) with K fragments by ldmatrix; its C fragment, packed and
+// transposed by movmatrix, is the B fragment of O^T += V^T P^T, whose V^T fragments come by
+// ldmatrix.trans.  Rows are 2 D + 16 bytes apart, so that eight of them meet no bank twice.
 #include "paged_types.cuh"
 
 namespace kvx {
@@ -41,81 +40,98 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
                      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 (8) bytes that are read once.
-__device__ __forceinline__ uint4 load16(const uint16_t *p) {
-    uint4 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p));
-    return v;
-}
-__device__ __forceinline__ uint2 load8(const uint16_t *p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + TT - 1) / TT; }
 
-// A worker's stretch of one unit.
+// Length of the line (less than 2^31, checked on the host) and of a worker's run.
+__device__ __forceinline__ int stream_line(const PagedArgs &a, int tail_line) {
+    return a.stream_prefix * (tiles_of(a.prefix_len) + kUnitTiles) + tail_line * (a.n_kv_heads * a.tail_groups);
+}
+__device__ __forceinline__ int stream_run(const PagedArgs &a, int line) {
+    const int n = a.stream_ctas * NW;
+    return max(1, (line + n - 1) / n);
+}
+
+// A unit, and where it is on the line.
 struct Unit {
     const int32_t *table;
-    int64_t end;        // tile of the line after the unit's last
-    int tokens;         // of the unit
-    int skip;           // its tiles before the stretch
+    int at;             // position of its first tile
+    int tokens;
     int first, n;       // query rows first .. first + n - 1 of the head's (sequence, g) list
     int head;           // KV head
-    int index;          // in the line
+    int index;          // among the units
+    int b, k;           // sequence (-1: a prefix unit) and (head, group) in it
 };
 
-// The unit that tile f of the line belongs to.  starts[b]: tiles of one (head, group) of the
-// sequences before b.
-__device__ __forceinline__ Unit unit_at(const PagedArgs &a, const int32_t *starts, int64_t f) {
-    Unit u;
-    const int pt = tiles_of(a.prefix_len);
-    const int64_t pre = int64_t(a.stream_prefix) * pt;
-    if (f < pre) {
-        u.index = int(f / pt);
-        u.skip = int(f - int64_t(u.index) * pt);
-        u.end = int64_t(u.index + 1) * pt;
-        u.head = u.index / a.pre_groups;
-        u.first = 8 * (u.index - u.head * a.pre_groups);
+struct Line {
+    const int32_t *starts, *lens;   // of the sequences (see scan_starts)
+    int per, prefix, pre;           // units a sequence; positions of a prefix unit and of all of them
+    __device__ __forceinline__ void of(const PagedArgs &a, const int32_t *starts_, const int32_t *lens_) {
+        starts = starts_, lens = lens_;
+        per = a.n_kv_heads * a.tail_groups;
+        prefix = tiles_of(a.prefix_len) + kUnitTiles;
+        pre = a.stream_prefix * prefix;
+    }
+    __device__ __forceinline__ Unit prefix_unit(const PagedArgs &a, int i) const {
+        Unit u;
+        u.index = i, u.at = i * prefix, u.b = -1, u.k = 0;
+        u.head = i / a.pre_groups;
+        u.first = 8 * (i - u.head * a.pre_groups);
         u.n = min(8, a.batch * a.group - u.first);
         u.tokens = a.prefix_len;
         u.table = a.prefix_table;
         return u;
     }
-    f -= pre;
-    const int per = a.n_kv_heads * a.tail_groups;
-    int lo = 0, hi = a.batch;  // starts[lo] * per <= f < starts[hi] * per
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (int64_t(starts[mid]) * per <= f) lo = mid;
-        else hi = mid;
+    __device__ __forceinline__ Unit tail_unit(const PagedArgs &a, int b, int k) const {
+        Unit u;
+        u.b = b, u.k = k, u.index = a.stream_prefix + b * per + k;
+        u.tokens = lens[b];
+        u.at = pre + starts[b] * per + k * (tiles_of(u.tokens) + kUnitTiles);
+        u.head = a.tail_groups == 1 ? k : k / a.tail_groups;
+        const int qg = k - u.head * a.tail_groups;
+        u.first = b * a.group + 8 * qg;
+        u.n = min(8, a.group - 8 * qg);
+        u.table = a.table + int64_t(b) * a.table_stride;
+        return u;
     }
-    const int n = starts[lo + 1] - starts[lo];  // > 0: starts[lo + 1] * per > f
-    const int64_t at = f - int64_t(starts[lo]) * per;
-    const int k = int(at / n);
-    u.skip = int(at - int64_t(k) * n);
-    u.end = pre + int64_t(starts[lo]) * per + int64_t(k + 1) * n;
-    u.head = k / a.tail_groups;
-    const int qg = k - u.head * a.tail_groups;
-    u.first = lo * a.group + 8 * qg;
-    u.n = min(8, a.group - 8 * qg);
-    u.tokens = tail_len(a, lo);
-    u.table = a.table + int64_t(lo) * a.table_stride;
-    u.index = a.stream_prefix + lo * per + k;
-    return u;
-}
+    // The unit that position f is in.
+    __device__ __forceinline__ Unit find(const PagedArgs &a, int f) const {
+        if (f < pre) return prefix_unit(a, f / prefix);
+        f -= pre;
+        int lo = 0, hi = a.batch;  // starts[lo] * per <= f < starts[hi] * per
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (starts[mid] * per <= f) lo = mid;
+            else hi = mid;
+        }
+        return tail_unit(a, lo, (f - starts[lo] * per) / (starts[lo + 1] - starts[lo]));
+    }
+    // The unit after u; false: there is none.
+    __device__ __forceinline__ bool next(const PagedArgs &a, Unit &u) const {
+        if (u.b < 0 && u.index + 1 < a.stream_prefix) {
+            u = prefix_unit(a, u.index + 1);
+            return true;
+        }
+        int b = u.b, k = u.k + 1;
+        if (b < 0 || k == per) {
+            k = 0;
+            do {
+                if (++b >= a.batch) return false;
+            } while (lens[b] == 0);
+        }
+        u = tail_unit(a, b, k);
+        return true;
+    }
+};
 
-// starts[b], b = 0 .. batch, from the lengths (every thread of the CTA).
-__device__ __forceinline__ void scan_starts(const PagedArgs &a, int32_t *starts) {
+// The lengths, and starts[b], b = 0 .. batch: positions that one unit of every sequence before b takes
+// (every thread of the CTA).
+__device__ __forceinline__ void scan_starts(const PagedArgs &a, int32_t *starts, int32_t *lens) {
     __shared__ int32_t part[NW];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int32_t base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += NW * 32) {
         const int b = b0 + int(threadIdx.x);
-        const int n = b < a.batch && a.max_len > 0 ? tiles_of(tail_len(a, b)) : 0;
+        const int len = b < a.batch && a.max_len > 0 ? tail_len(a, b) : 0, n = len > 0 ? tiles_of(len) + kUnitTiles : 0;
         int s = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -130,7 +146,7 @@ __device__ __forceinline__ void scan_starts(const PagedArgs &a, int32_t *starts)
             if (w < warp) before += part[w];
             all += part[w];
         }
-        if (b < a.batch) starts[b] = before + s - n;
+        if (b < a.batch) starts[b] = before + s - n, lens[b] = len;
         base += all;
         __syncthreads();
     }
@@ -139,11 +155,39 @@ __device__ __forceinline__ void scan_starts(const PagedArgs &a, int32_t *starts)
 }
 
 template <int D> struct Cfg {
-    static constexpr int KJ = D / 32;                 // 32-dim pieces of a K row
-    static constexpr int VI = D >= 64 ? D / 64 : 1;   // pieces of a V row
-    static constexpr int VW = D >= 64 ? 4 : 2;        // words a lane loads of each
-    static constexpr int NT = D <= 64 ? 128 / D : 1;  // tiles taken together: 8 KB in flight a warp
+    static constexpr int KS = D / 16;                 // k-steps of QK, m-tiles of PV
+    static constexpr int NT = D == 32 ? 2 : 1;        // tiles of a stage
+    static constexpr int TOK = NT * TT;
+    static constexpr int NS = D <= 64 ? 5 : 3;        // stages of a warp
+    static constexpr int ROW = 2 * D + 16;            // bytes of a staged row
+    static constexpr int O_V = TOK * ROW, O_DEAD = 2 * O_V;
+    static constexpr int STAGE = O_DEAD + 16;
+    static constexpr int RING = NS * STAGE;           // of a warp
     static constexpr int CTAS = D <= 128 ? 2 : 1;
+    static_assert(TOK <= 32, "a lane for each token of a stage");
+};
+
+// A worker's place on the line: its stages one after another.
+struct Walk {
+    Unit u;
+    int tok, t1;    // the stage's first token, the end of the stretch
+    bool more;
+    // The stretch of u from position f on.
+    __device__ __forceinline__ void stretch(int f, int f_end) {
+        tok = (f - u.at) * TT;
+        t1 = min(u.tokens, (f_end - u.at) * TT);
+    }
+    __device__ __forceinline__ void begin(const PagedArgs &a, const Line &line, int f, int f_end) {
+        more = f < f_end;
+        if (!more) return;
+        u = line.find(a, f);
+        stretch(f, f_end);
+        if (tok >= u.tokens) next(a, line, f_end);  // the run begins in the unit's margin
+    }
+    __device__ __forceinline__ void next(const PagedArgs &a, const Line &line, int f_end) {
+        more = line.next(a, u) && u.at < f_end;
+        if (more) stretch(u.at, f_end);
+    }
 };
 
 // BESIDE: launched behind the same call's prefix kernel, beside which it may run: that kernel's CTAs
@@ -152,194 +196,170 @@ template <int D> struct Cfg {
 template <int D, int DT, bool BESIDE>
 __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const PagedArgs a) {
     using C = Cfg<D>;
-    constexpr int KJ = C::KJ, VI = C::VI, VW = C::VW, NT = C::NT;
-    extern __shared__ int32_t starts[];
+    constexpr int KS = C::KS, NT = C::NT;
+    extern __shared__ __align__(16) uint8_t smem[];
+    int32_t *starts = reinterpret_cast<int32_t *>(smem + NW * C::RING), *lens = starts + a.batch + 1;
     if constexpr (!BESIDE) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    scan_starts(a, starts);
+    scan_starts(a, starts, lens);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= a.batch; b += NW * 32) a.starts[b] = starts[b];
-    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int worker = int(blockIdx.x) * NW + int(threadIdx.x >> 5);
-    const int64_t total = int64_t(a.stream_prefix) * tiles_of(a.prefix_len) +
-                          int64_t(starts[a.batch]) * a.n_kv_heads * a.tail_groups;
-    const int workers = stream_workers(a, total);
-    int64_t f = worker < workers ? worker * total / workers : 0;
-    const int64_t f_end = worker < workers ? (worker + 1) * total / workers : 0;
-    while (f < f_end) {
-        const Unit u = unit_at(a, starts, f);
-        const int t0 = u.skip * TT;
-        const int t1 = min(u.tokens, t0 + int(min(u.end, f_end) - f) * TT);
-        f = u.end;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int worker = int(blockIdx.x) * NW + warp;
+    const int total = stream_line(a, starts[a.batch]), run = stream_run(a, total);
+    const int f0 = int(min(int64_t(total), int64_t(worker) * run)), f_end = min(total, f0 + run);
+    Line line;
+    line.of(a, starts, lens);
+    const uint32_t ring = smem_u32(smem) + uint32_t(warp * C::RING);
 
-        // Q rows as A fragments
-        uint4 qf[KJ];
+    // ---- copies, NS - 1 stages ahead ----
+    Walk ahead;
+    ahead.begin(a, line, f0, f_end);
+    Walk w = ahead;
+    // lane i: the page of token i from `looked` on (nothing looks at the entry before its stage is
+    // issued, so its load is not waited for here) and its place in it (-1: no such token)
+    int32_t page = 0, place = -1;
+    auto look_up = [&]() {
+        page = 0, place = -1;
+        const int tok = ahead.tok + lane;
+        if (ahead.more && tok < ahead.t1) {
+            int64_t at;
+            a.pool.split.at(tok, at, place);
+            page = __ldg(ahead.u.table + at);
+        }
+    };
+    look_up();
+    int half = 0;  // which of the lookup's stages is next
+    auto issue = [&](int stage) {
+        if (ahead.more) {
+            const bool in = place >= 0, good = in && unsigned(page) < unsigned(a.pool.n_pages);
+            if (in && !good) report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
+            const int64_t row = good ? int64_t(page) * a.pool.page_stride + int64_t(place) * a.pool.token_stride +
+                                           int64_t(ahead.u.head) * a.pool.head_stride
+                                     : -1;
+            const uint32_t dead = __ballot_sync(FULL, !good) >> (half * C::TOK);
+            const uint32_t dst = ring + uint32_t(stage % C::NS * C::STAGE);
+            if (lane == 0) sts_u32(dst + C::O_DEAD, dead);
+            constexpr int CH = D / 8, RPI = 32 / CH;  // pieces a row, rows a step
+            const int c = lane % CH;
+#pragma unroll
+            for (int k = 0; k < C::TOK / RPI; ++k) {
+                const int r = k * RPI + lane / CH;
+                const int64_t o = __shfl_sync(FULL, row, half * C::TOK + r);
+                const int64_t at = (o >= 0 ? o : 0) + 8 * c;
+                copy16(dst + uint32_t(r * C::ROW + 16 * c), a.pool.k + at, o >= 0);
+                copy16(dst + uint32_t(C::O_V + r * C::ROW + 16 * c), a.pool.v + at, o >= 0);
+            }
+            ahead.tok += C::TOK;
+            ++half;
+            if (ahead.tok >= ahead.t1) ahead.next(a, line, f_end), half = 32;
+            if (half >= 32 / C::TOK) look_up(), half = 0;
+        }
+        copy_commit();
+    };
+#pragma unroll 1
+    for (int i = 0; i < C::NS - 1; ++i) issue(i);
+
+    // fragment addresses: lanes 8 i .. 8 i + 7 give the rows of matrix i
+    const uint32_t k_at = uint32_t(((lane & 7) + ((lane >> 3) & 1) * 8) * C::ROW + (lane >> 4) * 16);
+    const uint32_t v_at = uint32_t(C::O_V + ((lane & 7) + (lane >> 4) * 8) * C::ROW + ((lane >> 3) & 1) * 16);
+    int stage = 0;
+    while (w.more) {
+        const Unit u = w.u;
+        // Q rows as B fragments (rows past n repeat the first)
+        uint32_t qf[KS][2];
         {
             const int r = u.first + (g < u.n ? g : 0), b = r / a.group;
-            const uint16_t *q = a.q + int64_t(b) * a.q_token + int64_t(u.head * a.group + r - b * a.group) * a.q_head + 8 * t;
+            const uint16_t *q = a.q + int64_t(b) * a.q_token + int64_t(u.head * a.group + r - b * a.group) * a.q_head + 2 * t;
 #pragma unroll
-            for (int j = 0; j < KJ; ++j) qf[j] = load16(q + 32 * j);  // (rows past n repeat the first)
+            for (int k = 0; k < KS; ++k) {
+                qf[k][0] = __ldg(reinterpret_cast<const uint32_t *>(q + 16 * k));
+                qf[k][1] = __ldg(reinterpret_cast<const uint32_t *>(q + 16 * k + 8));
+            }
         }
-        const uint16_t *kb = a.pool.k + int64_t(u.head) * a.pool.head_stride + 8 * t;
-        const uint16_t *vb = a.pool.v + int64_t(u.head) * a.pool.head_stride + 2 * VW * g;
-        float acc[VI * VW][4];
+        // lane (g, t): queries 2 t (m0, l0, acc[.][0, 2]) and 2 t + 1; acc[i]: dims 16 i + g, + 8
+        float acc[KS][4];
 #pragma unroll
-        for (int i = 0; i < VI * VW; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-        float m = -INFINITY, l = 0.f;
-
-        // The lanes look up the pages of the next tiles' tokens ahead of their use; nothing looks at an
-        // entry before then, so its load is not waited for.  place -1: no such token.
-        constexpr int LOOK = NT * TT > 32 ? 2 : 1;
-        int32_t page[LOOK], place[LOOK];
-        auto look_up = [&](int tok0) {
-#pragma unroll
-            for (int i = 0; i < LOOK; ++i) {
-                const int tok = tok0 + 32 * i + (NT * TT >= 32 ? lane : lane & 15);
-                page[i] = 0, place[i] = -1;
-                if (tok < t1) {
-                    int64_t at;
-                    a.pool.split.at(tok, at, place[i]);
-                    page[i] = __ldg(u.table + at);
-                }
-            }
-        };
-        look_up(t0);
-        for (int tok = t0; tok < t1; tok += NT * TT) {
-            // Rows of the tiles' tokens.  Where there is no token (the run's end, a bad entry) the pool's
-            // first row is loaded in its place and then replaced by zeros: loads that depend on a
-            // condition would be waited for one by one (3200 cycles an iteration).
-            int64_t row[LOOK];
-            uint32_t dead[LOOK];
-#pragma unroll
-            for (int i = 0; i < LOOK; ++i) {
-                const bool in = place[i] >= 0, good = in && unsigned(page[i]) < unsigned(a.pool.n_pages);
-                if (in && !good) report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
-                row[i] = good ? int64_t(page[i]) * a.pool.page_stride + int64_t(place[i]) * a.pool.token_stride : 0;
-                dead[i] = __ballot_sync(FULL, !good);  // (NT = 1: lanes 16-31 repeat lanes 0-15)
-            }
-            uint4 kf[NT][2][KJ];
-            uint32_t vf[NT][4][VI][VW];
-            auto load_k = [&]() {
-#pragma unroll
-                for (int k = 0; k < NT; ++k)
-#pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const uint16_t *r = kb + __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 8 * n + g);
-#pragma unroll
-                        for (int j = 0; j < KJ; ++j) kf[k][n][j] = load16(r + 32 * j);
-                    }
-            };
-            auto load_v = [&]() {
-#pragma unroll
-                for (int k = 0; k < NT; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint16_t *r = vb + __shfl_sync(FULL, row[k / 2], TT * (k & 1) + 2 * t + (e & 1) + 8 * (e >> 1));
-#pragma unroll
-                        for (int i = 0; i < VI; ++i) {
-                            if constexpr (VW == 4) {
-                                const uint4 v = load16(r + 64 * i);
-                                vf[k][e][i][0] = v.x, vf[k][e][i][1] = v.y, vf[k][e][i][2] = v.z, vf[k][e][i][3] = v.w;
-                            } else {
-                                const uint2 v = load8(r);
-                                vf[k][e][i][0] = v.x, vf[k][e][i][1] = v.y;
-                            }
-                        }
-                    }
-            };
-            load_k();
-            if constexpr (D <= 128) load_v();  // (at 256 the registers hold one of K and V at a time)
-            look_up(tok + NT * TT);
-
-            float s[NT][2][4];
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    s[k][n][0] = s[k][n][1] = s[k][n][2] = s[k][n][3] = 0.f;
-#pragma unroll
-                    for (int j = 0; j < KJ; ++j) {
-                        mma16<DT>(s[k][n], qf[j].x, 0u, qf[j].y, 0u, kf[k][n][j].x, kf[k][n][j].y);
-                        mma16<DT>(s[k][n], qf[j].z, 0u, qf[j].w, 0u, kf[k][n][j].z, kf[k][n][j].w);
-                    }
-                }
-            if constexpr (D > 128) load_v();
-            // online softmax of query g: this lane has 4 of each tile's 16 tokens
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) s[k][n][e] *= a.scale_log2;
-            if (LOOK == 2 ? (dead[0] | dead[LOOK - 1]) != 0u : dead[0] != 0u) {
-#pragma unroll
-                for (int k = 0; k < NT; ++k)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int at = TT * (k & 1) + 2 * t + (e & 1) + 8 * (e >> 1);
-                        if ((dead[k / 2] >> at) & 1u) {
-                            s[k][e >> 1][e & 1] = -INFINITY;
-#pragma unroll
-                            for (int i = 0; i < VI; ++i)
-#pragma unroll
-                                for (int w = 0; w < VW; ++w) vf[k][e][i][w] = 0u;
-                        }
-                    }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int k = 0; k < NT; ++k)
-#pragma unroll
-                for (int n = 0; n < 2; ++n) mx = fmaxf(mx, fmaxf(s[k][n][0], s[k][n][1]));
-            if (__any_sync(FULL, mx > m)) {
-                mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, 2));
-                const float mn = fmaxf(m, mx);
-                const float al = mn == -INFINITY ? 1.f : exp2_sfu(m - mn);
-                m = mn;
-                l *= al;
-                const float al0 = __shfl_sync(FULL, al, 8 * t), al1 = __shfl_sync(FULL, al, 8 * t + 4);
-#pragma unroll
-                for (int i = 0; i < VI * VW; ++i) acc[i][0] *= al0, acc[i][1] *= al1, acc[i][2] *= al0, acc[i][3] *= al1;
-            }
-            const float mu = m == -INFINITY ? 0.f : m - Elem<DT>::kBias;
+        for (int i = 0; i < KS; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+        float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+        for (; w.tok < w.t1; w.tok += C::TOK, ++stage) {
+            __syncwarp();  // every lane has read the stage that is issued into next
+            issue(stage + C::NS - 1);
+            copy_wait<C::NS - 1>();
+            __syncwarp();
+            const uint32_t at = ring + uint32_t(stage % C::NS * C::STAGE);
+            const uint32_t dead = lds_u32(at + C::O_DEAD);
+            float s[NT][4];
 #pragma unroll
             for (int k = 0; k < NT; ++k) {
-                uint32_t b[2];
+                float s2[2][4] = {};  // two chains
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const float p0 = exp2_sfu(s[k][n][0] - mu), p1 = exp2_sfu(s[k][n][1] - mu);
-                    l += p0 + p1;
-                    b[n] = Elem<DT>::pack(p0, p1);
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t f[4];
+                    ldsm_x4(at + k_at + uint32_t(k * TT * C::ROW + 32 * i), f[0], f[1], f[2], f[3]);
+                    mma16<DT>(s2[i & 1], f[0], f[1], f[2], f[3], qf[i][0], qf[i][1]);
                 }
 #pragma unroll
-                for (int i = 0; i < VI; ++i)
+                for (int e = 0; e < 4; ++e) s[k][e] = (s2[0][e] + s2[1][e]) * a.scale_log2;
+            }
+            if (dead != 0u) {  // (rows of zeros were stored)
 #pragma unroll
-                    for (int w = 0; w < VW; ++w) {
-                        const uint32_t(&v)[4][VI][VW] = vf[k];
-                        mma16<DT>(acc[i * VW + w], prmt(v[0][i][w], v[1][i][w], 0x5410u), prmt(v[0][i][w], v[1][i][w], 0x7632u),
-                                  prmt(v[2][i][w], v[3][i][w], 0x5410u), prmt(v[2][i][w], v[3][i][w], 0x7632u), b[0], b[1]);
-                    }
+                for (int k = 0; k < NT; ++k) {
+                    if ((dead >> (TT * k + g)) & 1u) s[k][0] = s[k][1] = -INFINITY;
+                    if ((dead >> (TT * k + g + 8)) & 1u) s[k][2] = s[k][3] = -INFINITY;
+                }
+            }
+            float x0 = fmaxf(s[0][0], s[0][2]), x1 = fmaxf(s[0][1], s[0][3]);
+#pragma unroll
+            for (int k = 1; k < NT; ++k) x0 = fmaxf(x0, fmaxf(s[k][0], s[k][2])), x1 = fmaxf(x1, fmaxf(s[k][1], s[k][3]));
+            if (__any_sync(FULL, x0 > m0 || x1 > m1)) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) {
+                    x0 = fmaxf(x0, __shfl_xor_sync(FULL, x0, o));
+                    x1 = fmaxf(x1, __shfl_xor_sync(FULL, x1, o));
+                }
+                x0 = fmaxf(x0, m0), x1 = fmaxf(x1, m1);
+                const float e0 = x0 == -INFINITY ? 1.f : exp2_sfu(m0 - x0), e1 = x1 == -INFINITY ? 1.f : exp2_sfu(m1 - x1);
+                m0 = x0, m1 = x1;
+                l0 *= e0, l1 *= e1;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) acc[i][0] *= e0, acc[i][1] *= e1, acc[i][2] *= e0, acc[i][3] *= e1;
+            }
+            const float u0 = m0 == -INFINITY ? 0.f : m0 - Elem<DT>::kBias, u1 = m1 == -INFINITY ? 0.f : m1 - Elem<DT>::kBias;
+#pragma unroll
+            for (int k = 0; k < NT; ++k) {
+                const float p0 = exp2_sfu(s[k][0] - u0), p1 = exp2_sfu(s[k][1] - u1), p2 = exp2_sfu(s[k][2] - u0),
+                            p3 = exp2_sfu(s[k][3] - u1);
+                l0 += p0 + p2, l1 += p1 + p3;
+                const uint32_t b0 = movm_t(Elem<DT>::pack(p0, p1)), b1 = movm_t(Elem<DT>::pack(p2, p3));
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    uint32_t f[4];
+                    ldsm_x4_t(at + v_at + uint32_t(k * TT * C::ROW + 32 * i), f[0], f[1], f[2], f[3]);
+                    mma16<DT>(acc[i], f[0], f[1], f[2], f[3], b0, b1);
+                }
             }
         }
 
         // the part's state
-        l += __shfl_xor_sync(FULL, l, 1);
-        l += __shfl_xor_sync(FULL, l, 2);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            l0 += __shfl_xor_sync(FULL, l0, o);
+            l1 += __shfl_xor_sync(FULL, l1, o);
+        }
         const int64_t out = a.stream_base + 8 * int64_t(worker + u.index);
-        if (t == 0 && g < u.n) a.ml[out + g] = make_float2(m == -INFINITY ? m : m - Elem<DT>::kBias, l);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             if (2 * t + e >= u.n) continue;
-            float *o = a.acc + (out + 2 * t + e) * D + 2 * VW * g;
+            const float m = e ? m1 : m0;
+            if (g == 0) a.ml[out + 2 * t + e] = make_float2(m == -INFINITY ? m : m - Elem<DT>::kBias, e ? l1 : l0);
+            float *o = a.acc + (out + 2 * t + e) * D + g;
 #pragma unroll
-            for (int i = 0; i < VI; ++i)
-#pragma unroll
-                for (int w = 0; w < VW; w += 2)
-                    *reinterpret_cast<float4 *>(o + 64 * i + 2 * w) =
-                        make_float4(acc[i * VW + w][e], acc[i * VW + w][2 + e], acc[i * VW + w + 1][e], acc[i * VW + w + 1][2 + e]);
+            for (int i = 0; i < KS; ++i) o[16 * i] = acc[i][e], o[16 * i + 8] = acc[i][2 + e];
         }
+        w.next(a, line, f_end);
     }
+    copy_wait<0>();
     if constexpr (BESIDE) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
@@ -361,27 +381,24 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Paged
     int np = a.n_split, ns = 0;
     int64_t prow = int64_t(head) * a.n_split * a.row_pad + row, pstep = a.row_pad, srow = 0;
     if (a.stream_ctas > 0) {
-        const int64_t pt = tiles_of(a.prefix_len), pre = a.stream_prefix * pt;
-        const int per = a.n_kv_heads * a.tail_groups;
-        const int64_t total = pre + int64_t(a.starts[a.batch]) * per;
-        const int workers = stream_workers(a, total);
-        // the workers that met tiles [f, f + n) of the line, and the first one's row of unit u;
-        // worker_of(f) = the largest w with floor(w total / workers) <= f
-        auto worker_of = [&](int64_t f) { return int(((f + 1) * workers - 1) / total); };
-        auto parts = [&](int64_t f, int64_t n, int u, int64_t &first) {
-            const int w = worker_of(f);
-            first = a.stream_base + 8 * int64_t(w + u);
-            return worker_of(f + n - 1) - w + 1;
+        const int s0 = a.starts[b], n = a.starts[b + 1] - s0 - kUnitTiles;  // the sequence's tiles (< 0: none)
+        const int run = stream_run(a, stream_line(a, a.starts[a.batch]));
+        const int pt = tiles_of(a.prefix_len), per = a.n_kv_heads * a.tail_groups;
+        // the workers that met tiles [f, f + n) of the line, and the first one's row of unit u
+        auto parts = [&](int f, int n, int u, int64_t &first) {
+            const int w = f / run;
+            first = a.stream_base + 8 * (int64_t(w) + u);
+            return (f + n - 1) / run - w + 1;
         };
         if (a.stream_prefix > 0) {
             const int u = head * a.pre_groups + (row >> 3);
-            np = parts(u * pt, pt, u, prow);
+            np = parts(u * (pt + kUnitTiles), pt, u, prow);
             prow += row & 7;
             pstep = 8;
         }
-        const int n = a.starts[b + 1] - a.starts[b], k = head * a.tail_groups + (gi >> 3);
         if (n > 0) {
-            ns = parts(pre + int64_t(a.starts[b]) * per + int64_t(k) * n, n, a.stream_prefix + b * per + k, srow);
+            const int k = head * a.tail_groups + (gi >> 3);
+            ns = parts(a.stream_prefix * (pt + kUnitTiles) + s0 * per + k * (n + kUnitTiles), n, a.stream_prefix + b * per + k, srow);
             srow += gi & 7;
         }
     }
@@ -441,7 +458,10 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Paged
 }
 
 template <int D, int DT, bool BESIDE> cudaError_t stream_launch(const PagedArgs &a, cudaStream_t s) {
-    return launch_paged(stream_kernel<D, DT, BESIDE>, dim3(unsigned(a.stream_ctas)), NW * 32, 4 * (a.batch + 1), s, a);
+    constexpr int ring = NW * Cfg<D>::RING;
+    static const cudaError_t attr = allow_smem(stream_kernel<D, DT, BESIDE>, ring + 8 * kMaxStreamBatch + 4);
+    if (attr != cudaSuccess) return attr;
+    return launch_paged(stream_kernel<D, DT, BESIDE>, dim3(unsigned(a.stream_ctas)), NW * 32, ring + 8 * a.batch + 4, s, a);
 }
 template <int D, int DT> cudaError_t stream_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, false>(a, s); }
 template <int D, int DT> cudaError_t beside_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, true>(a, s); }

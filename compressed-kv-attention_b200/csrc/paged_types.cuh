@@ -64,6 +64,21 @@ __device__ __forceinline__ int tail_len(const PagedArgs &a, int b) {
     return n < 0 ? 0 : a.max_len;
 }
 
+// 16 bytes global -> shared, zeros when there is no such row.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Lets a kernel take up to `bytes` of dynamic shared memory a CTA and all of the SM's (the default split
+// with L1 may leave room for one CTA where two fit).
+template <class K> cudaError_t allow_smem(K k, int bytes) {
+    cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    return e;
+}
+
 // A launch that may be set up while the grid before it in the stream drains (programmatic dependent
 // launch; every kernel launched so waits for that grid itself).
 template <class K, class... More>

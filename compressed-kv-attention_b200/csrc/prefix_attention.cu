@@ -160,13 +160,6 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 16 bytes global -> shared, zeros when there is no such row.
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 // One TMA box global -> shared, completing its bytes on `bar`.
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
     asm volatile(
@@ -669,8 +662,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
 template <int D, int DT, int LOAD>
 cudaError_t prefix_launch(const PagedArgs &a, const PrefixMaps &maps, cudaStream_t s) {
     using C = Cfg<D, LOAD>;
-    static const cudaError_t attr =
-        cudaFuncSetAttribute(prefix_kernel<D, DT, LOAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static const cudaError_t attr = allow_smem(prefix_kernel<D, DT, LOAD>, C::SMEM);
     if (attr != cudaSuccess) return attr;
     return launch_paged(prefix_kernel<D, DT, LOAD>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), C::THREADS, C::SMEM, s, a, maps);
 }
