@@ -35,6 +35,18 @@ int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 // the tensor-core kernel.
 constexpr int kStreamRows = 8;
 
+// The streaming kernel's share of the device beside the prefix kernel.  A prefix item's tile (64 tokens,
+// 128 rows) takes a CTA's room about as long as four streamed tiles of 16 tokens at head dims from 128
+// on and eight below (the softmax of 128 rows does not shrink with the head), and tails are taken to be
+// half of max_len on average.  Shares below kLeastShare or above kMostShare are not worth the cut (the
+// streaming kernel then simply follows): 64 sequences of up to 1024 tokens behind 32K took 82 us one
+// after the other and 70 us sharing, the ones whose tails weigh 2 % or 80 % 3 % and 25 % longer.
+constexpr double kLeastShare = 0.15, kMostShare = 0.6;
+double stream_share(int dim, int64_t prefix_tiles, int64_t tail_tiles) {
+    const double share = double(tail_tiles) / double(tail_tiles + (dim >= 128 ? 4 : 8) * prefix_tiles);
+    return share >= kLeastShare && share <= kMostShare ? share : 0.0;
+}
+
 // The cut of a prefix for the tensor-core kernel: tiles a split, the splits that end soonest when
 // `slots` CTAs run at a time and an item costs its tiles and about kItemTiles more (its queries,
 // the pipeline's fill and the write of its state).
@@ -166,7 +178,8 @@ int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int 
     h->cap_rows = scratch_rows(h, max_batch);
     cudaError_t e = cudaMalloc(&h->status, 2 * sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(h->status, 0, 2 * sizeof(int));
-    if (e == cudaSuccess) e = cudaMalloc(&h->starts, (size_t(max_batch) + 1) * sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMalloc(&h->starts, (size_t(max_batch) + 2) * sizeof(int32_t));
+    if (e == cudaSuccess) e = cudaMemset(h->starts, 0, (size_t(max_batch) + 2) * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMalloc(&h->acc, size_t(h->cap_rows) * dim * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&h->ml, size_t(h->cap_rows) * sizeof(float2));
     if (e != cudaSuccess) {
@@ -276,13 +289,18 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     a.ml = h->ml;
     a.status = h->status;
     a.starts = h->starts;
+    a.next_run = h->starts + h->max_batch + 1;
     const int rows = x->batch * h->group;
     const bool tensor = coded || (paged && rows > kStreamRows);
     if (tensor) {
         a.row_groups = ceil_div(rows, kPrefixRows);
         a.row_pad = kPrefixRows * a.row_groups;
         a.prefix_tiles = coded ? a.xkv.tiles : ceil_div(x->prefix_len, kPrefixTile);
-        a.split_tiles = prefix_split_tiles(a.prefix_tiles, h->n_kv_heads * a.row_groups, prefix_ctas_per_sm(h->dim) * h->sms);
+        const double share = stream_share(h->dim, int64_t(a.prefix_tiles) * h->n_kv_heads * a.row_groups,
+                                          int64_t(x->batch) * h->n_kv_heads * ceil_div(h->group, 8) * ceil_div(x->max_len, 2 * kStreamTile));
+        const int slots = prefix_ctas_per_sm(h->dim) * h->sms;
+        a.split_tiles = prefix_split_tiles(a.prefix_tiles, h->n_kv_heads * a.row_groups, std::max(1, int(slots * (1.0 - share))));
+        a.shared_runs = share > 0.0;
         a.n_split = ceil_div(a.prefix_tiles, a.split_tiles);
         a.stream_base = int64_t(h->n_kv_heads) * a.n_split * a.row_pad;
     }
@@ -295,7 +313,8 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     if (most_tiles + units * kUnitTiles > INT32_MAX - (1 << 20))  // (positions are counted in 32 bits)
         return fail(KVX_ERR_UNSUPPORTED, "kvx_batch_attend: more than 2^31 tiles of 16 tokens in one call");
     a.stream_ctas = int(std::min<int64_t>(stream_ctas(h), ceil_div(most_tiles, kStreamWarps)));
-    const int64_t used = a.stream_base + (a.stream_ctas > 0 ? 8 * (int64_t(a.stream_ctas) * kStreamWarps + units) : 0);
+    a.stream_runs = a.stream_ctas * kStreamWarps;
+    const int64_t used = a.stream_base + (a.stream_ctas > 0 ? 8 * (int64_t(a.stream_runs) + units) : 0);
     if (used > h->cap_rows) return fail(KVX_ERR_RUNTIME, "kvx_batch_attend: scratch too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (tensor) KVX_CUDA(launch_paged_prefix(h->dim, h->dtype, a, s));

@@ -113,15 +113,18 @@ struct PagedArgs {
     int32_t stream_prefix;  // units of a streamed prefix (0: the prefix is not streamed)
     int32_t pre_groups;     // its groups of 8 rows
     int32_t tail_groups;    // groups of 8 heads of a KV head
-    int32_t stream_ctas;    // of kStreamWarps workers
+    int32_t stream_ctas;    // of kStreamWarps warps
+    int32_t stream_runs;
+    int32_t shared_runs;    // 0: warp i of the grid takes run i; 1: the warps take runs from next_run
+    int32_t *next_run;      // 0 before the call, and again after it
     int32_t *starts;        // [batch + 1] positions of a unit of each sequence before, for the combine
 };
 
-constexpr int kStreamWarps = 4;   // workers a CTA
+constexpr int kStreamWarps = 4;   // a CTA
 constexpr int kStreamTile = 16;   // tokens
 // Positions a unit takes besides its tiles: its queries' loads, the walk to it and the write of its
-// state take a worker about as long as three tiles.  (Without them a worker whose run met a dozen
-// short sequences ended 40 us after the others.)
+// state take a warp about as long as three tiles.  (Without them a warp whose run met a dozen short
+// sequences ended 40 us after the others.)
 constexpr int kUnitTiles = 3;
 constexpr int kMaxStreamBatch = 2048;
 

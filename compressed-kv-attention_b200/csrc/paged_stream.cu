@@ -3,9 +3,12 @@
 //
 // A unit is up to 8 query rows and the tokens they share: the own pages of one sequence under one KV
 // head or (batches of few rows) the shared prefix.  All units' 16-token tiles form one line, with a
-// margin after each for what a unit costs besides its tiles, cut into equal runs, one for each warp of
-// the grid, whatever the lengths are: a warp walks its run with an online softmax of its own and
-// leaves one partial state per row for each unit it met.  No warp waits for another.
+// margin after each for what a unit costs besides its tiles, cut into equal runs whatever the lengths
+// are, one for each warp of the grid: a warp walks its run with an online softmax of its own and leaves
+// one partial state per row for each unit it met.  No warp waits for another.  Where the kernel shares
+// the device with the prefix kernel, the warps take runs from a counter instead, so that those that
+// find room at once take more of them and the others what is left; which warp takes a run changes no
+// result.
 //
 // The work is 4 bytes and 2 rows FMAs per K and V element, so it is bound by HBM; everything is
 // arranged to keep loads in flight.  Each warp has a ring of stages of its own in shared memory (NT
@@ -42,13 +45,12 @@ __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, u
 
 __device__ __forceinline__ int tiles_of(int tokens) { return (tokens + TT - 1) / TT; }
 
-// Length of the line (less than 2^31, checked on the host) and of a worker's run.
+// Length of the line (less than 2^31, checked on the host) and of a run.
 __device__ __forceinline__ int stream_line(const PagedArgs &a, int tail_line) {
     return a.stream_prefix * (tiles_of(a.prefix_len) + kUnitTiles) + tail_line * (a.n_kv_heads * a.tail_groups);
 }
 __device__ __forceinline__ int stream_run(const PagedArgs &a, int line) {
-    const int n = a.stream_ctas * NW;
-    return max(1, (line + n - 1) / n);
+    return max(1, (line + a.stream_runs - 1) / a.stream_runs);
 }
 
 // A unit, and where it is on the line.
@@ -167,26 +169,27 @@ template <int D> struct Cfg {
     static_assert(TOK <= 32, "a lane for each token of a stage");
 };
 
-// A worker's place on the line: its stages one after another.
+// A place in a run: its stages one after another.
 struct Walk {
     Unit u;
     int tok, t1;    // the stage's first token, the end of the stretch
+    int end;        // of the run
     bool more;
     // The stretch of u from position f on.
-    __device__ __forceinline__ void stretch(int f, int f_end) {
+    __device__ __forceinline__ void stretch(int f) {
         tok = (f - u.at) * TT;
-        t1 = min(u.tokens, (f_end - u.at) * TT);
+        t1 = min(u.tokens, (end - u.at) * TT);
     }
     __device__ __forceinline__ void begin(const PagedArgs &a, const Line &line, int f, int f_end) {
-        more = f < f_end;
-        if (!more) return;
+        end = f_end;
         u = line.find(a, f);
-        stretch(f, f_end);
-        if (tok >= u.tokens) next(a, line, f_end);  // the run begins in the unit's margin
+        more = true;
+        stretch(f);
+        if (tok >= u.tokens) next(a, line);  // the run begins in the unit's margin
     }
-    __device__ __forceinline__ void next(const PagedArgs &a, const Line &line, int f_end) {
-        more = line.next(a, u) && u.at < f_end;
-        if (more) stretch(u.at, f_end);
+    __device__ __forceinline__ void next(const PagedArgs &a, const Line &line) {
+        more = line.next(a, u) && u.at < end;
+        if (more) stretch(u.at);
     }
 };
 
@@ -201,22 +204,47 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
     int32_t *starts = reinterpret_cast<int32_t *>(smem + NW * C::RING), *lens = starts + a.batch + 1;
     if constexpr (!BESIDE) asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // the warp's next run (in lane 0): fetched ahead, and not looked at before it is needed
+    auto fetch = [&]() -> int { return !a.shared_runs ? INT_MAX : lane == 0 ? atomicAdd(a.next_run, 1) : 0; };
+    int fetched = a.shared_runs ? fetch() : int(blockIdx.x) * NW + warp;
     scan_starts(a, starts, lens);
     if (blockIdx.x == 0)
         for (int b = threadIdx.x; b <= a.batch; b += NW * 32) a.starts[b] = starts[b];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int worker = int(blockIdx.x) * NW + warp;
-    const int total = stream_line(a, starts[a.batch]), run = stream_run(a, total);
-    const int f0 = int(min(int64_t(total), int64_t(worker) * run)), f_end = min(total, f0 + run);
+    // (the last unit's margin is no part of the line)
+    const int total = max(0, stream_line(a, starts[a.batch]) - kUnitTiles), run = stream_run(a, total), runs = (total + run - 1) / run;
     Line line;
     line.of(a, starts, lens);
     const uint32_t ring = smem_u32(smem) + uint32_t(warp * C::RING);
+    // the warp's next run that is not all margin, with a walk at its beginning; false: there is none
+    auto take = [&](Walk &x, int &r) -> bool {
+        for (;;) {
+            r = __shfl_sync(FULL, fetched, 0);
+            if (r >= runs) return false;
+            fetched = fetch();
+            x.begin(a, line, r * run, min(total, (r + 1) * run));
+            if (x.more) return true;
+        }
+    };
 
     // ---- copies, NS - 1 stages ahead ----
-    Walk ahead;
-    ahead.begin(a, line, f0, f_end);
-    Walk w = ahead;
-    // lane i: the page of token i from `looked` on (nothing looks at the entry before its stage is
+    int r;
+    Walk w, ahead;
+    w.more = take(w, r);
+    ahead = w;
+    // runs that the copies have entered and the computation has not (a run has a stage at least; the
+    // copies enter the next one as soon as they have issued a run's last)
+    int queue[C::NS], queued = 0;
+    auto cross = [&]() {
+        int next;
+        ahead.more = take(ahead, next);
+        if (!ahead.more) return;
+#pragma unroll
+        for (int i = 0; i < C::NS; ++i)
+            if (i == queued) queue[i] = next;
+        ++queued;
+    };
+    // lane i: the page of token i from the lookup's first on (nothing looks at the entry before its stage is
     // issued, so its load is not waited for here) and its place in it (-1: no such token)
     int32_t page = 0, place = -1;
     auto look_up = [&]() {
@@ -252,7 +280,11 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
             }
             ahead.tok += C::TOK;
             ++half;
-            if (ahead.tok >= ahead.t1) ahead.next(a, line, f_end), half = 32;
+            if (ahead.tok >= ahead.t1) {
+                ahead.next(a, line);
+                if (!ahead.more) cross();
+                half = 32;
+            }
             if (half >= 32 / C::TOK) look_up(), half = 0;
         }
         copy_commit();
@@ -347,7 +379,7 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
             l0 += __shfl_xor_sync(FULL, l0, o);
             l1 += __shfl_xor_sync(FULL, l1, o);
         }
-        const int64_t out = a.stream_base + 8 * int64_t(worker + u.index);
+        const int64_t out = a.stream_base + 8 * int64_t(r + u.index);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             if (2 * t + e >= u.n) continue;
@@ -357,7 +389,14 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
 #pragma unroll
             for (int i = 0; i < KS; ++i) o[16 * i] = acc[i][e], o[16 * i + 8] = acc[i][2 + e];
         }
-        w.next(a, line, f_end);
+        w.next(a, line);
+        if (!w.more && queued > 0) {
+            r = queue[0];
+#pragma unroll
+            for (int i = 0; i + 1 < C::NS; ++i) queue[i] = queue[i + 1];
+            --queued;
+            w.begin(a, line, r * run, min(total, (r + 1) * run));
+        }
     }
     copy_wait<0>();
     if constexpr (BESIDE) asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -374,6 +413,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Paged
     __shared__ float2 sml[kCombineWarps];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (a.shared_runs && blockIdx.x + blockIdx.y + threadIdx.x == 0) *a.next_run = 0;  // for the next call
     const int b = blockIdx.y, h = blockIdx.x, head = h / a.group, gi = h - head * a.group;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
     // the row's parts: of the prefix (np, from row prow, pstep apart), then of its own tokens (ns)
@@ -382,9 +422,9 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Paged
     int64_t prow = int64_t(head) * a.n_split * a.row_pad + row, pstep = a.row_pad, srow = 0;
     if (a.stream_ctas > 0) {
         const int s0 = a.starts[b], n = a.starts[b + 1] - s0 - kUnitTiles;  // the sequence's tiles (< 0: none)
-        const int run = stream_run(a, stream_line(a, a.starts[a.batch]));
+        const int run = stream_run(a, max(0, stream_line(a, a.starts[a.batch]) - kUnitTiles));
         const int pt = tiles_of(a.prefix_len), per = a.n_kv_heads * a.tail_groups;
-        // the workers that met tiles [f, f + n) of the line, and the first one's row of unit u
+        // the runs that met tiles [f, f + n) of the line, and the first one's row of unit u
         auto parts = [&](int f, int n, int u, int64_t &first) {
             const int w = f / run;
             first = a.stream_base + 8 * (int64_t(w) + u);
@@ -469,7 +509,7 @@ template <int D, int DT> cudaError_t beside_d(const PagedArgs &a, cudaStream_t s
 template <int D, int DT> cudaError_t combine_d(const PagedArgs &a, cudaStream_t s) {
     // about this many parts a row: more warps where each would take several in turn
     const int units = a.stream_prefix + a.batch * a.n_kv_heads * a.tail_groups;
-    const int parts = a.n_split + a.stream_ctas * NW / units;
+    const int parts = a.n_split + a.stream_runs / units;
     return launch_paged(combine_kernel<D, DT>, dim3(unsigned(a.n_q_heads), unsigned(a.batch)),
                         32 * (parts > 16 ? kCombineWarps : 4), 0, s, a);
 }
