@@ -661,8 +661,7 @@ static int prefix_create_impl(const kvx_unit *heads, int n_kv_heads, int dim, kv
     p->dev.tile_tokens = tokens;
     p->dev.esc = plan->esc;
     p->dev.b7 = plan->b7;
-    p->dev.blocks = heads[0].n_blocks;
-    p->dev.tiles_per_block = tpb;
+    p->dev.head_tiles = int32_t(per_head);
     *out = p.release();
     g_err.clear();
     return KVX_OK;

@@ -72,13 +72,13 @@ struct XkvGroup {
 };
 static_assert(sizeof(XkvGroup) == 32, "XkvGroup is 32 bytes");
 
-// An XKV prefix: every block takes tiles_per_block tiles of kPrefixTile tokens (fewer or none in
-// the last ones), every tile four groups a tensor.
+// An XKV prefix: every block takes the same number of tiles of kPrefixTile tokens (fewer tokens or none
+// in the last ones), every tile four groups a tensor.
 struct XkvDev {
-    const XkvGroup *groups;      // [kv head][block][K, V][tiles_per_block][4]
-    const uint8_t *tile_tokens;  // [kv head][block][tiles_per_block]
+    const XkvGroup *groups;      // [kv head][tile][K, V][4]
+    const uint8_t *tile_tokens;  // [kv head][tile]
     const uint32_t *esc, *b7;
-    int32_t blocks, tiles_per_block;
+    int32_t head_tiles;          // of a head (0: no XKV prefix)
     int32_t tiles;               // up to the last with tokens
 };
 
@@ -92,7 +92,7 @@ struct PagedArgs {
     const int32_t *prefix_table, *table, *lens;
     int64_t table_stride;
     int32_t prefix_len, max_len;
-    XkvDev xkv;             // the prefix when xkv.blocks > 0
+    XkvDev xkv;             // the prefix when xkv.tiles > 0
     int32_t batch, n_q_heads, n_kv_heads, group;
     float scale_log2;       // scale * log2(e)
     int *status;

@@ -284,35 +284,31 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             const int w = warp - SW, c8 = lane % C8, r0 = lane / C8;
             const int total = 2 * it.tiles * (TT / 16), mine = (total - w + LW - 1) / LW;
             const uint32_t stages = sb + uint32_t(C::O_STAGE + w * NS * C::STAGE);
+            const XkvGroup *groups = a.xkv.groups + int64_t(it.head) * a.xkv.head_tiles * (2 * (TT / 16));
             auto entry = [&](int k) -> const uint4 * {
                 const int id = w + LW * k, q = id >> 2;
                 const bool v = is_v_item(q);
                 const int tile = it.tile0 + (q == 0 ? 0 : (q == 2 * it.tiles - 1 ? it.tiles - 1 : (v ? q / 2 - 1 : (q + 1) / 2)));
-                const int block = tile / a.xkv.tiles_per_block, sub = tile - block * a.xkv.tiles_per_block;
-                const int64_t i = ((int64_t(it.head) * a.xkv.blocks + block) * 2 + (v ? 1 : 0)) * a.xkv.tiles_per_block + sub;
-                return reinterpret_cast<const uint4 *>(a.xkv.groups + i * 4 + (id & 3));
+                return reinterpret_cast<const uint4 *>(groups + (2 * tile + (v ? 1 : 0)) * (TT / 16) + (id & 3));
             };
             auto staged = [&](int k) { return bar(B_COUNT + w * NS + k % NS); };
             // group k into its staging slot: the table entry, and the copies of a coded group
             auto issue = [&](int k, const uint4 &e0, const uint4 &e1) {
                 const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
+                const uint64_t rows = (uint64_t(e0.y) << 32) | e0.x, codes = rows + e0.z;
+                const uint32_t mode = (e1.y >> 16) & 0xFFu, n = e1.y >> 24;
+                // lane 0: the rows, lane 1: the codes (each the 16-byte aligned superset)
+                const uint64_t at = lane == 0 ? rows : codes;
+                const uint32_t len = (uint32_t(at & 15u) + (lane == 0 ? n * D : n * D * mode / 8) + 15u) & ~15u;
+                const bool copied = mode != 0 && n > 0;
+                const uint32_t both = len + __shfl_sync(FULL, len, 1);
                 if (lane == 0) {
                     sts_v4(slot, e0.x, e0.y, e0.z, e0.w);
                     sts_v4(slot + 16, e1.x, e1.y, e1.z, e1.w);
-                    const uint64_t rows = (uint64_t(e0.y) << 32) | e0.x;
-                    const uint32_t mode = (e1.y >> 16) & 0xFFu, n = e1.y >> 24;
-                    uint32_t len0 = 0, len1 = 0;
-                    const uint64_t codes = rows + e0.z;
-                    if (mode != 0 && n > 0) {
-                        len0 = (uint32_t(rows & 15u) + n * D + 15u) & ~15u;
-                        len1 = (uint32_t(codes & 15u) + n * D * mode / 8 + 15u) & ~15u;
-                    }
-                    mbar_arrive_expect_tx(staged(k), len0 + len1);
-                    if (len0 != 0) {
-                        bulk_g2s(slot + C::S_ROWS, reinterpret_cast<const void *>(rows & ~uint64_t(15)), len0, staged(k));
-                        bulk_g2s(slot + C::S_CODES, reinterpret_cast<const void *>(codes & ~uint64_t(15)), len1, staged(k));
-                    }
+                    mbar_arrive_expect_tx(staged(k), copied ? both : 0u);
                 }
+                if (lane < 2 && copied)
+                    bulk_g2s(slot + (lane == 0 ? C::S_ROWS : C::S_CODES), reinterpret_cast<const void *>(at & ~uint64_t(15)), len, staged(k));
             };
             uint4 e0 = make_uint4(0u, 0u, 0u, 0u), e1 = e0;
             int issued = 0;
@@ -561,7 +557,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
         for (int i = 0; i < it.tiles && ok; ++i) {
             int valid = a.prefix_len - (it.tile0 + i) * TT;  // tokens of the tile
             if constexpr (XKV)
-                valid = __ldg(a.xkv.tile_tokens + int64_t(it.head) * a.xkv.blocks * a.xkv.tiles_per_block + it.tile0 + i);
+                valid = __ldg(a.xkv.tile_tokens + int64_t(it.head) * a.xkv.head_tiles + it.tile0 + i);
             ok = __all_sync(FULL, wait(bar(B_S0 + (i & 1)), i >> 1));
             if (!ok) break;
             fence_after();
@@ -718,7 +714,7 @@ template <int D, int DT> cudaError_t prefix_d(const PagedArgs &args, cudaStream_
     PagedArgs a = args;
     PrefixMaps maps{};
     if constexpr (DT == KVX_DTYPE_BF16)
-        if (a.xkv.blocks > 0) return prefix_launch<D, DT, LOAD_XKV>(a, maps, s);
+        if (a.xkv.tiles > 0) return prefix_launch<D, DT, LOAD_XKV>(a, maps, s);
     // boxes of fewer than 8 tokens would not fill a swizzle pattern
     for (a.box_tokens = TT; a.pool.split.tokens % a.box_tokens != 0;) a.box_tokens >>= 1;
     if (a.box_tokens >= 8 && encode_maps(D, DT, a, maps)) return prefix_launch<D, DT, LOAD_TMA>(a, maps, s);
@@ -754,7 +750,7 @@ __global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int
                     g.n_esc = uint16_t(e1 - e0);
                 }
             }
-            groups[((b * 2 + T) * tpb + sub) * (TT / 16) + j] = g;
+            groups[(i * 2 + T) * (TT / 16) + j] = g;
         }
     }
 }
