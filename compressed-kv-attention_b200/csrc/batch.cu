@@ -70,7 +70,7 @@ int stream_ctas(const kvx_batch_s *h) { return (h->dim <= 128 ? 2 : 1) * h->sms;
 // Rows of an upper bound of the scratch an attention call of `batch` sequences takes.
 int64_t scratch_rows(const kvx_batch_s *h, int batch) {
     const int64_t rows = int64_t(batch) * h->group;
-    const int64_t tensor = (4 * int64_t(prefix_ctas_per_sm(h->dim)) * h->sms + h->n_kv_heads * int64_t(ceil_div(rows, kPrefixRows))) *
+    const int64_t tensor = (4 * int64_t(prefix_ctas_per_sm(h->dim, false)) * h->sms + h->n_kv_heads * int64_t(ceil_div(rows, kPrefixRows))) *
                            kPrefixRows;
     const int64_t units = h->n_kv_heads * (int64_t(batch) * ceil_div(h->group, 8) + ceil_div(kStreamRows, 8));
     return tensor + 8 * (int64_t(stream_ctas(h)) * kStreamWarps + units);
@@ -298,7 +298,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
         a.prefix_tiles = coded ? a.xkv.tiles : ceil_div(x->prefix_len, kPrefixTile);
         const double share = stream_share(h->dim, int64_t(a.prefix_tiles) * h->n_kv_heads * a.row_groups,
                                           int64_t(x->batch) * h->n_kv_heads * ceil_div(h->group, 8) * ceil_div(x->max_len, 2 * kStreamTile));
-        const int slots = prefix_ctas_per_sm(h->dim) * h->sms;
+        const int slots = prefix_ctas_per_sm(h->dim, coded) * h->sms;
         a.split_tiles = prefix_split_tiles(a.prefix_tiles, h->n_kv_heads * a.row_groups, std::max(1, int(slots * (1.0 - share))));
         a.shared_runs = share > 0.0;
         a.n_split = ceil_div(a.prefix_tiles, a.split_tiles);

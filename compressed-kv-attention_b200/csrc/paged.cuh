@@ -130,7 +130,7 @@ constexpr int kMaxStreamBatch = 2048;
 
 // Query rows of an item and tokens of a tile of the tensor-core prefix kernel.
 constexpr int kPrefixRows = 128, kPrefixTile = 64;
-int prefix_ctas_per_sm(int dim);
+int prefix_ctas_per_sm(int dim, bool coded);
 
 // The tensor-core kernel over the prefix items of `a`.
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s);

@@ -56,19 +56,21 @@ enum { LOAD_TMA, LOAD_ROWS, LOAD_XKV };
 
 template <int D, int LOAD> struct Cfg {
     static constexpr bool XKV = LOAD == LOAD_XKV;
-    static constexpr int LW = LOAD == LOAD_TMA ? 1 : 3;     // loader warps
+    // loader warps; an XKV group takes one about 2700 cycles at D = 128, hence as many as fit a SM's
+    // registers and staging memory, with one CTA a SM (two CTAs of three: 75 us where this takes XKV_US)
+    static constexpr int LW = LOAD == LOAD_TMA ? 1 : (LOAD == LOAD_ROWS ? 3 : (D == 256 ? 8 : 11));
     static constexpr int THREADS = 32 * (SW + LW + 1);
     static constexpr int ROWB = D >= 64 ? 128 : 64;         // bytes of a row of one panel of head dims
     static constexpr int SLOT = TT * D * 2;
-    static constexpr int NSLOT = XKV ? (D == 32 ? 8 : (D == 64 ? 6 : 3)) : (D == 32 ? 12 : (D == 64 ? 10 : 5));
+    static constexpr int NSLOT = XKV ? (D == 32 ? 16 : (D == 64 ? 10 : (D == 128 ? 5 : 2))) : (D == 32 ? 12 : (D == 64 ? 10 : 5));
     static constexpr int LAG = NSLOT / 2;                   // row copies: tiles in flight before one is announced
     static constexpr int PANELS = D >= 64 ? D / 64 : 1;
-    static constexpr int CTAS = D == 256 ? 1 : 2;           // per SM
+    static constexpr int CTAS = XKV || D == 256 ? 1 : 2;    // per SM
     static constexpr int O_Q = 0;
     static constexpr int O_RING = ROWS * D * 2;
     // staging slots of a loader warp (XKV): the group's table entry, 16 rows, their codes, each piece
     // landing 0-15 bytes past its 16-byte aligned start
-    static constexpr int NSTAGE = XKV ? (D <= 64 ? 8 : 3) : 0;
+    static constexpr int NSTAGE = XKV ? (D <= 64 ? 6 : (D == 128 ? 3 : 2)) : 0;
     static constexpr int S_ROWS = 32, S_CODES = S_ROWS + 16 * D + 32;
     static constexpr int STAGE = S_CODES + 8 * D + 32;
     static constexpr int O_STAGE = O_RING + NSLOT * SLOT;
@@ -81,7 +83,7 @@ template <int D, int LOAD> struct Cfg {
     static constexpr int TMEM = D == 256 ? 512 : 256;       // columns: O at 0, S / P buffers at D, D + 64
     static constexpr uint64_t LAYOUT = D >= 64 ? 2 : 4;     // 128- / 64-byte swizzle
     static_assert(PANELS * (TT / 8) <= 32, "a lane for each TMA box");
-    static_assert(LAG < NSLOT - 1, "the tile that frees the ring's next slot has been announced");
+    static_assert(XKV || LAG < NSLOT - 1, "the tile that frees the ring's next slot has been announced");
     static_assert(ROWS * LDO * 4 <= O_BAR, "the staged outputs fit where Q and the ring were");
     static_assert(D + 2 * TT <= TMEM && CTAS * TMEM <= 512, "TMEM columns");
     static_assert(CTAS * (SMEM + 1024) <= 233472, "shared memory");
@@ -757,7 +759,7 @@ __global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int
 
 }  // namespace
 
-int prefix_ctas_per_sm(int dim) { return dim == 256 ? Cfg<256, LOAD_TMA>::CTAS : Cfg<128, LOAD_TMA>::CTAS; }
+int prefix_ctas_per_sm(int dim, bool coded) { return coded || dim == 256 ? Cfg<256, LOAD_TMA>::CTAS : Cfg<128, LOAD_TMA>::CTAS; }
 
 cudaError_t launch_xkv_groups(const BlockDesc *desc, int64_t n_blocks, int tiles_per_block, int dim, XkvGroup *groups,
                               uint8_t *tile_tokens, cudaStream_t s) {

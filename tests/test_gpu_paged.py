@@ -377,20 +377,25 @@ def test_attend_xkv(kvx, cuda, H, hq, hkv, dim, seq, lens, block, bits):
         b.attend(c.q, out, pages, c.table, c.lens, c.max_len, prefix=prefix, lse=lse)
     b.check()
     H.assert_attends(out, lse, c.truth())
-    if block == 128 and len(lens) * (hq // hkv) > 8:
-        # the same tiles reach the tensor cores as from pages: the same bits
-        page = 16
-        n = -(-seq // page)
-        kp = torch.full((n + c.k_pool.shape[0], page, hkv, dim), math.nan, device="cuda", dtype=torch.bfloat16)
-        vp = kp.clone()
-        table = torch.arange(n, device="cuda", dtype=torch.int32)
-        t = torch.arange(seq, device="cuda")
-        kp[t // page, t % page], vp[t // page, t % page] = c.prefix
-        kp[n:], vp[n:] = c.k_pool, c.v_pool
-        same = torch.empty_like(out)
-        b.attend(c.q, same, kvx.Pages(kp, vp), c.table + n, c.lens, c.max_len, prefix_table=table, prefix_len=seq)
-        b.check()
-        assert torch.equal(same, out)
+
+
+@pytest.mark.parametrize("hq,hkv,dim,seq,batch,bits", [(14, 2, 64, 1000, 3, 0x1C), (8, 2, 128, 700, 40, 0x14),
+                                                       (6, 3, 32, 999, 70, 0x1C), (4, 2, 256, 515, 5, 0x1C)])
+def test_xkv_prefix_is_the_paged_prefix(kvx, cuda, H, hq, hkv, dim, seq, batch, bits):
+    """The same tiles reach the tensor cores as from pages: the same bits where both are cut alike (a tile an item,
+    as long as the items are no more than the SMs)."""
+    torch = cuda
+    k, v = _modes(torch, seq, hkv, dim, 128, 0), _modes(torch, seq, hkv, dim, 128, 1, special=0.1)
+    assert -(-seq // 64) * hkv * -(-batch * (hq // hkv) // 128) <= 148
+    c = H.Paged(batch, hq, hkv, dim, seq, [0] * batch, 16, q_scale=0.7)
+    c.prefix = (k.transpose(0, 1), v.transpose(0, 1))
+    c._store(c.prefix_table, *c.prefix)
+    b, pages = kvx.Batch(batch, hq, hkv, dim), kvx.Pages(c.k_pool, c.v_pool)
+    out, same = (torch.empty((batch, hq, dim), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    b.attend(c.q, out, pages, None, None, 0, prefix=kvx.Prefix.encode(k, v, code_bits=bits))
+    b.attend(c.q, same, pages, None, None, 0, prefix_table=c.prefix_table, prefix_len=seq)
+    b.check()
+    assert torch.equal(out, same)
 
 
 def test_xkv_prefix_special_values(kvx, cuda, H):
