@@ -61,14 +61,19 @@ cudaError_t launch_rotate(int dtype, bool vec, const RotArgs &a, cudaStream_t s)
 // 16 tokens of one tensor of an XKV prefix, as the loader warps of the prefix kernel take them
 // (built once by kvx_prefix_create; 32 bytes for 16 tokens).
 struct XkvGroup {
-    uint64_t rows;    // address of the first token's sign/mantissa bytes (raw block: BF16 values)
-    uint32_t codes;   // from there to its residual codes
+    uint64_t rows;    // first token's sign/mantissa bytes, down to the 16-byte line they start in (raw block:
+                      // address of its BF16 values)
+    uint64_t codes;   // its residual codes, likewise
     uint32_t esc;     // first escape entry (index in XkvDev::esc)
     uint32_t b7;      // the block's merge words (index in XkvDev::b7)
-    uint16_t n_esc;
-    uint8_t mode;     // 0 raw, 2, 3, 4
-    uint8_t n;        // tokens (0 past the block's end)
-    uint32_t pad[2];
+    uint16_t n_rows;  // bytes to copy from rows and from codes (multiples of 16; 0: nothing, a raw block or
+    uint16_t n_codes; // no tokens)
+    uint32_t bits;    // escapes | tokens << 13 | mode << 18 | (offset of the rows / 2) << 21 | of the codes << 24
+    __host__ __device__ int n_esc() const { return int(bits & 0x1FFFu); }
+    __host__ __device__ int n() const { return int((bits >> 13) & 31u); }     // 0 past the block's end
+    __host__ __device__ int mode() const { return int((bits >> 18) & 7u); }   // 0 raw, 2, 3, 4
+    __host__ __device__ uint32_t row_off() const { return (bits >> 20) & 14u; }
+    __host__ __device__ uint32_t code_off() const { return (bits >> 23) & 14u; }
 };
 static_assert(sizeof(XkvGroup) == 32, "XkvGroup is 32 bytes");
 

@@ -294,23 +294,20 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                 return reinterpret_cast<const uint4 *>(groups + (2 * tile + (v ? 1 : 0)) * (TT / 16) + (id & 3));
             };
             auto staged = [&](int k) { return bar(B_COUNT + w * NS + k % NS); };
-            // group k into its staging slot: the table entry, and the copies of a coded group
+            // group k into its staging slot: the table entry, and the copies of a coded group (lane 0 the
+            // rows, lane 1 the codes)
             auto issue = [&](int k, const uint4 &e0, const uint4 &e1) {
                 const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
-                const uint64_t rows = (uint64_t(e0.y) << 32) | e0.x, codes = rows + e0.z;
-                const uint32_t mode = (e1.y >> 16) & 0xFFu, n = e1.y >> 24;
-                // lane 0: the rows, lane 1: the codes (each the 16-byte aligned superset)
-                const uint64_t at = lane == 0 ? rows : codes;
-                const uint32_t len = (uint32_t(at & 15u) + (lane == 0 ? n * D : n * D * mode / 8) + 15u) & ~15u;
-                const bool copied = mode != 0 && n > 0;
-                const uint32_t both = len + __shfl_sync(FULL, len, 1);
+                const uint32_t len = lane == 0 ? e1.z & 0xFFFFu : e1.z >> 16;
                 if (lane == 0) {
                     sts_v4(slot, e0.x, e0.y, e0.z, e0.w);
                     sts_v4(slot + 16, e1.x, e1.y, e1.z, e1.w);
-                    mbar_arrive_expect_tx(staged(k), copied ? both : 0u);
+                    mbar_arrive_expect_tx(staged(k), (e1.z & 0xFFFFu) + (e1.z >> 16));
                 }
-                if (lane < 2 && copied)
-                    bulk_g2s(slot + (lane == 0 ? C::S_ROWS : C::S_CODES), reinterpret_cast<const void *>(at & ~uint64_t(15)), len, staged(k));
+                if (lane < 2 && len != 0u) {
+                    const uint64_t at = lane == 0 ? (uint64_t(e0.y) << 32) | e0.x : (uint64_t(e0.w) << 32) | e0.z;
+                    bulk_g2s(slot + (lane == 0 ? C::S_ROWS : C::S_CODES), reinterpret_cast<const void *>(at), len, staged(k));
+                }
             };
             uint4 e0 = make_uint4(0u, 0u, 0u, 0u), e1 = e0;
             int issued = 0;
@@ -322,40 +319,43 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             __syncwarp();
             // what a group needs from global memory besides its copies, fetched a group ahead: the
             // lane's merge words and escape entry
-            uint4 h0, h1, b7n = make_uint4(0u, 0u, 0u, 0u);
+            XkvGroup next;
+            uint4 b7n = make_uint4(0u, 0u, 0u, 0u);
             uint32_t escn = 0;
             auto fetch = [&](int k) {
                 const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
+                uint4 h0, h1;
                 lds_v4(slot, h0.x, h0.y, h0.z, h0.w);
                 lds_v4(slot + 16, h1.x, h1.y, h1.z, h1.w);
-                if (((h1.y >> 16) & 0xFFu) != 0) b7n = __ldg(reinterpret_cast<const uint4 *>(a.xkv.b7 + h1.x) + c8);
-                if (lane < int(h1.y & 0xFFFFu)) escn = __ldg(a.xkv.esc + h0.w + lane);
+                next.rows = (uint64_t(h0.y) << 32) | h0.x;
+                next.esc = h1.x, next.b7 = h1.y, next.bits = h1.w;
+                if (next.mode() != 0) b7n = __ldg(reinterpret_cast<const uint4 *>(a.xkv.b7 + next.b7) + c8);
+                if (lane < next.n_esc()) escn = __ldg(a.xkv.esc + next.esc + lane);
             };
             if (mine > 0) fetch(0);
             bool ok = true;
             int k = 0;
             for (; k < mine; ++k) {
                 const int id = w + LW * k, q = id >> 2, j0 = 16 * (id & 3);
-                const uint4 g0 = h0, g1 = h1;
+                const XkvGroup grp = next;
                 const uint32_t b7[4] = {b7n.x, b7n.y, b7n.z, b7n.w}, ent = escn;
                 if (k + 1 < mine) fetch(k + 1);
                 if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
                 if (ok) ok = __all_sync(FULL, wait(staged(k), k / NS));
                 if (!ok) break;
-                const uint64_t rows = (uint64_t(g0.y) << 32) | g0.x;
-                const int n_esc = int(g1.y & 0xFFFFu), mode = int((g1.y >> 16) & 0xFFu), n = int(g1.y >> 24);
+                const int n_esc = grp.n_esc(), mode = grp.mode(), n = grp.n();
                 const uint32_t slot = stages + uint32_t(k % NS * C::STAGE);
                 const uint32_t dst = sb + uint32_t(C::O_RING + (q % C::NSLOT) * C::SLOT);
-                const Lay ly = make_lay<D>(uint32_t(rows) & 15u, uint32_t(rows + g0.z) & 15u, mode, c8, false, C::S_CODES - C::S_ROWS);
+                const Lay ly = make_lay<D>(grp.row_off(), grp.code_off(), mode, c8, false, C::S_CODES - C::S_ROWS);
                 const uint32_t sr = slot + C::S_ROWS + ly.rows + uint32_t(r0 * D), sc = slot + C::S_ROWS + ly.codes;
                 if (mode == 4) decode_group<D, 4>(sr, sc + uint32_t(r0 * (D / 2)), 0, ly, b7, dst, j0, n, lane);
                 else if (mode == 2) decode_group<D, 2>(sr, sc + uint32_t(r0 * (D / 4)), 0, ly, b7, dst, j0, n, lane);
                 else if (mode == 3) decode_group<D, 3>(sr, sc + uint32_t(r0 * (D * 3 / 8)), 0, ly, b7, dst, j0, n, lane);
-                else decode_group<D, 0>(0, 0, rows, ly, b7, dst, j0, n, lane);
+                else decode_group<D, 0>(0, 0, grp.rows, ly, b7, dst, j0, n, lane);
                 __syncwarp();
                 // escapes: the entry's element by its byte in a 16-row tile (swizzled like this one's rows)
                 for (int i = lane; i < n_esc; i += 32) {
-                    const uint32_t e = i == lane ? ent : __ldg(a.xkv.esc + g0.w + i);
+                    const uint32_t e = i == lane ? ent : __ldg(a.xkv.esc + grp.esc + i);
                     const uint32_t at = e & 0xFFFEu, r = at / (2 * D), in_row = at % (2 * D);
                     if (int(r) < n)
                         sts_u16(dst + (in_row / C::ROWB) * (TT * C::ROWB) + (uint32_t(j0) + r) * C::ROWB + in_row % C::ROWB, e >> 16);
@@ -738,20 +738,27 @@ __global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int
         for (int j = 0; j < TT / 16; ++j) {
             const int g16 = sub * (TT / 16) + j, t0 = 16 * g16;
             XkvGroup g{};
-            g.mode = uint8_t(mode);
             const int m = int(d.valid) - t0;
-            g.n = uint8_t(m < 0 ? 0 : (m < 16 ? m : 16));
+            const uint32_t n_tok = uint32_t(m < 0 ? 0 : (m < 16 ? m : 16));
+            uint32_t n_esc = 0, row_off = 0, code_off = 0;
             g.b7 = uint32_t(d.b7_block) * uint32_t(dim) + uint32_t(T * (dim / 2));
-            if (g.n > 0) {
-                const uint64_t rows = blk + kHeaderBytes + (mode != 0 ? dim : 0);
-                g.rows = rows + uint64_t(t0) * dim * (mode != 0 ? 1 : 2);
-                g.codes = mode != 0 ? uint32_t(int(d.n_tok) * dim + t0 * dim * mode / 8 - t0 * dim) : 0u;
-                if (mode != 0 && nesc != 0) {
+            if (n_tok > 0 && mode == 0) {
+                g.rows = blk + kHeaderBytes + uint64_t(t0) * dim * 2;
+                row_off = uint32_t(g.rows & 2u);
+            } else if (n_tok > 0) {
+                const uint64_t rows = blk + kHeaderBytes + dim + uint64_t(t0) * dim;
+                const uint64_t codes = blk + kHeaderBytes + dim + uint64_t(d.n_tok) * dim + uint64_t(t0) * dim * mode / 8;
+                row_off = uint32_t(rows & 15u), code_off = uint32_t(codes & 15u);
+                g.rows = rows - row_off, g.codes = codes - code_off;
+                g.n_rows = uint16_t((row_off + n_tok * dim + 15u) & ~15u);
+                g.n_codes = uint16_t((code_off + n_tok * dim * mode / 8 + 15u) & ~15u);
+                if (nesc != 0) {
                     const int e0 = g16 == 0 ? 0 : d.em[T][g16 - 1], e1 = d.em[T][g16];
                     g.esc = (T ? d.v_rec : d.k_rec) + uint32_t(kEscRecHead + e0);
-                    g.n_esc = uint16_t(e1 - e0);
+                    n_esc = uint32_t(e1 - e0);
                 }
             }
+            g.bits = n_esc | (n_tok << 13) | (uint32_t(mode) << 18) | (row_off << 20) | (code_off << 23);
             groups[(i * 2 + T) * (TT / 16) + j] = g;
         }
     }
