@@ -47,18 +47,17 @@ double stream_share(int dim, int64_t prefix_tiles, int64_t tail_tiles) {
     return share >= kLeastShare && share <= kMostShare ? share : 0.0;
 }
 
-// The cut of a prefix for the tensor-core kernel: tiles a split, the splits that end soonest when
-// `slots` CTAs run at a time and an item costs its tiles and about kItemTiles more (its queries,
-// the pipeline's fill and the write of its state).
-constexpr int kItemTiles = 4;
+// The cut of a prefix for the tensor-core kernel: tiles an item, such that the work of `lists` (KV head,
+// 128 rows) pairs ends soonest when `slots` CTAs run at a time.  In tiles' time an item costs its tiles
+// and kItemTiles (its queries, the pipeline's fill and drain, the write of its state), and the combine
+// pass kPartTiles for every part of a row.
+constexpr double kItemTiles = 5.0, kPartTiles = 0.15;
 int prefix_split_tiles(int tiles, int lists, int slots) {
     int best = tiles;
-    int64_t least = INT64_MAX;
-    for (int waves = 1; waves <= 4; ++waves) {
-        const int splits = std::max(1, int(int64_t(waves) * slots / lists));
-        const int per = ceil_div(tiles, splits);
-        const int64_t items = int64_t(ceil_div(tiles, per)) * lists;
-        const int64_t cost = (items + slots - 1) / slots * (per + kItemTiles);
+    double least = 1e300;
+    for (int splits = 1; splits <= tiles && splits <= std::max(1, 2 * slots / lists); ++splits) {
+        const int per = ceil_div(tiles, splits), parts = ceil_div(tiles, per);
+        const double cost = ceil_div(int64_t(parts) * lists, slots) * (per + kItemTiles) + kPartTiles * parts;
         if (cost < least) least = cost, best = per;
     }
     return best;

@@ -78,9 +78,9 @@ struct XkvGroup {
 static_assert(sizeof(XkvGroup) == 32, "XkvGroup is 32 bytes");
 
 // An XKV prefix: every block takes the same number of tiles of kPrefixTile tokens (fewer tokens or none
-// in the last ones), every tile four groups a tensor.
+// in the last ones), every tile a group for each 16 tokens and tensor.
 struct XkvDev {
-    const XkvGroup *groups;      // [kv head][tile][K, V][4]
+    const XkvGroup *groups;      // [kv head][tile][K, V][kPrefixTile / 16]
     const uint8_t *tile_tokens;  // [kv head][tile]
     const uint32_t *esc, *b7;
     int32_t head_tiles;          // of a head (0: no XKV prefix)

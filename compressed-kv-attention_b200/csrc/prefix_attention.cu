@@ -11,9 +11,9 @@
 //    64 / R boxes of R tokens (R the power of two, at most 64, that divides the page) a panel.  For
 //    other lengths three warps copy row by row, 16 bytes a thread.  (TMA for the long pages is what
 //    lets the other roles run: the row copies take about 1600 cycles a tile of 128 dims.)
-//  * One more warp issues the MMAs (one thread): S(i) = Q K(i)^T into one of two TMEM buffers, then
-//    O += P(i - 1) V(i - 1) with P read from TMEM (it replaces S there), so that S(i) is computed
-//    while the softmax of tile i - 1 runs.  V is the N-major operand: the same rows as stored.
+//  * One more warp issues the MMAs (one thread): S(i) = Q K(i)^T into one of two TMEM buffers, then O +=
+//    P(i - 1) V(i - 1) with P read from TMEM (it replaces S there), so that S(i) is computed while the
+//    softmax of tile i - 1 runs.  V is the N-major operand: the same rows as stored.
 //  * Warps 0-3 do the softmax, a thread to a row: no shuffles.  The maximum that weights are
 //    relative to is raised, and O rescaled in TMEM, only when some row's scores pass it by 2^8
 //    (2^5 for FP16 weights), which is rare after the first tile; l and O share it, so it cancels.
@@ -25,10 +25,9 @@
 // multiply-add a pair, escapes stored over them, rows past the block's end as zeros.  The blocks are
 // decoded once for the item's 128 rows.
 //
-// What bounds it: per 64-token tile and 128 rows the SM's exponentials take 64 x 128 / 16 = 512
-// cycles, the MMAs 4 D (256 at D = 64, 512 at D = 128) and the tile's bytes from HBM 256 D / 23
-// (712 at D = 64, 1425 at D = 128, shared by all 128-row items of the head through L2).  Two CTAs
-// a SM (one at D = 256) overlap one's softmax with the other's waits.
+// What bounds it: per 64 tokens and 128 rows the SM's exponentials take 64 x 128 / 16 = 512 cycles, the
+// MMAs 4 D (256 at D = 64, 512 at D = 128) and the bytes from HBM 256 D / 23 (712 at D = 64, 1425 at D =
+// 128, shared by all 128-row items of the head through L2).
 #include <cuda.h>
 
 #include <utility>
@@ -63,7 +62,7 @@ template <int D, int LOAD> struct Cfg {
     static constexpr int ROWB = D >= 64 ? 128 : 64;         // bytes of a row of one panel of head dims
     static constexpr int SLOT = TT * D * 2;
     static constexpr int NSLOT = XKV ? (D == 32 ? 16 : (D == 64 ? 10 : (D == 128 ? 5 : 2))) : (D == 32 ? 12 : (D == 64 ? 10 : 5));
-    static constexpr int LAG = NSLOT / 2;                   // row copies: tiles in flight before one is announced
+    static constexpr int LAG = (NSLOT - 1) / 2;                   // row copies: tiles in flight before one is announced
     static constexpr int PANELS = D >= 64 ? D / 64 : 1;
     static constexpr int CTAS = XKV || D == 256 ? 1 : 2;    // per SM
     static constexpr int O_Q = 0;
@@ -75,7 +74,7 @@ template <int D, int LOAD> struct Cfg {
     static constexpr int STAGE = S_CODES + 8 * D + 32;
     static constexpr int O_STAGE = O_RING + NSLOT * SLOT;
     static constexpr int O_BAR = O_STAGE + LW * NSTAGE * STAGE;
-    static constexpr int N_BAR = 2 * NSLOT + 7 + LW * NSTAGE;
+    static constexpr int N_BAR = 2 * NSLOT + 8 + LW * NSTAGE;
     static constexpr int SMEM = O_BAR + 8 * N_BAR + 16;
     // arrivals that announce a tile: one of each loader warp, or one for each 16-token group
     static constexpr int ARRIVE = XKV ? TT / 16 : LW;  // (TMA: with the bytes)
@@ -83,7 +82,7 @@ template <int D, int LOAD> struct Cfg {
     static constexpr int TMEM = D == 256 ? 512 : 256;       // columns: O at 0, S / P buffers at D, D + 64
     static constexpr uint64_t LAYOUT = D >= 64 ? 2 : 4;     // 128- / 64-byte swizzle
     static_assert(PANELS * (TT / 8) <= 32, "a lane for each TMA box");
-    static_assert(XKV || LAG < NSLOT - 1, "the tile that frees the ring's next slot has been announced");
+    static_assert(XKV || LAG < NSLOT - 1 || LAG == 0, "the tile that frees the ring's next slot has been announced");
     static_assert(ROWS * LDO * 4 <= O_BAR, "the staged outputs fit where Q and the ring were");
     static_assert(D + 2 * TT <= TMEM && CTAS * TMEM <= 512, "TMEM columns");
     static_assert(CTAS * (SMEM + 1024) <= 233472, "shared memory");
@@ -170,9 +169,46 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, i
         : "memory");
 }
 
+// 64 scores of this thread's row from TMEM, those from token `valid` on as -inf.
+__device__ __forceinline__ void load_scores(uint32_t addr, int valid, uint32_t (&x)[64]) {
+    uint32_t(&a)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[0]), (&b)[32] = *reinterpret_cast<uint32_t(*)[32]>(&x[32]);
+    tmem_ld32(addr, a);
+    tmem_ld32(addr + 32, b);
+    tmem_wait_ld(a);
+    tmem_wait_ld(b);
+    if (valid < 64) {
+#pragma unroll
+        for (int j = 0; j < 64; ++j)
+            if (j >= valid) x[j] = 0xFF800000u;
+    }
+}
+
+// Pairs of FP32 values in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void unpair(uint64_t x, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // Barriers of a CTA (8 bytes each): full and empty of every ring slot, these, then one for each
 // staging slot.
-enum { B_S0, B_S1, B_P0, B_P1, B_PV, B_Q, B_END, B_COUNT };
+enum { B_S0, B_S1, B_P0, B_P1, B_PV, B_Q, B_END, B_DONE, B_COUNT };
 
 // One item.
 struct Item {
@@ -194,9 +230,15 @@ __device__ __forceinline__ Item item_of(const PagedArgs &a, int i) {
     return x;
 }
 
-// The ring's order: K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1).
-__device__ __forceinline__ int k_item(int i) { return i == 0 ? 0 : 2 * i - 1; }
-__device__ __forceinline__ int v_item(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
+// The ring's order for n tiles: K0, K1, V0, K2, V1, ..., K(n-1), V(n-2), V(n-1).
+struct Ring {
+    static __device__ __forceinline__ int k_item(int i) { return i == 0 ? 0 : 2 * i - 1; }
+    static __device__ __forceinline__ int v_item(int i, int n) { return i == n - 1 ? 2 * n - 1 : 2 * i + 2; }
+    static __device__ __forceinline__ bool is_v(int q, int n) { return q == 2 * n - 1 || (q > 0 && (q & 1) == 0); }
+    static __device__ __forceinline__ int tile(int q, int n) {
+        return q == 0 ? 0 : (q == 2 * n - 1 ? n - 1 : (is_v(q, n) ? q / 2 - 1 : (q + 1) / 2));
+    }
+};
 
 // Chunk steps of one 16-token group: rebuild them from the staged sections (coded modes) or the raw
 // rows into the tile at `dst` (rows j0 .. j0 + 15), rows at or past n as zeros.
@@ -268,6 +310,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
         for (int i = 0; i < LW * C::NSTAGE; ++i) mbar_init(bar(B_COUNT + i), 1);
         mbar_init(bar(B_S0), 1), mbar_init(bar(B_S1), 1), mbar_init(bar(B_P0), SW), mbar_init(bar(B_P1), SW);
         mbar_init(bar(B_PV), 1), mbar_init(bar(B_Q), SW), mbar_init(bar(B_END), 1);
+        mbar_init(bar(B_DONE), 1);
         fence_mbar_init();
     }
     fence_before();
@@ -277,21 +320,18 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
 
     if (warp >= SW && warp < SW + LW) {
         // ---- loads ----
-        // tile of ring item q, and which of K and V: K of the next tile, then V of the one before
-        auto is_v_item = [&](int q) { return q == 2 * it.tiles - 1 || (q > 0 && (q & 1) == 0); };
+        const int n_items = 2 * it.tiles;
         if constexpr (XKV) {
             // Loader warp w takes the 16-token groups w, w + LW, ... of the ring's items in order: each
             // tile's four arrivals come from whichever warps had them.
             constexpr int C8 = D / 8, NS = C::NSTAGE;
             const int w = warp - SW, c8 = lane % C8, r0 = lane / C8;
-            const int total = 2 * it.tiles * (TT / 16), mine = (total - w + LW - 1) / LW;
+            const int total = n_items * (TT / 16), mine = (total - w + LW - 1) / LW;
             const uint32_t stages = sb + uint32_t(C::O_STAGE + w * NS * C::STAGE);
             const XkvGroup *groups = a.xkv.groups + int64_t(it.head) * a.xkv.head_tiles * (2 * (TT / 16));
             auto entry = [&](int k) -> const uint4 * {
-                const int id = w + LW * k, q = id >> 2;
-                const bool v = is_v_item(q);
-                const int tile = it.tile0 + (q == 0 ? 0 : (q == 2 * it.tiles - 1 ? it.tiles - 1 : (v ? q / 2 - 1 : (q + 1) / 2)));
-                return reinterpret_cast<const uint4 *>(groups + (2 * tile + (v ? 1 : 0)) * (TT / 16) + (id & 3));
+                const int id = w + LW * k, q = id / (TT / 16), tile = it.tile0 + Ring::tile(q, it.tiles);
+                return reinterpret_cast<const uint4 *>(groups + (2 * tile + (Ring::is_v(q, it.tiles) ? 1 : 0)) * (TT / 16) + id % (TT / 16));
             };
             auto staged = [&](int k) { return bar(B_COUNT + w * NS + k % NS); };
             // group k into its staging slot: the table entry, and the copies of a coded group (lane 0 the
@@ -336,7 +376,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             bool ok = true;
             int k = 0;
             for (; k < mine; ++k) {
-                const int id = w + LW * k, q = id >> 2, j0 = 16 * (id & 3);
+                const int id = w + LW * k, q = id / (TT / 16), j0 = 16 * (id % (TT / 16));
                 const XkvGroup grp = next;
                 const uint32_t b7[4] = {b7n.x, b7n.y, b7n.z, b7n.w}, ent = escn;
                 if (k + 1 < mine) fetch(k + 1);
@@ -393,16 +433,17 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             int32_t pg_k = 0, pg_before = 0, pg_next = look_up(0, place_next);
             bool ok = true;
             int q = 0;
-            for (; q < 2 * it.tiles; ++q) {
-                const bool last = q == 2 * it.tiles - 1, is_v = is_v_item(q);
+            for (; q < n_items; ++q) {
+                const bool is_v = Ring::is_v(q, it.tiles);
+                const int tile = Ring::tile(q, it.tiles);
                 if (!is_v) {
                     pg_before = pg_k, place_before = place_k;
                     pg_k = pg_next, place_k = place_next;
-                    pg_next = look_up((q + 1) / 2 + 1, place_next);
+                    pg_next = look_up(tile + 1, place_next);
                 }
                 if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
                 if (!ok) break;
-                const bool before = is_v && !last;
+                const bool before = is_v && q < n_items - 1;
                 const int32_t pg = before ? pg_before : pg_k;
                 const int place = before ? place_before : place_k;
                 bool live = place >= 0;
@@ -413,7 +454,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                 const uint32_t dst = sb + uint32_t(C::O_RING + (q % C::NSLOT) * C::SLOT);
                 // V rows past the prefix's end meet weights of 0 and must be finite: that tile's boxes
                 // are waited for here and the rows zeroed before the tile is announced
-                const int valid = a.prefix_len - (it.tile0 + (last ? it.tiles : q / 2) - 1) * TT;
+                const int valid = a.prefix_len - (it.tile0 + tile) * TT;
                 const bool ends = is_v && valid < TT;
                 const uint32_t to = ends ? bar(B_END) : full(q);
                 const uint32_t boxes = uint32_t(__popc(__ballot_sync(FULL, live)));
@@ -436,54 +477,63 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             if (!ok)
                 for (int i = max(0, q - C::NSLOT); i < q; ++i) mbar_wait_bounded(full(i), uint32_t((i / C::NSLOT) & 1), kWaitUs);
         } else {
-        // Loader warp w copies rows w, w + LW, ... of every tile: lane k holds the offset of row w +
-        // LW k (-1: no such token), looked up a tile ahead of its use.
+        // Loader warp w copies rows w, w + LW, ... of every tile: lane k holds the offsets of rows w + LW k
+        // and w + LW (k + 32) (-1: no such token), looked up a tile ahead of their use.
         constexpr int CH = D / 8, RPS = 32 / CH;              // pieces a row, rows a step
-        constexpr int MINE = (TT + LW - 1) / LW, STEPS = (MINE + RPS - 1) / RPS;
+        constexpr int MINE = (TT + LW - 1) / LW, STEPS = (MINE + RPS - 1) / RPS, H = (MINE + 31) / 32;
         const int w = warp - SW, c = lane % CH;
         const int64_t head = int64_t(it.head) * a.pool.head_stride + 8 * c;
-        // (nothing looks at the entry before the next K tile: its load is not waited for here)
-        int place_next = -1;
-        auto look_up = [&](int tile) -> int32_t {
-            const int r = w + LW * lane, tok = (it.tile0 + tile) * TT + r;
-            place_next = -1;
-            if (r >= TT || tok >= a.prefix_len || tile >= it.tiles) return 0;
-            int64_t i;
-            a.pool.split.at(tok, i, place_next);
-            return __ldg(a.prefix_table + i);
-        };
-        auto row_of = [&](int32_t page, int place) -> int64_t {
-            if (place < 0) return -1;
-            if (unsigned(page) < unsigned(a.pool.n_pages)) return int64_t(page) * a.pool.page_stride + int64_t(place) * a.pool.token_stride;
-            report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
-            return -1;
+        // (nothing looks at the entries before the next K tile: their loads are not waited for here)
+        int32_t page_next[H];
+        int place_next[H];
+        auto look_up = [&](int tile) {
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                const int r = w + LW * (lane + 32 * h), tok = (it.tile0 + tile) * TT + r;
+                place_next[h] = -1, page_next[h] = 0;
+                if (r < TT && tok < a.prefix_len && tile < it.tiles) {
+                    int64_t i;
+                    a.pool.split.at(tok, i, place_next[h]);
+                    page_next[h] = __ldg(a.prefix_table + i);
+                }
+            }
         };
         auto announce = [&](int i) {
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(full(i));
         };
-        // rows of the latest K tile, of the one before it (V follows a tile behind) and of the next
-        int64_t r_k = -1, r_before = -1;
-        int32_t pg_next = look_up(0);
+        // rows of the latest K tile and of the one before it (V follows a tile behind)
+        int64_t r_k[H], r_before[H];
+        look_up(0);
+#pragma unroll
+        for (int h = 0; h < H; ++h) r_k[h] = r_before[h] = -1;
         bool ok = true;
         int q = 0;
-        for (; q < 2 * it.tiles; ++q) {
-            const bool last = q == 2 * it.tiles - 1, is_v = is_v_item(q);
+        for (; q < n_items; ++q) {
+            const bool is_v = Ring::is_v(q, it.tiles);
             if (!is_v) {
-                r_before = r_k;
-                r_k = row_of(pg_next, place_next);
-                pg_next = look_up((q + 1) / 2 + 1);
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    r_before[h] = r_k[h];
+                    r_k[h] = -1;
+                    if (place_next[h] < 0) continue;
+                    if (unsigned(page_next[h]) < unsigned(a.pool.n_pages))
+                        r_k[h] = int64_t(page_next[h]) * a.pool.page_stride + int64_t(place_next[h]) * a.pool.token_stride;
+                    else report(a.status, KVX_ERR_RUNTIME, DERR_PAGE);
+                }
+                look_up(Ring::tile(q, it.tiles) + 1);
             }
             if (q >= C::NSLOT) ok = __all_sync(FULL, wait(empty(q), q / C::NSLOT - 1));
             if (!ok) break;
             const uint16_t *src = (is_v ? a.pool.v : a.pool.k) + head;
             const uint32_t dst = sb + uint32_t(C::O_RING + (q % C::NSLOT) * C::SLOT);
-            const int64_t mine = is_v && !last ? r_before : r_k;
+            const bool before = is_v && q < n_items - 1;
 #pragma unroll
             for (int j = 0; j < STEPS; ++j) {
                 const int k = j * RPS + lane / CH, r = w + LW * k;
-                const int64_t o = __shfl_sync(FULL, mine, k);
+                const int h = j * RPS / 32;
+                const int64_t o = __shfl_sync(FULL, before ? r_before[h] : r_k[h], k & 31);
                 if (r < TT) copy16(dst + tile_off<D, TT>(r, c), src + (o >= 0 ? o : 0), o >= 0);
             }
             copy_commit();
@@ -506,7 +556,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                            v0 = smem_desc(sb + C::O_RING, TT * C::ROWB, K8, C::LAYOUT);
             for (int i = 0; i <= it.tiles; ++i) {
                 if (i < it.tiles) {
-                    const int x = k_item(i);
+                    const int x = Ring::k_item(i);
                     if (!wait(full(x), x / C::NSLOT)) break;
                     fence_after();
                     const uint64_t kk = k0 + uint32_t(x % C::NSLOT) * uint32_t(C::SLOT / 16);
@@ -520,16 +570,16 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     mma_commit(bar(B_S0 + (i & 1)));
                 }
                 if (i > 0) {
-                    const int j = i - 1, x = v_item(j, it.tiles);
+                    const int j = i - 1, x = Ring::v_item(j, it.tiles);
                     if (!wait(full(x), x / C::NSLOT) || !wait(bar(B_P0 + (j & 1)), j >> 1)) break;
                     fence_after();
                     const uint64_t vv = v0 + uint32_t(x % C::NSLOT) * uint32_t(C::SLOT / 16);
 #pragma unroll
                     for (int s = 0; s < TT / 16; ++s)
-                        mma_ts(tm, tm + D + (j & 1) * TT + 8 * s, vv + 2 * s * K8 / 16,
-                               pv, j > 0 || s > 0);
+                        mma_ts(tm, tm + D + (j & 1) * TT + 8 * s, vv + 2 * s * K8 / 16, pv, j > 0 || s > 0);
                     mma_commit(empty(x));
                     mma_commit(bar(B_PV));
+                    if (j == it.tiles - 1) mma_commit(bar(B_DONE));
                 }
             }
         }
@@ -566,21 +616,17 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             bool pv_seen = i == 0;  // PV(i - 1) has completed
             if (live) {
                 const uint32_t st = tm + lanes + uint32_t(D + (i & 1) * TT);
-                uint32_t x0[32], x1[32];
-                tmem_ld32(st, x0);
-                tmem_ld32(st + 32, x1);
-                tmem_wait_ld(x0);
-                tmem_wait_ld(x1);
-                if (valid < TT) {
+                uint32_t x[64];
+                load_scores(st, valid, x);
+                float y[4];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        if (j >= valid) x0[j] = 0xFF800000u;
-                        if (j + 32 >= valid) x1[j] = 0xFF800000u;
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    y[k] = __uint_as_float(x[k]);
+#pragma unroll
+                    for (int j = 4; j + 4 < 64; j += 8) y[k] = max3(y[k], __uint_as_float(x[j + k]), __uint_as_float(x[j + 4 + k]));
+                    y[k] = fmaxf(y[k], __uint_as_float(x[60 + k]));
                 }
-                float mx = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) mx = fmaxf(mx, fmaxf(__uint_as_float(x0[j]), __uint_as_float(x1[j])));
+                float mx = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));
                 mx *= a.scale_log2;
                 if (__any_sync(FULL, mx > m + kGrow || (m == -INFINITY && mx > m))) {
                     const float mn = fmaxf(m, mx);
@@ -589,7 +635,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     l *= al;
                     if (i > 0) {
                         // O is complete up to tile i - 1, and the next PV waits for this warp
-                        ok = __all_sync(FULL, wait(bar(B_PV), i - 1));
+                        if (!pv_seen) ok = __all_sync(FULL, wait(bar(B_PV), i - 1));
                         if (!ok) break;
                         pv_seen = true;
                         fence_after();
@@ -605,18 +651,21 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     }
                 }
                 const float mu = m == -INFINITY ? 0.f : m - Elem<DT>::kBias;
+                const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), mu2 = pair(-mu, -mu);
+                uint64_t sum[2] = {pair(l, 0.f), pair(0.f, 0.f)};
                 uint32_t p[32];
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const float u = exp2_sfu(__fmaf_rn(__uint_as_float(x0[2 * j]), a.scale_log2, -mu));
-                    const float v = exp2_sfu(__fmaf_rn(__uint_as_float(x0[2 * j + 1]), a.scale_log2, -mu));
-                    const float w = exp2_sfu(__fmaf_rn(__uint_as_float(x1[2 * j]), a.scale_log2, -mu));
-                    const float z = exp2_sfu(__fmaf_rn(__uint_as_float(x1[2 * j + 1]), a.scale_log2, -mu));
+                for (int j = 0; j < 32; ++j) {
+                    float u, v;
+                    unpair(fma2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), scale2, mu2), u, v);
+                    u = exp2_sfu(u), v = exp2_sfu(v);
+                    sum[j & 1] = add2(sum[j & 1], pair(u, v));
                     p[j] = Elem<DT>::pack(u, v);
-                    p[16 + j] = Elem<DT>::pack(w, z);
-                    l += (u + v) + (w + z);
                 }
                 tmem_st32(st, p);
+                float u, v;
+                unpair(add2(sum[0], sum[1]), u, v);
+                l = u + v;
                 tmem_wait_st();
             }
             // B_PV is waited for once a tile, before the arrival that lets its next phase begin: a
@@ -627,7 +676,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(B_P0 + (i & 1)));
         }
-        if (ok) ok = __all_sync(FULL, wait(bar(B_PV), it.tiles - 1));
+        if (ok) ok = __all_sync(FULL, wait(bar(B_DONE), 0));
         if (ok && live) {
             // every copy and MMA of the CTA has completed: Q and the ring make room for the rows
             fence_after();
@@ -718,12 +767,12 @@ template <int D, int DT> cudaError_t prefix_d(const PagedArgs &args, cudaStream_
     if constexpr (DT == KVX_DTYPE_BF16)
         if (a.xkv.tiles > 0) return prefix_launch<D, DT, LOAD_XKV>(a, maps, s);
     // boxes of fewer than 8 tokens would not fill a swizzle pattern
-    for (a.box_tokens = TT; a.pool.split.tokens % a.box_tokens != 0;) a.box_tokens >>= 1;
+    for (a.box_tokens = kPrefixTile; a.pool.split.tokens % a.box_tokens != 0;) a.box_tokens >>= 1;
     if (a.box_tokens >= 8 && encode_maps(D, DT, a, maps)) return prefix_launch<D, DT, LOAD_TMA>(a, maps, s);
     return prefix_launch<D, DT, LOAD_ROWS>(a, maps, s);
 }
 
-// One thread per (flat block, tile): its eight groups and its token count.
+// One thread per (flat block, tile): its groups and its token count.
 __global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int dim, XkvGroup *groups, uint8_t *tokens) {
     const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
     if (i >= n * tpb) return;
