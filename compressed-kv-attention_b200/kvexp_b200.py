@@ -17,6 +17,7 @@ from __future__ import annotations
 import ctypes as C
 import enum
 import os
+import struct
 
 import numpy as np
 
@@ -147,22 +148,28 @@ class kvx_rope(C.Structure):
 
 
 class kvx_attend(C.Structure):
-    _fields_ = [("q", kvx_view), ("out", kvx_view), ("lse", _vp), ("pages", C.POINTER(kvx_pages)),
+    _fields_ = [("q", kvx_view), ("out", kvx_view), ("lse", _vp), ("pages", _vp),
                 ("prefix_table", _vp), ("prefix", _vp), ("table", _vp), ("lens", _vp), ("table_stride", C.c_int64),
                 ("prefix_len", C.c_int32), ("max_len", C.c_int32), ("batch", C.c_int32),
                 ("scale", C.c_float)]
 
 
+# The serving-step calls take these structs many times a token: they go as packed bytes, whose address
+# ctypes passes as it is (building the ctypes objects costs several microseconds a call).
+_pack_view = struct.Struct("@Pqq").pack
+_pack_rope = struct.Struct("@PPPPqiiii").pack
+_pack_attend = struct.Struct("@PqqPqqPPPPPPqiiif").pack
+assert struct.calcsize("@Pqq") == C.sizeof(kvx_view) and struct.calcsize("@PPPPqiiii") == C.sizeof(kvx_rope)
+assert struct.calcsize("@PqqPqqPPPPPPqiiif") == C.sizeof(kvx_attend)
+_buf = C.c_char_p
+
 _batch_create = _sig("kvx_batch_create", C.c_int,
                      [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(_vp)])
 _batch_rotate = _sig("kvx_batch_rotate", C.c_int,
-                     [_vp, C.POINTER(kvx_view), C.POINTER(kvx_view), C.c_int, C.c_int,
-                      C.POINTER(kvx_rope), C.c_int, _vp])
+                     [_vp, _buf, _buf, C.c_int, C.c_int, _buf, C.c_int, _vp])
 _batch_append = _sig("kvx_batch_append", C.c_int,
-                     [_vp, C.POINTER(kvx_view), C.POINTER(kvx_view), C.POINTER(kvx_view),
-                      C.POINTER(kvx_view), C.c_int, C.POINTER(kvx_rope), _vp, C.POINTER(kvx_pages),
-                      _vp])
-_batch_attend = _sig("kvx_batch_attend", C.c_int, [_vp, C.POINTER(kvx_attend), _vp])
+                     [_vp, _buf, _buf, _buf, _buf, C.c_int, _buf, _vp, _buf, _vp])
+_batch_attend = _sig("kvx_batch_attend", C.c_int, [_vp, _buf, _vp])
 _batch_check = _sig("kvx_batch_check", C.c_int, [_vp])
 _batch_destroy = _sig("kvx_batch_destroy", None, [_vp])
 _prefix_create = _sig("kvx_prefix_create", C.c_int, [_vp, C.c_int, C.c_int, C.POINTER(_vp)])
@@ -467,21 +474,22 @@ def exponent_report(kv, seq_len, head_dim, block_tokens=K_ENCODE_BLOCK, bit_widt
 # These calls take CUDA tensors (torch) of any strides whose last dimension is contiguous, run on
 # `stream` (a cudaStream_t address, default the legacy stream) and return at once.
 
-DTYPES = {"bf16": (0, "torch.bfloat16"), "fp16": (1, "torch.float16")}
+DTYPES = {"bf16": (0, "bfloat16"), "fp16": (1, "float16")}
 
 
 def _device_tensor(x, name, dtype, ndim):
     """Checks what the device code takes on trust: a CUDA tensor of this type and rank, its last
-    dimension contiguous."""
+    dimension contiguous.  Returns its strides."""
     if not getattr(x, "is_cuda", False):
         raise ValueError(f"{name} must be a CUDA tensor")
-    if str(x.dtype) != dtype:
+    if x.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
-    if x.dim() != ndim:
-        raise ValueError(f"{name} must have {ndim} dimensions, not {x.dim()}")
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    st = x.stride()
+    if len(st) != ndim:
+        raise ValueError(f"{name} must have {ndim} dimensions, not {len(st)}")
+    if st[-1] != 1 and x.shape[-1] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
-    return x
+    return st
 
 
 class Rope:
@@ -489,32 +497,31 @@ class Rope:
     (time, height, width), axis [rot_dim / 2] uint8 gives each pair's."""
 
     def __init__(self, cos, sin, axis=None, n_axes=1, interleaved=False):
+        import torch
         for name, x in (("cos", cos), ("sin", sin)):
-            _device_tensor(x, name, "torch.float32", 2)
+            _device_tensor(x, name, torch.float32, 2)
             if not x.is_contiguous() or x.shape != cos.shape:
                 raise ValueError("cos and sin must be contiguous and of one shape")
         if axis is not None:
-            _device_tensor(axis, "axis", "torch.uint8", 1)
+            _device_tensor(axis, "axis", torch.uint8, 1)
             if axis.shape[0] != cos.shape[1]:
                 raise ValueError("axis must name one axis for each pair")
         elif n_axes != 1:
             raise ValueError("several axes need the axis of each pair")
         self._keep = (cos, sin, axis)
+        self._int32 = torch.int32
         self.n_axes = int(n_axes)
-        self._fixed = (_addr(cos), _addr(sin)), _addr(axis), (
-            int(cos.shape[0]), 2 * int(cos.shape[1]), self.n_axes, int(bool(interleaved)))
+        self._tables = _addr(cos), _addr(sin)
+        self._axis = _addr(axis) or 0
+        self._rest = int(cos.shape[0]), 2 * int(cos.shape[1]), self.n_axes, int(bool(interleaved))
 
     def _at(self, pos, n_tokens):
         """kvx_rope for positions [n_tokens] or [n_axes, n_tokens] int32."""
-        _device_tensor(pos, "pos", "torch.int32", pos.dim())
-        if pos.dim() == 1:
-            ok = self.n_axes == 1 and pos.shape[0] == n_tokens
-        else:
-            ok = pos.dim() == 2 and pos.shape[0] == self.n_axes and pos.shape[1] == n_tokens
-        if not ok:
+        shape = pos.shape
+        st = _device_tensor(pos, "pos", self._int32, len(shape))
+        if shape != (self.n_axes, n_tokens) and (shape != (n_tokens,) or self.n_axes != 1):
             raise ValueError("pos must be [n_tokens], or [n_axes, n_tokens]")
-        tables, axis, rest = self._fixed
-        return kvx_rope(*tables, pos.data_ptr(), axis, pos.stride(0) if pos.dim() == 2 else 0, *rest)
+        return _pack_rope(*self._tables, pos.data_ptr(), self._axis, st[0] if len(st) == 2 else 0, *self._rest)
 
 
 class Pages:
@@ -523,15 +530,16 @@ class Pages:
 
     def __init__(self, k, v):
         for name, x in (("k", k), ("v", v)):
-            _device_tensor(x, name, str(k.dtype), 4)
+            _device_tensor(x, name, k.dtype, 4)
             if x.shape != k.shape or x.stride() != k.stride():
                 raise ValueError("k and v must have one shape and one set of strides")
         self.k, self.v = k, v
-        self.n_heads, self.dim, self.dtype = int(k.shape[2]), int(k.shape[3]), str(k.dtype)
+        self.n_heads, self.dim, self.dtype = int(k.shape[2]), int(k.shape[3]), k.dtype
         self.page_tokens = int(k.shape[1])
-        self._c = kvx_pages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                            int(k.shape[0]), self.page_tokens)
-        self._ref = C.pointer(self._c)
+        c = kvx_pages(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), int(k.shape[0]),
+                      self.page_tokens)
+        self._c = bytes(c)
+        self._at = C.cast(C.c_char_p(self._c), _vp).value
 
 
 class Prefix:
@@ -554,7 +562,7 @@ class Prefix:
         """Encodes k and v (BF16 CUDA tensors [n_kv_heads, tokens, dim], contiguous) on the GPU."""
         import torch
         for name, x in (("k", k), ("v", v)):
-            _device_tensor(x, name, "torch.bfloat16", 3)
+            _device_tensor(x, name, torch.bfloat16, 3)
             if not x.is_contiguous() or x.shape != k.shape:
                 raise ValueError("k and v must be contiguous and of one shape")
         heads, seq, dim = (int(n) for n in k.shape)
@@ -595,9 +603,11 @@ class Batch:
     "fp16"), with scratch for up to max_batch sequences."""
 
     def __init__(self, max_batch, n_q_heads, n_kv_heads, dim, dtype="bf16"):
+        import torch
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
-        code, self._type = DTYPES[dtype]
+        code, name = DTYPES[dtype]
+        self._type, self._int32, self._int64, self._float32 = getattr(torch, name), torch.int32, torch.int64, torch.float32
         self.n_q_heads, self.n_kv_heads, self.dim = int(n_q_heads), int(n_kv_heads), int(dim)
         h = _vp()
         self._h = None
@@ -606,73 +616,80 @@ class Batch:
         self._h = h
 
     def _view(self, x, name, tokens, heads):
-        _device_tensor(x, name, self._type, 3)
-        if tuple(x.shape) != (tokens, heads, self.dim):
+        """(address, token stride, head stride) of a [tokens, heads, dim] tensor."""
+        st = _device_tensor(x, name, self._type, 3)
+        if x.shape != (tokens, heads, self.dim):
             raise ValueError(f"{name} must be {(tokens, heads, self.dim)}, not {tuple(x.shape)}")
-        st = x.stride()
-        return kvx_view(x.data_ptr(), st[0], st[1])
+        return x.data_ptr(), st[0], st[1]
 
     def _pages(self, pages):
-        if pages.n_heads != self.n_kv_heads or pages.dim != self.dim or pages.dtype != self._type:
+        if pages.n_heads != self.n_kv_heads or pages.dim != self.dim or pages.dtype is not self._type:
             raise ValueError("the page pools have other heads, another head_dim or another type")
-        return pages._ref
+        return pages
 
     def rotate(self, x, pos, rope, out, inverse=False, stream=None):
         """out = x [tokens, heads, dim] rotated by its positions (inverse: back, which is the
         gradient's rotation); out may be x."""
-        n, heads = int(x.shape[0]), int(x.shape[1])
-        _check(_batch_rotate(self._h, self._view(x, "x", n, heads), self._view(out, "out", n, heads), n,
-                             heads, rope._at(pos, n), int(bool(inverse)), stream))
+        n, heads = x.shape[:2]
+        rc = _batch_rotate(self._h, _pack_view(*self._view(x, "x", n, heads)),
+                           _pack_view(*self._view(out, "out", n, heads)), n, heads, rope._at(pos, n),
+                           1 if inverse else 0, stream)
+        if rc:
+            _check(rc)
 
     def append(self, q, k, v, pos, rope, slots, pages, q_out, stream=None):
         """Store new tokens: k [tokens, n_kv_heads, dim] rotated and v at `slots` (int64, page *
         page_tokens + place; negative: not stored), q rotated into q_out (both None: no queries).
         rope None: nothing is rotated."""
-        n = int(k.shape[0])
-        _device_tensor(slots, "slots", "torch.int64", 1)
-        if slots.shape[0] != n:
+        n = k.shape[0]
+        if _device_tensor(slots, "slots", self._int64, 1) and slots.shape[0] != n:
             raise ValueError("slots must be one for each token")
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out go together")
-        _check(_batch_append(
-            self._h, None if q is None else self._view(q, "q", n, self.n_q_heads),
-            self._view(k, "k", n, self.n_kv_heads), self._view(v, "v", n, self.n_kv_heads),
-            None if q is None else self._view(q_out, "q_out", n, self.n_q_heads), n,
-            None if rope is None else rope._at(pos, n), slots.data_ptr(), self._pages(pages), stream))
+        kv = self.n_kv_heads
+        rc = _batch_append(
+            self._h, None if q is None else _pack_view(*self._view(q, "q", n, self.n_q_heads)),
+            _pack_view(*self._view(k, "k", n, kv)), _pack_view(*self._view(v, "v", n, kv)),
+            None if q is None else _pack_view(*self._view(q_out, "q_out", n, self.n_q_heads)), n,
+            None if rope is None else rope._at(pos, n), slots.data_ptr(), self._pages(pages)._c, stream)
+        if rc:
+            _check(rc)
 
     def attend(self, q, out, pages, table, lens, max_len, *, prefix_table=None, prefix_len=0, prefix=None,
                scale=None, lse=None, stream=None):
         """out[b, h] = attention of q [batch, n_q_heads, dim] over the shared prefix (prefix_len
-        tokens in the pages of prefix_table, int32, or a Prefix) and then the first lens[b] tokens of row b of
-        table (int32 [batch, pages]); max_len bounds lens.  lse [batch, n_q_heads] FP32 receives
-        the log-sum-exp of the scaled scores."""
-        n = int(q.shape[0])
+        tokens in the pages of prefix_table, int32, or a Prefix) and then the first lens[b] tokens of
+        row b of table (int32 [batch, pages]); max_len bounds lens.  lse [batch, n_q_heads] FP32
+        receives the log-sum-exp of the scaled scores."""
+        n, heads = q.shape[0], self.n_q_heads
         max_len, prefix_len = int(max_len), int(prefix_len)
-        at_table = at_lens = at_prefix = None
-        stride = 0
+        at_table = at_lens = at_prefix = at_lse = stride = 0
         if max_len > 0:
-            _device_tensor(table, "table", "torch.int32", 2)
-            _device_tensor(lens, "lens", "torch.int32", 1)
+            st = _device_tensor(table, "table", self._int32, 2)
+            _device_tensor(lens, "lens", self._int32, 1)
             if table.shape[0] != n or lens.shape[0] != n:
                 raise ValueError("table and lens must have one row for each sequence")
             if table.shape[1] * pages.page_tokens < max_len:
                 raise ValueError("table rows hold fewer than max_len tokens")
-            at_table, at_lens, stride = table.data_ptr(), lens.data_ptr(), table.stride(0)
+            at_table, at_lens, stride = table.data_ptr(), lens.data_ptr(), st[0]
         if prefix_table is not None and prefix_len > 0:
-            _device_tensor(prefix_table, "prefix_table", "torch.int32", 1)
+            _device_tensor(prefix_table, "prefix_table", self._int32, 1)
             if prefix_table.shape[0] * pages.page_tokens < prefix_len:
                 raise ValueError("prefix_table holds fewer than prefix_len tokens")
             at_prefix = prefix_table.data_ptr()
         if lse is not None:
-            _device_tensor(lse, "lse", "torch.float32", 2)
-            if tuple(lse.shape) != (n, self.n_q_heads) or not lse.is_contiguous():
+            _device_tensor(lse, "lse", self._float32, 2)
+            if lse.shape != (n, heads) or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous [batch, n_q_heads]")
+            at_lse = lse.data_ptr()
         if scale is not None and not scale > 0:
             raise ValueError("scale must be positive")
-        a = kvx_attend(self._view(q, "q", n, self.n_q_heads), self._view(out, "out", n, self.n_q_heads),
-                       None if lse is None else lse.data_ptr(), self._pages(pages), at_prefix,
-                       None if prefix is None else prefix._h, at_table, at_lens, stride, prefix_len, max_len, n, 0.0 if scale is None else scale)
-        _check(_batch_attend(self._h, a, stream))
+        rc = _batch_attend(self._h, _pack_attend(
+            *self._view(q, "q", n, heads), *self._view(out, "out", n, heads), at_lse, self._pages(pages)._at,
+            at_prefix, 0 if prefix is None else prefix._h.value, at_table, at_lens, stride, prefix_len, max_len,
+            n, scale or 0.0), stream)
+        if rc:
+            _check(rc)
 
     def check(self):
         """Synchronise and raise what the device reported since the last check."""

@@ -13,12 +13,12 @@ def test_batch_create_refuses(kvx, args):
 
 
 def test_null_handles(kvx):
-    v = kvx.kvx_view(16, 64, 64)
-    r = kvx.kvx_rope(16, 16, 16, None, 0, 1, 64, 1, 0)
-    p = kvx.kvx_pages(16, 16, 64, 64, 64, 1, 1)
+    v = bytes(kvx.kvx_view(16, 64, 64))
+    r = bytes(kvx.kvx_rope(16, 16, 16, None, 0, 1, 64, 1, 0))
+    p = bytes(kvx.kvx_pages(16, 16, 64, 64, 64, 1, 1))
     assert kvx._batch_rotate(None, v, v, 1, 1, r, 0, None) == kvx.KVX_ERR_INVALID_ARGUMENT
     assert kvx._batch_append(None, None, v, v, None, 1, None, 16, p, None) == kvx.KVX_ERR_INVALID_ARGUMENT
-    assert kvx._batch_attend(None, kvx.kvx_attend(), None) == kvx.KVX_ERR_INVALID_ARGUMENT
+    assert kvx._batch_attend(None, bytes(kvx.kvx_attend()), None) == kvx.KVX_ERR_INVALID_ARGUMENT
     assert kvx._batch_check(None) == kvx.KVX_ERR_INVALID_ARGUMENT
     kvx._batch_destroy(None)
 
