@@ -39,7 +39,8 @@ constexpr int kStreamRows = 8;
 // 128 rows) takes a CTA's room about as long as four streamed tiles of 16 tokens at head dims from 128
 // on and eight below (the softmax of 128 rows does not shrink with the head), and tails are taken to be
 // half of max_len on average.  Shares below kLeastShare or above kMostShare are not worth the cut (the
-// streaming kernel then simply follows): 64 sequences of up to 1024 tokens behind 32K took 82 us one
+// streaming kernel then simply follows), and a coded prefix, whose CTAs take a SM each, shares nothing
+// (32 sequences of up to 512 tokens behind 32731 coded ones: 74 us shared, 64 not): 64 sequences of up to 1024 tokens behind 32K took 82 us one
 // after the other and 70 us sharing, the ones whose tails weigh 2 % or 80 % 3 % and 25 % longer.
 constexpr double kLeastShare = 0.15, kMostShare = 0.6;
 double stream_share(int dim, int64_t prefix_tiles, int64_t tail_tiles) {
@@ -295,7 +296,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
         a.row_groups = ceil_div(rows, kPrefixRows);
         a.row_pad = kPrefixRows * a.row_groups;
         a.prefix_tiles = coded ? a.xkv.tiles : ceil_div(x->prefix_len, kPrefixTile);
-        const double share = stream_share(h->dim, int64_t(a.prefix_tiles) * h->n_kv_heads * a.row_groups,
+        const double share = coded ? 0.0 : stream_share(h->dim, int64_t(a.prefix_tiles) * h->n_kv_heads * a.row_groups,
                                           int64_t(x->batch) * h->n_kv_heads * ceil_div(h->group, 8) * ceil_div(x->max_len, 2 * kStreamTile));
         const int slots = prefix_ctas_per_sm(h->dim, coded) * h->sms;
         a.split_tiles = prefix_split_tiles(a.prefix_tiles, h->n_kv_heads * a.row_groups, std::max(1, int(slots * (1.0 - share))));

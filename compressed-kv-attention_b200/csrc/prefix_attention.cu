@@ -138,15 +138,24 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])::"memory");
 }
 // Waits for the loads and names their registers, so that no use of them moves above it.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
@@ -640,29 +649,32 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                         pv_seen = true;
                         fence_after();
 #pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(tm + lanes + c, o);
+                        for (int c = 0; c < D; c += 16) {  // (16 columns: the scores stay in registers)
+                            uint32_t o[16];
+                            tmem_ld16(tm + lanes + c, o);
                             tmem_wait_ld(o);
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
-                            tmem_st32(tm + lanes + c, o);
+                            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * al);
+                            tmem_st16(tm + lanes + c, o);
                         }
                     }
                 }
                 const float mu = m == -INFINITY ? 0.f : m - Elem<DT>::kBias;
                 const uint64_t scale2 = pair(a.scale_log2, a.scale_log2), mu2 = pair(-mu, -mu);
                 uint64_t sum[2] = {pair(l, 0.f), pair(0.f, 0.f)};
-                uint32_t p[32];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    float u, v;
-                    unpair(fma2(pair(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), scale2, mu2), u, v);
-                    u = exp2_sfu(u), v = exp2_sfu(v);
-                    sum[j & 1] = add2(sum[j & 1], pair(u, v));
-                    p[j] = Elem<DT>::pack(u, v);
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        float u, v;
+                        unpair(fma2(pair(__uint_as_float(x[32 * h + 2 * j]), __uint_as_float(x[32 * h + 2 * j + 1])), scale2, mu2), u, v);
+                        u = exp2_sfu(u), v = exp2_sfu(v);
+                        sum[j & 1] = add2(sum[j & 1], pair(u, v));
+                        p[j] = Elem<DT>::pack(u, v);
+                    }
+                    tmem_st16(st + 16 * h, p);
                 }
-                tmem_st32(st, p);
                 float u, v;
                 unpair(add2(sum[0], sum[1]), u, v);
                 l = u + v;
