@@ -28,7 +28,8 @@ struct kvx_batch_s {
 
 namespace {
 
-constexpr int kMaxTokens = 1 << 30;   // of a prefix or a tail (token arithmetic in 32 bits)
+constexpr int kMaxTokens = 1 << 30;   // of a prefix, a tail or a rotation (token arithmetic in 32 bits)
+constexpr int kMaxHeads = 1 << 16;
 int ceil_div(int64_t a, int64_t b) { return int((a + b - 1) / b); }
 
 // A batch of at most this many rows a KV head streams its prefix like a tail; more rows go through
@@ -38,10 +39,11 @@ constexpr int kStreamRows = 8;
 // The streaming kernel's share of the device beside the prefix kernel.  A prefix item's tile (64 tokens,
 // 128 rows) takes a CTA's room about as long as four streamed tiles of 16 tokens at head dims from 128
 // on and eight below (the softmax of 128 rows does not shrink with the head), and tails are taken to be
-// half of max_len on average.  Shares below kLeastShare or above kMostShare are not worth the cut (the
-// streaming kernel then simply follows), and a coded prefix, whose CTAs take a SM each, shares nothing
-// (32 sequences of up to 512 tokens behind 32731 coded ones: 74 us shared, 64 not): 64 sequences of up to 1024 tokens behind 32K took 82 us one
-// after the other and 70 us sharing, the ones whose tails weigh 2 % or 80 % 3 % and 25 % longer.
+// half of max_len on average.  64 sequences of up to 1024 tokens behind 32K of 128 dims took 82 us one kernel
+// after the other and 70 us sharing.  Shares below kLeastShare or above kMostShare are not worth the cut
+// (tails of 2 % and of 80 % of the work took 3 % and 25 % longer sharing; the streaming kernel then
+// simply follows), and a coded prefix, whose CTAs take a SM each, shares nothing (32 sequences of up to
+// 512 tokens behind 32731 coded ones: 74 us shared, 64 not).
 constexpr double kLeastShare = 0.15, kMostShare = 0.6;
 double stream_share(int dim, int64_t prefix_tiles, int64_t tail_tiles) {
     const double share = double(tail_tiles) / double(tail_tiles + (dim >= 128 ? 4 : 8) * prefix_tiles);
@@ -67,10 +69,11 @@ int prefix_split_tiles(int tiles, int lists, int slots) {
 // CTAs of the streaming kernel that fill the device.
 int stream_ctas(const kvx_batch_s *h) { return (h->dim <= 128 ? 2 : 1) * h->sms; }
 
-// Rows of an upper bound of the scratch an attention call of `batch` sequences takes.
+// Rows of an upper bound of the scratch an attention call of `batch` sequences takes: at most twice as
+// many items as CTAs that run at a time, or one for each list, and a part for each run and each unit.
 int64_t scratch_rows(const kvx_batch_s *h, int batch) {
     const int64_t rows = int64_t(batch) * h->group;
-    const int64_t tensor = (4 * int64_t(prefix_ctas_per_sm(h->dim, false)) * h->sms + h->n_kv_heads * int64_t(ceil_div(rows, kPrefixRows))) *
+    const int64_t tensor = (2 * int64_t(prefix_ctas_per_sm(h->dim, false)) * h->sms + h->n_kv_heads * int64_t(ceil_div(rows, kPrefixRows))) *
                            kPrefixRows;
     const int64_t units = h->n_kv_heads * (int64_t(batch) * ceil_div(h->group, 8) + ceil_div(kStreamRows, 8));
     return tensor + 8 * (int64_t(stream_ctas(h)) * kStreamWarps + units);
@@ -160,8 +163,8 @@ bool view_ok(const kvx_view *v) { return v != nullptr && v->data != nullptr; }
 extern "C" {
 
 int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int dtype, kvx_batch *out) {
-    if (out == nullptr || max_batch <= 0 || max_batch > kMaxStreamBatch || n_q_heads <= 0 || n_kv_heads <= 0 ||
-        n_q_heads % n_kv_heads != 0 || dim <= 0 || dim % 2 != 0 || dim > kMaxHeadDim ||
+    if (out == nullptr || max_batch <= 0 || max_batch > kMaxStreamBatch || n_q_heads <= 0 || n_q_heads > kMaxHeads ||
+        n_kv_heads <= 0 || n_q_heads % n_kv_heads != 0 || dim <= 0 || dim % 2 != 0 || dim > kMaxHeadDim ||
         (dtype != KVX_DTYPE_BF16 && dtype != KVX_DTYPE_FP16))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_create: bad argument");
     *out = nullptr;
@@ -204,7 +207,8 @@ int kvx_batch_check(kvx_batch h) {
 int kvx_batch_rotate(kvx_batch h, const kvx_view *x, const kvx_view *out, int n_tokens, int n_heads,
                      const kvx_rope *rope, int inverse, void *stream) {
     if (h != nullptr && n_tokens == 0) return KVX_OK;  // (an empty tensor's address is null)
-    if (h == nullptr || !view_ok(x) || !view_ok(out) || n_tokens < 0 || n_heads <= 0 || rope == nullptr)
+    if (h == nullptr || !view_ok(x) || !view_ok(out) || n_tokens < 0 || n_tokens > kMaxTokens || n_heads <= 0 ||
+        n_heads > kMaxHeads || rope == nullptr)
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_rotate: bad argument");
     RotArgs a{};
     if (int rc = rope_of("kvx_batch_rotate", h, rope, a)) return rc;
@@ -222,7 +226,7 @@ int kvx_batch_append(kvx_batch h, const kvx_view *q, const kvx_view *k, const kv
                      int n_tokens, const kvx_rope *rope, const int64_t *slots, const kvx_pages *pages, void *stream) {
     if (h != nullptr && n_tokens == 0) return KVX_OK;
     const bool has_q = q != nullptr && q->data != nullptr;
-    if (h == nullptr || !view_ok(k) || !view_ok(v) || n_tokens < 0 || slots == nullptr ||
+    if (h == nullptr || !view_ok(k) || !view_ok(v) || n_tokens < 0 || n_tokens > kMaxTokens || slots == nullptr ||
         has_q != (q_out != nullptr && q_out->data != nullptr))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_append: bad argument");
     RotArgs a{};

@@ -68,7 +68,7 @@ struct XkvGroup {
     uint32_t b7;      // the block's merge words (index in XkvDev::b7)
     uint16_t n_rows;  // bytes to copy from rows and from codes (multiples of 16; 0: nothing, a raw block or
     uint16_t n_codes; // no tokens)
-    uint32_t bits;    // escapes | tokens << 13 | mode << 18 | (offset of the rows / 2) << 21 | of the codes << 24
+    uint32_t bits;    // escapes | tokens << 13 | mode << 18 | offset of the rows << 20 | of the codes << 23 (both even)
     __host__ __device__ int n_esc() const { return int(bits & 0x1FFFu); }
     __host__ __device__ int n() const { return int((bits >> 13) & 31u); }     // 0 past the block's end
     __host__ __device__ int mode() const { return int((bits >> 18) & 7u); }   // 0 raw, 2, 3, 4
@@ -112,8 +112,9 @@ struct PagedArgs {
     // Streamed units, laid end to end in 16-token tiles: first (a streamed prefix) KV head by KV
     // head and group of 8 rows, prefix_len tokens each; then sequence by sequence, KV head by KV
     // head, group of 8 heads by group, the sequence's own tokens; each unit's tiles are followed by
-    // kUnitTiles empty positions.  The line is cut into equal runs, one for each worker (warp); the part that worker w leaves of unit u is in rows stream_base + 8
-    // (w + u) .., which no other pair has (w + u grows along the line).
+    // kUnitTiles empty positions.  The line is cut into equal runs; the part that run r
+    // leaves of unit u is in rows stream_base + 8 (r + u) .., which no other pair has (r + u grows along
+    // the line).
     int64_t stream_base;
     int32_t stream_prefix;  // units of a streamed prefix (0: the prefix is not streamed)
     int32_t pre_groups;     // its groups of 8 rows

@@ -403,8 +403,50 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
 }
 
 // Folds the partial states of one (sequence, head): M = max m_i, l = sum l_i 2^(m_i - M), out =
-// (sum acc_i 2^(m_i - M)) / l.  One CTA per row; its warps take the parts in turn, each with a
-// running maximum, so that no load waits for another's value; sums run in a fixed order.
+// (sum acc_i 2^(m_i - M)) / l.  One CTA per row; its warps take the parts in turn, a few parts' loads at
+// a time and each with a running maximum, so that no load waits for another's value; sums run in a
+// fixed order.
+template <int V> struct Fold {
+    static constexpr int U = V <= 4 ? 4 : 2;  // parts loaded together
+    float m = -INFINITY, l = 0.f, o[V] = {};
+    // Parts i, i + step, ... of `n` in rows first, first + stride, ...
+    template <int D>
+    __device__ __forceinline__ void take(const PagedArgs &a, int64_t first, int64_t stride, int n, int i, int step, int lane) {
+        for (; i < n; i += U * step) {
+            float2 z[U];
+            float v[U][V];
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const int64_t r = first + int64_t(min(i + k * step, n - 1)) * stride;
+                z[k] = a.ml[r];
+                const float *p = a.acc + r * D + V * lane;
+                if constexpr (V == 1) v[k][0] = p[0];
+                else if constexpr (V == 2) {
+                    const float2 x = *reinterpret_cast<const float2 *>(p);
+                    v[k][0] = x.x, v[k][1] = x.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; j += 4) {
+                        const float4 x = *reinterpret_cast<const float4 *>(p + j);
+                        v[k][j] = x.x, v[k][j + 1] = x.y, v[k][j + 2] = x.z, v[k][j + 3] = x.w;
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k)
+                if (i + k * step < n) {
+                    const float mn = fmaxf(m, z[k].x);
+                    // (a part without a maximum has l = 0, or NaN, which stays)
+                    const float e = mn == -INFINITY ? 1.f : exp2_sfu(m - mn), w = z[k].x == -INFINITY ? 0.f : exp2_sfu(z[k].x - mn);
+                    m = mn;
+                    l = l * e + z[k].y * w;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) o[j] = o[j] * e + (z[k].x == -INFINITY ? 0.f : w * v[k][j]);
+                }
+        }
+    }
+};
+
 constexpr int kCombineWarps = 8;
 template <int D, int DT>
 __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const PagedArgs a) {
@@ -416,81 +458,49 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Paged
     if (a.shared_runs && blockIdx.x + blockIdx.y + threadIdx.x == 0) *a.next_run = 0;  // for the next call
     const int b = blockIdx.y, h = blockIdx.x, head = h / a.group, gi = h - head * a.group;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-    // the row's parts: of the prefix (np, from row prow, pstep apart), then of its own tokens (ns)
     const int row = b * a.group + gi;
-    int np = a.n_split, ns = 0;
-    int64_t prow = int64_t(head) * a.n_split * a.row_pad + row, pstep = a.row_pad, srow = 0;
+    // (the line's lengths, for the streamed parts, are on their way while the prefix's parts are folded)
+    int s0 = 0, s1 = 0, s_end = 0;
+    if (a.stream_ctas > 0) s0 = a.starts[b], s1 = a.starts[b + 1], s_end = a.starts[a.batch];
+    Fold<V> f;
+    if (a.n_split > 0) f.template take<D>(a, int64_t(head) * a.n_split * a.row_pad + row, a.row_pad, a.n_split, warp, nw, lane);
     if (a.stream_ctas > 0) {
-        const int s0 = a.starts[b], n = a.starts[b + 1] - s0 - kUnitTiles;  // the sequence's tiles (< 0: none)
-        const int run = stream_run(a, max(0, stream_line(a, a.starts[a.batch]) - kUnitTiles));
+        const int n = s1 - s0 - kUnitTiles;  // the sequence's tiles (< 0: none)
+        const int run = stream_run(a, max(0, stream_line(a, s_end) - kUnitTiles));
         const int pt = tiles_of(a.prefix_len), per = a.n_kv_heads * a.tail_groups;
-        // the runs that met tiles [f, f + n) of the line, and the first one's row of unit u
-        auto parts = [&](int f, int n, int u, int64_t &first) {
-            const int w = f / run;
-            first = a.stream_base + 8 * (int64_t(w) + u);
-            return (f + n - 1) / run - w + 1;
+        // the runs that met tiles [at, at + n) of the line left rows of unit u from the first one's on
+        auto fold_unit = [&](int at, int n, int u, int g) {
+            const int w = at / run;
+            f.template take<D>(a, a.stream_base + 8 * (int64_t(w) + u) + g, 8, (at + n - 1) / run - w + 1, warp, nw, lane);
         };
         if (a.stream_prefix > 0) {
             const int u = head * a.pre_groups + (row >> 3);
-            np = parts(u * (pt + kUnitTiles), pt, u, prow);
-            prow += row & 7;
-            pstep = 8;
+            fold_unit(u * (pt + kUnitTiles), pt, u, row & 7);
         }
-        if (n > 0) {
-            const int k = head * a.tail_groups + (gi >> 3);
-            ns = parts(a.stream_prefix * (pt + kUnitTiles) + s0 * per + k * (n + kUnitTiles), n, a.stream_prefix + b * per + k, srow);
-            srow += gi & 7;
-        }
-    }
-    float m = -INFINITY, l = 0.f, o[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) o[j] = 0.f;
-#pragma unroll 4
-    for (int i = warp; i < np + ns; i += nw) {
-        const int64_t r = i < np ? prow + i * pstep : srow + 8 * int64_t(i - np);
-        const float2 z = a.ml[r];
-        const float *p = a.acc + r * D + V * lane;
-        float v[V];
-        if constexpr (V == 1) v[0] = p[0];
-        else if constexpr (V == 2) {
-            const float2 x = *reinterpret_cast<const float2 *>(p);
-            v[0] = x.x, v[1] = x.y;
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; j += 4) {
-                const float4 x = *reinterpret_cast<const float4 *>(p + j);
-                v[j] = x.x, v[j + 1] = x.y, v[j + 2] = x.z, v[j + 3] = x.w;
-            }
-        }
-        const float mn = fmaxf(m, z.x);
-        // (a part without a maximum has l = 0, or NaN, which stays)
-        const float e = mn == -INFINITY ? 1.f : exp2_sfu(m - mn), w = z.x == -INFINITY ? 0.f : exp2_sfu(z.x - mn);
-        m = mn;
-        l = l * e + z.y * w;
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = o[j] * e + (z.x == -INFINITY ? 0.f : w * v[j]);
+        const int k = head * a.tail_groups + (gi >> 3);
+        if (n > 0)
+            fold_unit(a.stream_prefix * (pt + kUnitTiles) + s0 * per + k * (n + kUnitTiles), n, a.stream_prefix + b * per + k, gi & 7);
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) sacc[warp][V * lane + j] = o[j];
-    if (lane == 0) sml[warp] = make_float2(m, l);
+    for (int j = 0; j < V; ++j) sacc[warp][V * lane + j] = f.o[j];
+    if (lane == 0) sml[warp] = make_float2(f.m, f.l);
     __syncthreads();
-    float M = -INFINITY;
+    float M = -INFINITY, l = 0.f, w8[kCombineWarps];
     for (int w = 0; w < nw; ++w) M = fmaxf(M, sml[w].x);
-    l = 0.f;
-    float f[kCombineWarps];
 #pragma unroll
     for (int w = 0; w < kCombineWarps; ++w) {
-        if (w >= nw) break;
+        w8[w] = 0.f;
+        if (w >= nw) continue;
         const float2 z = sml[w];
-        f[w] = z.x == -INFINITY ? 0.f : exp2_sfu(z.x - M);
-        l += z.y * f[w];
+        if (z.x != -INFINITY) w8[w] = exp2_sfu(z.x - M);
+        l += z.y * w8[w];
     }
     uint16_t *out = a.out + int64_t(b) * a.out_token + int64_t(h) * a.out_head;
     for (int d = threadIdx.x; d < D; d += blockDim.x) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < kCombineWarps; ++w)
-            if (w < nw) v += sacc[w][d] * f[w];
+            if (w < nw) v += sacc[w][d] * w8[w];
         out[d] = Elem<DT>::one(l == 0.f ? 0.f : v / l);
     }
     if (threadIdx.x == 0 && a.lse != nullptr)
@@ -507,11 +517,12 @@ template <int D, int DT> cudaError_t stream_d(const PagedArgs &a, cudaStream_t s
 template <int D, int DT> cudaError_t beside_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, true>(a, s); }
 
 template <int D, int DT> cudaError_t combine_d(const PagedArgs &a, cudaStream_t s) {
-    // about this many parts a row: more warps where each would take several in turn
+    // about this many parts a row: as many warps as take them in two rounds of loads (a fold of 14 heads
+    // by 16 rows of 3 parts: 2 warps 5.0 us, 4 warps 5.8; of 32 by 5 of 22 at dim 256: 8 warps 5.7, 4 warps 7.1)
     const int units = a.stream_prefix + a.batch * a.n_kv_heads * a.tail_groups;
     const int parts = a.n_split + a.stream_runs / units;
     return launch_paged(combine_kernel<D, DT>, dim3(unsigned(a.n_q_heads), unsigned(a.batch)),
-                        32 * (parts > 16 ? kCombineWarps : 4), 0, s, a);
+                        32 * (parts > 8 * Fold<D / 32>::U ? kCombineWarps : parts > 8 ? 4 : 2), 0, s, a);
 }
 
 }  // namespace

@@ -1,4 +1,4 @@
-// paged_types.cuh -- the two 16-bit types of the serving-step attention kernels.
+// paged_types.cuh -- what the serving-step attention kernels share: the two 16-bit types, copies, launches.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -8,7 +8,6 @@
 
 namespace kvx {
 
-constexpr float kPagedLog2e = 1.4426950408889634f;
 constexpr float kPagedLn2 = 0.6931471805599453f;
 
 // Softmax weights enter the tensor cores in the cache's type, rounded to nearest: 8 significant
@@ -40,20 +39,6 @@ __device__ __forceinline__ float exp2_sfu(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
-}
-
-// Row offset (elements, without the head) of token t of a page list, or -1 when the table's entry
-// is outside the pool (reported).
-__device__ __forceinline__ int64_t page_row(const PoolDev &p, const int32_t *table, int64_t t, int *status) {
-    int64_t i;
-    int32_t place;
-    p.split.at(t, i, place);
-    const int32_t page = __ldg(table + i);
-    if (unsigned(page) >= unsigned(p.n_pages)) {
-        report(status, KVX_ERR_RUNTIME, DERR_PAGE);
-        return -1;
-    }
-    return int64_t(page) * p.page_stride + int64_t(place) * p.token_stride;
 }
 
 // lens[b] clamped to [0, max_len] (reported when it was outside).
