@@ -74,7 +74,7 @@ template <int D, int LOAD> struct Cfg {
     static constexpr int STAGE = S_CODES + 8 * D + 32;
     static constexpr int O_STAGE = O_RING + NSLOT * SLOT;
     static constexpr int O_BAR = O_STAGE + LW * NSTAGE * STAGE;
-    static constexpr int N_BAR = 2 * NSLOT + 8 + LW * NSTAGE;
+    static constexpr int N_BAR = 2 * NSLOT + 9 + LW * NSTAGE;
     static constexpr int SMEM = O_BAR + 8 * N_BAR + 16;
     // arrivals that announce a tile: one of each loader warp, or one for each 16-token group
     static constexpr int ARRIVE = XKV ? TT / 16 : LW;  // (TMA: with the bytes)
@@ -215,9 +215,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 
-// Barriers of a CTA (8 bytes each): full and empty of every ring slot, these, then one for each
-// staging slot.
-enum { B_S0, B_S1, B_P0, B_P1, B_PV, B_Q, B_END, B_DONE, B_COUNT };
+// Barriers of a CTA (8 bytes each): full and empty of every ring slot, these (S, P and PV of even and
+// of odd tiles), then one for each staging slot.
+enum { B_S0, B_S1, B_P0, B_P1, B_PV0, B_PV1, B_Q, B_END, B_DONE, B_COUNT };
 
 // One item.
 struct Item {
@@ -293,8 +293,6 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
     constexpr int LW = C::LW;
     extern __shared__ __align__(1024) uint8_t smem[];
     volatile uint32_t *tmem_base = reinterpret_cast<volatile uint32_t *>(smem + C::O_BAR + 8 * C::N_BAR);
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t sb = smem_u32(smem);
     const uint32_t bars = sb + C::O_BAR;
@@ -318,7 +316,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
         for (int i = 0; i < C::NSLOT; ++i) mbar_init(full(i), C::ARRIVE), mbar_init(empty(i), 1);
         for (int i = 0; i < LW * C::NSTAGE; ++i) mbar_init(bar(B_COUNT + i), 1);
         mbar_init(bar(B_S0), 1), mbar_init(bar(B_S1), 1), mbar_init(bar(B_P0), SW), mbar_init(bar(B_P1), SW);
-        mbar_init(bar(B_PV), 1), mbar_init(bar(B_Q), SW), mbar_init(bar(B_END), 1);
+        mbar_init(bar(B_PV0), 1), mbar_init(bar(B_PV1), 1), mbar_init(bar(B_Q), SW), mbar_init(bar(B_END), 1);
         mbar_init(bar(B_DONE), 1);
         fence_mbar_init();
     }
@@ -326,6 +324,9 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
     __syncthreads();
     fence_after();
     const uint32_t tm = *tmem_base;
+    // what is above touches nothing of the grid before, which may still be running
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp >= SW && warp < SW + LW) {
         // ---- loads ----
@@ -575,8 +576,8 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                         mma_ss(tm + D + (i & 1) * TT, q0 + (p * (ROWS * C::ROWB) + o) / 16, kk + (p * (TT * C::ROWB) + o) / 16, qk,
                                s > 0);
                     }
-                    mma_commit(empty(x));
                     mma_commit(bar(B_S0 + (i & 1)));
+                    mma_commit(empty(x));
                 }
                 if (i > 0) {
                     const int j = i - 1, x = Ring::v_item(j, it.tiles);
@@ -586,8 +587,8 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
 #pragma unroll
                     for (int s = 0; s < TT / 16; ++s)
                         mma_ts(tm, tm + D + (j & 1) * TT + 8 * s, vv + 2 * s * K8 / 16, pv, j > 0 || s > 0);
+                    mma_commit(bar(B_PV0 + (j & 1)));
                     mma_commit(empty(x));
-                    mma_commit(bar(B_PV));
                     if (j == it.tiles - 1) mma_commit(bar(B_DONE));
                 }
             }
@@ -622,7 +623,6 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             ok = __all_sync(FULL, wait(bar(B_S0 + (i & 1)), i >> 1));
             if (!ok) break;
             fence_after();
-            bool pv_seen = i == 0;  // PV(i - 1) has completed
             if (live) {
                 const uint32_t st = tm + lanes + uint32_t(D + (i & 1) * TT);
                 uint32_t x[64];
@@ -644,9 +644,8 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     l *= al;
                     if (i > 0) {
                         // O is complete up to tile i - 1, and the next PV waits for this warp
-                        if (!pv_seen) ok = __all_sync(FULL, wait(bar(B_PV), i - 1));
+                        ok = __all_sync(FULL, wait(bar(B_PV0 + ((i - 1) & 1)), (i - 1) >> 1));
                         if (!ok) break;
-                        pv_seen = true;
                         fence_after();
 #pragma unroll
                         for (int c = 0; c < D; c += 16) {  // (16 columns: the scores stay in registers)
@@ -680,9 +679,11 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                 l = u + v;
                 tmem_wait_st();
             }
-            // B_PV is waited for once a tile, before the arrival that lets its next phase begin: a
-            // phase later its parity would not tell PV(i - 1) done from PV(i) to come
-            if (!pv_seen) ok = __all_sync(FULL, wait(bar(B_PV), i - 1));
+            // PV(i - 2) completed before S(i) did; its barrier is waited for all the same, before the arrival
+            // that lets PV(i) complete: a phase later its parity would not tell one from the other.  (That
+            // PV(i - 1) is not waited for lets two tiles' round trips between these warps and the MMA warp
+            // overlap.)
+            if (i > 1) ok = __all_sync(FULL, wait(bar(B_PV0 + (i & 1)), (i - 2) >> 1));
             if (!ok) break;
             fence_before();
             __syncwarp();
