@@ -32,3 +32,10 @@ def test_host_tensors_are_refused(kvx):
         kvx.Rope(torch.zeros((4, 32)), torch.zeros((4, 32)))
     with pytest.raises(ValueError, match="dtype"):
         kvx.Batch(1, 1, 1, 64, dtype="fp32")
+
+
+@pytest.mark.parametrize("args", [(2049, 8, 2, 64, 0), (1, 65538, 2, 64, 0)])
+def test_batch_create_refuses_what_it_cannot_count(kvx, args):
+    """More sequences or heads than the streaming kernel's lists and the grids are for."""
+    h = C.c_void_p()
+    assert kvx._batch_create(*args, C.byref(h)) == kvx.KVX_ERR_INVALID_ARGUMENT and not h.value
