@@ -18,6 +18,7 @@ struct kvx_batch_s {
     float2 *ml = nullptr;
     int32_t *starts = nullptr;
     int *status = nullptr;
+    bool runs_taken = false;   // a call failed between the kernels that use the counter of runs and zero it
     ~kvx_batch_s() {
         cudaFree(acc);
         cudaFree(ml);
@@ -321,9 +322,15 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     const int64_t used = a.stream_base + (a.stream_ctas > 0 ? 8 * (int64_t(a.stream_runs) + units) : 0);
     if (used > h->cap_rows) return fail(KVX_ERR_RUNTIME, "kvx_batch_attend: scratch too small");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (a.shared_runs) {
+        // the combine pass zeroes the counter: where it was not launched, the streaming kernel would find no runs
+        if (h->runs_taken) KVX_CUDA(cudaMemsetAsync(a.next_run, 0, sizeof(int32_t), s));
+        h->runs_taken = true;
+    }
     if (tensor) KVX_CUDA(launch_paged_prefix(h->dim, h->dtype, a, s));
     KVX_CUDA(launch_paged_stream(h->dim, h->dtype, a, tensor, s));
     KVX_CUDA(launch_paged_combine(h->dim, h->dtype, a, s));
+    if (a.shared_runs) h->runs_taken = false;
     return KVX_OK;
 }
 
