@@ -18,6 +18,7 @@ struct kvx_batch_s {
     float2 *ml = nullptr;
     int32_t *starts = nullptr;
     int *status = nullptr;
+    int wait_us = 1000000;     // limit of a wait inside a kernel
     bool runs_taken = false;   // a call failed between the kernels that use the counter of runs and zero it
     ~kvx_batch_s() {
         cudaFree(acc);
@@ -205,6 +206,14 @@ int kvx_batch_check(kvx_batch h) {
     return KVX_OK;
 }
 
+int kvx_batch_wait_limit(kvx_batch h, int microseconds) {
+    if (h == nullptr || microseconds < 0)
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_wait_limit: bad argument");
+    h->wait_us = microseconds;
+    clear_error();
+    return KVX_OK;
+}
+
 int kvx_batch_rotate(kvx_batch h, const kvx_view *x, const kvx_view *out, int n_tokens, int n_heads,
                      const kvx_rope *rope, int inverse, void *stream) {
     if (h != nullptr && n_tokens == 0) return KVX_OK;  // (an empty tensor's address is null)
@@ -293,6 +302,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     a.acc = h->acc;
     a.ml = h->ml;
     a.status = h->status;
+    a.wait_us = h->wait_us;
     a.starts = h->starts;
     a.next_run = h->starts + h->max_batch + 1;
     const int rows = x->batch * h->group;

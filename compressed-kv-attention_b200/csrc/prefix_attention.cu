@@ -47,7 +47,7 @@ constexpr uint32_t FULL = 0xFFFFFFFFu;
 constexpr int TT = kPrefixTile;         // tokens per tile
 constexpr int ROWS = kPrefixRows;       // query rows per item
 constexpr int SW = 4;                   // softmax warps
-constexpr uint32_t kWaitUs = 1000000;   // bounded waits
+constexpr uint32_t kDrainUs = 1000000;  // for copies and MMAs in flight, after a wait has run out
 
 // Tensor maps of the K and V pools (LOAD_TMA).
 struct alignas(64) PrefixMaps {
@@ -78,7 +78,7 @@ template <int D, int LOAD> struct Cfg {
     static constexpr int STAGE = S_CODES + 8 * D + 32;
     static constexpr int O_STAGE = O_RING + NSLOT * SLOT;
     static constexpr int O_BAR = O_STAGE + LW * NSTAGE * STAGE;
-    static constexpr int N_BAR = 2 * NSLOT + 9 + LW * NSTAGE;
+    static constexpr int N_BAR = 2 * NSLOT + 10 + LW * NSTAGE;
     static constexpr int SMEM = O_BAR + 8 * N_BAR + 16;
     // arrivals that announce a tile: one of each loader warp, or one for each 16-token group
     static constexpr int ARRIVE = XKV ? TT / 16 : LW;  // (TMA: with the bytes)
@@ -220,8 +220,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // Barriers of a CTA (8 bytes each): full and empty of every ring slot, these (S, P and PV of even and
-// of odd tiles), then one for each staging slot.
-enum { B_S0, B_S1, B_P0, B_P1, B_PV0, B_PV1, B_Q, B_END, B_DONE, B_COUNT };
+// of odd tiles; QUIT: the MMAs issued before a wait ran out), then one for each staging slot.
+enum { B_S0, B_S1, B_P0, B_P1, B_PV0, B_PV1, B_Q, B_END, B_DONE, B_QUIT, B_COUNT };
 
 // One item.
 struct Item {
@@ -305,10 +305,12 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
     auto bar = [&](int b) { return bars + 8u * uint32_t(2 * C::NSLOT + b); };
     const Item it = item_of(a, int(blockIdx.x));
     auto wait = [&](uint32_t b, int phase) -> bool {
-        if (mbar_wait_bounded(b, uint32_t(phase & 1), kWaitUs)) return true;
+        if (a.wait_us > 0 && mbar_wait_bounded(b, uint32_t(phase & 1), uint32_t(a.wait_us))) return true;
         report(a.status, KVX_ERR_TIMEOUT, DERR_TIMEOUT);
         return false;
     };
+    // copies and MMAs in flight end before the memory that they use goes away, whatever became of the waits
+    auto drain = [&](uint32_t b, int phase) { mbar_wait_bounded(b, uint32_t(phase & 1), kDrainUs); };
 
     if (warp == SW + LW) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bars + uint32_t(8 * C::N_BAR)),
@@ -321,7 +323,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
         for (int i = 0; i < LW * C::NSTAGE; ++i) mbar_init(bar(B_COUNT + i), 1);
         mbar_init(bar(B_S0), 1), mbar_init(bar(B_S1), 1), mbar_init(bar(B_P0), SW), mbar_init(bar(B_P1), SW);
         mbar_init(bar(B_PV0), 1), mbar_init(bar(B_PV1), 1), mbar_init(bar(B_Q), SW), mbar_init(bar(B_END), 1);
-        mbar_init(bar(B_DONE), 1);
+        mbar_init(bar(B_DONE), 1), mbar_init(bar(B_QUIT), 1);
         fence_mbar_init();
     }
     fence_before();
@@ -424,9 +426,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     __syncwarp();
                 }
             }
-            // after a wait that ran out: let the copies in flight land before the memory goes away
-            if (!ok)
-                for (; k < issued; ++k) mbar_wait_bounded(staged(k), uint32_t((k / NS) & 1), kWaitUs);
+            for (; k < issued; ++k) drain(staged(k), k / NS);  // (none are left where no wait ran out)
         } else if constexpr (LOAD == LOAD_TMA) {
             // Lane i loads box i of a tile: box_tokens tokens of one panel of 64 head dims.  pages of the
             // latest K tile, of the one before it (V follows a tile behind) and of the next; -1: no
@@ -479,7 +479,10 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                              a.heads_inside ? place : it.head, pg, to);
                 if (ends) {
                     ok = __all_sync(FULL, wait(to, 0));
-                    if (!ok) break;
+                    if (!ok) {
+                        drain(to, 0);
+                        break;
+                    }
                     for (int i = lane; i < (TT - valid) * (D / 8); i += 32)
                         sts_v4(dst + tile_off<D, TT>(valid + i / (D / 8), i % (D / 8)), 0u, 0u, 0u, 0u);
                     proxy_fence();
@@ -487,9 +490,8 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     if (lane == 0) mbar_arrive(full(q));
                 }
             }
-            // after a wait that ran out: let the boxes in flight land before the memory goes away
-            if (!ok)
-                for (int i = max(0, q - C::NSLOT); i < q; ++i) mbar_wait_bounded(full(i), uint32_t((i / C::NSLOT) & 1), kWaitUs);
+            // (the MMA warp, which waits for the boxes, may have given up)
+            for (int i = max(0, q - C::NSLOT); i < q; ++i) drain(full(i), i / C::NSLOT);
         } else {
         // Loader warp w copies rows w, w + LW, ... of every tile: lane k holds the offsets of rows w + LW k
         // and w + LW (k + 32) (-1: no such token), looked up a tile ahead of their use.
@@ -562,16 +564,18 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
         }
     } else if (warp == SW + LW) {
         // ---- MMAs ----
-        if (lane == 0 && wait(bar(B_Q), 0)) {
+        if (lane == 0) {
             constexpr uint32_t qk = instr_desc<DT>(TT, false), pv = instr_desc<DT>(D, true);
             constexpr uint32_t K8 = 8 * C::ROWB;  // bytes of 8 rows
             // descriptors of a tile are its base's plus steps of the start address
             const uint64_t q0 = smem_desc(sb + C::O_Q, 16, K8, C::LAYOUT), k0 = smem_desc(sb + C::O_RING, 16, K8, C::LAYOUT),
                            v0 = smem_desc(sb + C::O_RING, TT * C::ROWB, K8, C::LAYOUT);
-            for (int i = 0; i <= it.tiles; ++i) {
+            bool ok = wait(bar(B_Q), 0);
+            for (int i = 0; ok && i <= it.tiles; ++i) {
                 if (i < it.tiles) {
                     const int x = Ring::k_item(i);
-                    if (!wait(full(x), x / C::NSLOT)) break;
+                    ok = wait(full(x), x / C::NSLOT);
+                    if (!ok) break;
                     fence_after();
                     const uint64_t kk = k0 + uint32_t(x % C::NSLOT) * uint32_t(C::SLOT / 16);
 #pragma unroll
@@ -585,7 +589,8 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                 }
                 if (i > 0) {
                     const int j = i - 1, x = Ring::v_item(j, it.tiles);
-                    if (!wait(full(x), x / C::NSLOT) || !wait(bar(B_P0 + (j & 1)), j >> 1)) break;
+                    ok = wait(full(x), x / C::NSLOT) && wait(bar(B_P0 + (j & 1)), j >> 1);
+                    if (!ok) break;
                     fence_after();
                     const uint64_t vv = v0 + uint32_t(x % C::NSLOT) * uint32_t(C::SLOT / 16);
 #pragma unroll
@@ -596,6 +601,8 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     if (j == it.tiles - 1) mma_commit(bar(B_DONE));
                 }
             }
+            if (!ok) mma_commit(bar(B_QUIT));
+            drain(bar(ok ? B_DONE : B_QUIT), 0);
         }
         __syncwarp();
     } else {
@@ -694,6 +701,9 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             if (lane == 0) mbar_arrive(bar(B_P0 + (i & 1)));
         }
         if (ok) ok = __all_sync(FULL, wait(bar(B_DONE), 0));
+        const int n = min(32, it.n - 32 * warp);  // rows of this warp
+        // after a wait that ran out the rows' outputs become NaN (what an earlier call left there is no part of them)
+        if (!ok && lane < n) a.ml[it.row0 + 32 * warp + lane] = make_float2(-INFINITY, __int_as_float(0x7FFFFFFF));
         if (ok && live) {
             // every copy and MMA of the CTA has completed: Q and the ring make room for the rows
             fence_after();
@@ -708,7 +718,6 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
                     *reinterpret_cast<uint4 *>(stage + lane * C::LDO + c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
             __syncwarp();
-            const int n = min(32, it.n - 32 * warp);
             float *dst = a.acc + (it.row0 + 32 * warp) * D;
             for (int j = lane; j < n * (D / 4); j += 32)
                 reinterpret_cast<float4 *>(dst)[j] =

@@ -170,6 +170,7 @@ _batch_rotate = _sig("kvx_batch_rotate", C.c_int,
 _batch_append = _sig("kvx_batch_append", C.c_int,
                      [_vp, _buf, _buf, _buf, _buf, C.c_int, _buf, _vp, _buf, _vp])
 _batch_attend = _sig("kvx_batch_attend", C.c_int, [_vp, _buf, _vp])
+_batch_wait_limit = _sig("kvx_batch_wait_limit", C.c_int, [_vp, C.c_int])
 _batch_check = _sig("kvx_batch_check", C.c_int, [_vp])
 _batch_destroy = _sig("kvx_batch_destroy", None, [_vp])
 _prefix_create = _sig("kvx_prefix_create", C.c_int, [_vp, C.c_int, C.c_int, C.POINTER(_vp)])
@@ -184,7 +185,7 @@ EXPORTED = [
     "kvx_synth_bf16", "kvx_hbm_read_probe", "kvx_attention_decode_noalloc", "kvx_fold_shards",
     "kvx_exponent_stats", "kvx_encode_bf16_bits", "kvx_encode_batch_bits", "kvx_cache_append_bits",
     "kvx_batch_create", "kvx_batch_rotate", "kvx_batch_append", "kvx_batch_attend",
-    "kvx_batch_check", "kvx_batch_destroy", "kvx_prefix_create", "kvx_prefix_destroy",
+    "kvx_batch_wait_limit", "kvx_batch_check", "kvx_batch_destroy", "kvx_prefix_create", "kvx_prefix_destroy",
 ]
 
 # Residual code widths the encoder may use (include/kvexp_b200.h KVX_CODE_BITS_*): the reference's
@@ -690,6 +691,11 @@ class Batch:
             n, scale or 0.0), stream)
         if rc:
             _check(rc)
+
+    def wait_limit(self, microseconds):
+        """How long a kernel may wait for one of its own copies or matrix products (1 s unless set); what depends on
+        a wait that ran out is NaN, and check() raises."""
+        _check(_batch_wait_limit(self._h, int(microseconds)))
 
     def check(self):
         """Synchronise and raise what the device reported since the last check."""

@@ -342,9 +342,16 @@ KVX_API int kvx_batch_append(kvx_batch batch, const kvx_view *q, const kvx_view 
  * pages.  A sequence with neither gets zeros and an lse of -inf.  What a page holds past the
  * last token is never used, whatever its bits. */
 KVX_API int kvx_batch_attend(kvx_batch batch, const kvx_attend *args, void *stream);
+/* How long a kernel of the handle may wait for one of its own copies or matrix products before it gives
+ * up, in microseconds of wall time (1000000 unless set; longer under a debugger or on a device that is
+ * shared in time slices; 0: it gives up at once).  The outputs of a call in which a wait ran out are
+ * NaN as far as they depend on it, and kvx_batch_check reports KVX_ERR_TIMEOUT.  Holds for the calls
+ * after it. */
+KVX_API int kvx_batch_wait_limit(kvx_batch batch, int microseconds);
 /* Synchronise and report device-side errors since the last check: a position outside the tables or
  * a slot outside the pools (what they concern was not written), a table entry outside the pools (it is
- * not read: the outputs that need it mean nothing) or a length outside [0, max_len] (clamped). */
+ * not read: the outputs that need it mean nothing), a length outside [0, max_len] (clamped) or a wait
+ * that ran out (KVX_ERR_TIMEOUT; the outputs that need it are NaN). */
 KVX_API int kvx_batch_check(kvx_batch batch);
 KVX_API void kvx_batch_destroy(kvx_batch batch);
 

@@ -524,3 +524,62 @@ def test_refusals(kvx, cuda, H):
     b.attend(none, none, pages, None, None, 0)
     b.rotate(none, torch.empty(0, dtype=torch.int32, device="cuda"), kvx.Rope(*H.tables(4, 64)), none)
     b.check()
+
+
+# ---- waits that run out -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("limit", [0, 1])
+@pytest.mark.parametrize("hq,hkv,dim,prefix,batch,page,dtype,coded", [
+    (14, 2, 64, 3000, 9, 16, "bf16", False), (32, 8, 128, 20000, 40, 64, "fp16", False), (4, 4, 32, 100, 11, 8, "bf16", False),
+    (8, 4, 256, 2000, 10, 128, "bf16", False), (6, 2, 128, 5000, 7, 7, "fp16", False), (5, 1, 32, 700, 3, 20, "bf16", False),
+    (8, 4, 256, 900, 6, 5, "bf16", False),
+    (14, 2, 64, 4000, 9, 16, "bf16", True), (32, 8, 128, 6000, 20, 64, "bf16", True), (4, 4, 32, 100, 11, 8, "bf16", True),
+    (8, 4, 256, 2000, 10, 128, "bf16", True),
+])
+def test_waits_that_run_out(kvx, cuda, H, hq, hkv, dim, prefix, batch, page, dtype, coded, limit):
+    """With no time for its waits the prefix kernel gives up: the call reports it, and a row is right or NaN, never
+    what an earlier call left in the scratch.  With its time back the handle works as before."""
+    torch = cuda
+    lens = [(7 * i) % 40 for i in range(batch)]
+    c = H.Paged(batch, hq, hkv, dim, prefix, lens, page, dtype=dtype, paged_prefix=not coded)
+    b, pages = kvx.Batch(batch, hq, hkv, dim, dtype=dtype), kvx.Pages(c.k_pool, c.v_pool)
+    if coded:
+        kept = {"prefix": kvx.Prefix.encode(*(x.transpose(0, 1).contiguous() for x in c.prefix))}
+    else:
+        kept = {"prefix_table": c.prefix_table, "prefix_len": prefix}
+    want, want_lse, tol, _ = truth = c.truth()
+
+    def attend(q):
+        out = torch.full((batch, hq, dim), 7.0, device="cuda", dtype=c.q.dtype)
+        lse = torch.full((batch, hq), 7.0, device="cuda")
+        b.attend(q, out, pages, c.table, c.lens, c.max_len, lse=lse, **kept)
+        return out, lse
+
+    attend(c.q.flip(0))  # another call's rows are in the scratch
+    b.check()
+    b.wait_limit(limit)
+    out, lse = attend(c.q)
+    if limit == 0:
+        with pytest.raises(kvx.DeviceTimeout, match="timed out"):
+            b.check()
+        assert bool(out.isnan().all()) and bool(lse.isnan().all())
+    else:  # whether a wait takes longer is the device's affair
+        try:
+            b.check()
+            late = False
+        except kvx.DeviceTimeout:
+            late = True
+        gone = lse.isnan()
+        assert late or not bool(gone.any())
+        assert bool((out.isnan().all(-1) == gone).all())
+        assert bool(((out.double() - want).abs() <= tol)[~gone].all())
+    b.wait_limit(1000000)
+    out, lse = attend(c.q)
+    b.check()
+    H.assert_attends(out, lse, truth)
+
+
+def test_wait_limit_refuses(kvx, cuda):
+    b = kvx.Batch(1, 1, 1, 64)
+    with pytest.raises(ValueError, match="wait_limit"):
+        b.wait_limit(-1)

@@ -39,3 +39,7 @@ def test_batch_create_refuses_what_it_cannot_count(kvx, args):
     """More sequences or heads than the streaming kernel's lists and the grids are for."""
     h = C.c_void_p()
     assert kvx._batch_create(*args, C.byref(h)) == kvx.KVX_ERR_INVALID_ARGUMENT and not h.value
+
+
+def test_wait_limit_of_no_batch(kvx):
+    assert kvx._batch_wait_limit(None, 1) == kvx.KVX_ERR_INVALID_ARGUMENT
