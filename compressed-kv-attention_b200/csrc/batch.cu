@@ -81,6 +81,8 @@ int64_t scratch_rows(const kvx_batch_s *h, int batch) {
     return tensor + 8 * (int64_t(stream_ctas(h)) * kStreamWarps + units);
 }
 
+bool attends(int dim) { return dim == 32 || dim == 64 || dim == 128 || dim == 256; }
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 bool rows_aligned(const kvx_view &v) {
@@ -187,6 +189,8 @@ int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int 
     if (e == cudaSuccess) e = cudaMemset(h->starts, 0, (size_t(max_batch) + 2) * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMalloc(&h->acc, size_t(h->cap_rows) * dim * sizeof(float));
     if (e == cudaSuccess) e = cudaMalloc(&h->ml, size_t(h->cap_rows) * sizeof(float2));
+    if (e == cudaSuccess && attends(dim)) e = prepare_paged_prefix(dim, dtype);
+    if (e == cudaSuccess && attends(dim)) e = prepare_paged_stream(dim, dtype);
     if (e != cudaSuccess) {
         delete h;
         return fail(KVX_ERR_CUDA, std::string("kvx_batch_create: ") + cudaGetErrorString(e));
@@ -262,7 +266,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
         !view_ok(&x->out) || x->prefix_len < 0 || x->max_len < 0 || x->prefix_len > kMaxTokens ||
         x->max_len > kMaxTokens || !(x->scale >= 0.f))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: bad argument");
-    if (h->dim != 32 && h->dim != 64 && h->dim != 128 && h->dim != 256)
+    if (!attends(h->dim))
         return fail(KVX_ERR_UNSUPPORTED, "kvx_batch_attend: head_dim must be 32, 64, 128 or 256");
     const bool coded = x->prefix != nullptr, paged = !coded && x->prefix_table != nullptr && x->prefix_len > 0;
     if (coded && (x->prefix_table != nullptr || x->prefix_len > 0))

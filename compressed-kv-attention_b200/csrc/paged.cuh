@@ -139,6 +139,10 @@ constexpr int kMaxStreamBatch = 2048;
 constexpr int kPrefixRows = 128, kPrefixTile = 64;
 int prefix_ctas_per_sm(int dim, bool coded);
 
+// What the kernels of a head dim and type need once on a device before they are launched there (shared
+// memory beyond the default, which belongs to the device).
+cudaError_t prepare_paged_prefix(int dim, int dtype);
+cudaError_t prepare_paged_stream(int dim, int dtype);
 // The tensor-core kernel over the prefix items of `a`.
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s);
 // The group table of an XKV prefix from its flat blocks' descriptors (heads * blocks of them).

@@ -509,11 +509,14 @@ __global__ void __launch_bounds__(32 * kCombineWarps) combine_kernel(const Paged
         a.lse[int64_t(b) * a.n_q_heads + h] = l == 0.f ? -INFINITY : M * kPagedLn2 + logf(l);
 }
 
+constexpr int list_bytes(int batch) { return 8 * batch + 4; }   // of scan_starts
+template <int D, int DT> cudaError_t prepare_d() {
+    const int bytes = NW * Cfg<D>::RING + list_bytes(kMaxStreamBatch);
+    const cudaError_t e = allow_smem(stream_kernel<D, DT, false>, bytes);
+    return e != cudaSuccess ? e : allow_smem(stream_kernel<D, DT, true>, bytes);
+}
 template <int D, int DT, bool BESIDE> cudaError_t stream_launch(const PagedArgs &a, cudaStream_t s) {
-    constexpr int ring = NW * Cfg<D>::RING;
-    static const cudaError_t attr = allow_smem(stream_kernel<D, DT, BESIDE>, ring + 8 * kMaxStreamBatch + 4);
-    if (attr != cudaSuccess) return attr;
-    return launch_paged(stream_kernel<D, DT, BESIDE>, dim3(unsigned(a.stream_ctas)), NW * 32, ring + 8 * a.batch + 4, s, a);
+    return launch_paged(stream_kernel<D, DT, BESIDE>, dim3(unsigned(a.stream_ctas)), NW * 32, NW * Cfg<D>::RING + list_bytes(a.batch), s, a);
 }
 template <int D, int DT> cudaError_t stream_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, false>(a, s); }
 template <int D, int DT> cudaError_t beside_d(const PagedArgs &a, cudaStream_t s) { return stream_launch<D, DT, true>(a, s); }
@@ -529,15 +532,17 @@ template <int D, int DT> cudaError_t combine_d(const PagedArgs &a, cudaStream_t 
 
 }  // namespace
 
+cudaError_t prepare_paged_stream(int dim, int dtype) { KVX_PAGED_DIM(prepare_d) }
+
 cudaError_t launch_paged_stream(int dim, int dtype, const PagedArgs &a, bool beside, cudaStream_t s) {
     if (a.stream_ctas <= 0) return cudaSuccess;
-    if (beside) KVX_PAGED_DIM(beside_d)
-    KVX_PAGED_DIM(stream_d)
+    if (beside) KVX_PAGED_DIM(beside_d, a, s)
+    KVX_PAGED_DIM(stream_d, a, s)
 }
 
 cudaError_t launch_paged_combine(int dim, int dtype, const PagedArgs &a, cudaStream_t s) {
     if (a.batch <= 0) return cudaSuccess;
-    KVX_PAGED_DIM(combine_d)
+    KVX_PAGED_DIM(combine_d, a, s)
 }
 
 }  // namespace kvx

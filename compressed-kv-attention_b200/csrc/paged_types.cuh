@@ -57,7 +57,7 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // Lets a kernel take up to `bytes` of dynamic shared memory a CTA and all of the SM's (the default split
-// with L1 may leave room for one CTA where two fit).
+// with L1 may leave room for one CTA where two fit), on the current device.
 template <class K> cudaError_t allow_smem(K k, int bytes) {
     cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
@@ -83,12 +83,14 @@ cudaError_t launch_paged(K k, dim3 grid, int threads, int smem, cudaStream_t s, 
 
 }  // namespace kvx
 
-// The instantiation of fn<D, type> for a head dim and type given at run time.
-#define KVX_PAGED_DIM(fn)                                                                                     \
-    switch (dim) {                                                                                            \
-    case 32: return dtype == KVX_DTYPE_BF16 ? fn<32, KVX_DTYPE_BF16>(a, s) : fn<32, KVX_DTYPE_FP16>(a, s);    \
-    case 64: return dtype == KVX_DTYPE_BF16 ? fn<64, KVX_DTYPE_BF16>(a, s) : fn<64, KVX_DTYPE_FP16>(a, s);    \
-    case 128: return dtype == KVX_DTYPE_BF16 ? fn<128, KVX_DTYPE_BF16>(a, s) : fn<128, KVX_DTYPE_FP16>(a, s); \
-    case 256: return dtype == KVX_DTYPE_BF16 ? fn<256, KVX_DTYPE_BF16>(a, s) : fn<256, KVX_DTYPE_FP16>(a, s); \
-    default: return cudaErrorInvalidValue;                                                                    \
+// The instantiation of fn<D, type> for a head dim and type given at run time, called with the other arguments.
+#define KVX_PAGED_TYPE(fn, D, ...) \
+    return dtype == KVX_DTYPE_BF16 ? fn<D, KVX_DTYPE_BF16>(__VA_ARGS__) : fn<D, KVX_DTYPE_FP16>(__VA_ARGS__)
+#define KVX_PAGED_DIM(fn, ...)                           \
+    switch (dim) {                                       \
+    case 32: KVX_PAGED_TYPE(fn, 32, __VA_ARGS__);        \
+    case 64: KVX_PAGED_TYPE(fn, 64, __VA_ARGS__);        \
+    case 128: KVX_PAGED_TYPE(fn, 128, __VA_ARGS__);      \
+    case 256: KVX_PAGED_TYPE(fn, 256, __VA_ARGS__);      \
+    default: return cudaErrorInvalidValue;               \
     }

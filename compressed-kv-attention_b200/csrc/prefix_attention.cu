@@ -735,8 +735,6 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
 template <int D, int DT, int LOAD>
 cudaError_t prefix_launch(const PagedArgs &a, const PrefixMaps &maps, cudaStream_t s) {
     using C = Cfg<D, LOAD>;
-    static const cudaError_t attr = allow_smem(prefix_kernel<D, DT, LOAD>, C::SMEM);
-    if (attr != cudaSuccess) return attr;
     return launch_paged(prefix_kernel<D, DT, LOAD>, dim3(unsigned(a.n_kv_heads * a.n_split * a.row_groups)), C::THREADS, C::SMEM, s, a, maps);
 }
 
@@ -798,6 +796,14 @@ template <int D, int DT> cudaError_t prefix_d(const PagedArgs &args, cudaStream_
     return prefix_launch<D, DT, LOAD_ROWS>(a, maps, s);
 }
 
+template <int D, int DT> cudaError_t prepare_d() {
+    cudaError_t e = allow_smem(prefix_kernel<D, DT, LOAD_TMA>, Cfg<D, LOAD_TMA>::SMEM);
+    if (e == cudaSuccess) e = allow_smem(prefix_kernel<D, DT, LOAD_ROWS>, Cfg<D, LOAD_ROWS>::SMEM);
+    if constexpr (DT == KVX_DTYPE_BF16)
+        if (e == cudaSuccess) e = allow_smem(prefix_kernel<D, DT, LOAD_XKV>, Cfg<D, LOAD_XKV>::SMEM);
+    return e;
+}
+
 // One thread per (flat block, tile): its groups and its token count.
 __global__ void xkv_groups_kernel(const BlockDesc *desc, int64_t n, int tpb, int dim, XkvGroup *groups, uint8_t *tokens) {
     const int64_t i = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -851,9 +857,11 @@ cudaError_t launch_xkv_groups(const BlockDesc *desc, int64_t n_blocks, int tiles
     return cudaGetLastError();
 }
 
+cudaError_t prepare_paged_prefix(int dim, int dtype) { KVX_PAGED_DIM(prepare_d) }
+
 cudaError_t launch_paged_prefix(int dim, int dtype, const PagedArgs &a, cudaStream_t s) {
     if (a.n_split <= 0) return cudaSuccess;
-    KVX_PAGED_DIM(prefix_d)
+    KVX_PAGED_DIM(prefix_d, a, s)
 }
 
 }  // namespace kvx

@@ -29,3 +29,31 @@ def test_runs_after_a_failed_call(dev, kvx, again):
     assert dev.attend(h, **again) == kvx.KVX_OK
     assert [(x.kind, x.shared_runs, x.counter) for x in dev.launches()[:2]] == [("prefix", 1, 0), ("stream", 1, 0)]
     dev.lib.kvx_batch_destroy(h)
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_shared_memory_is_allowed_on_every_device(dev, kvx, dim, dtype):
+    """A kernel's limit of shared memory belongs to a device: a handle on another one launches as well."""
+    for ordinal in (0, 1, 2):
+        dev.lib.fake_set_device(ordinal)
+        rc, h = dev.create(2048, 8, 2, dim, dtype)
+        assert rc == kvx.KVX_OK
+        coded = [dev.lib.fake_prefix(2, dim, 5000)] if dtype == 0 else []
+        for prefix in [dict(prefix_len=1000), dict(prefix_len=1000, page_tokens=5), {}] + [dict(coded=p) for p in coded]:
+            assert dev.attend(h, 2048, 8, 2, dim, max_len=100, **prefix) == kvx.KVX_OK, (ordinal, prefix, dev.lib.fake_last_error())
+        assert {x.device for x in dev.launches()} == {ordinal}
+        for p in coded:
+            dev.lib.fake_prefix_free(p)
+        dev.lib.kvx_batch_destroy(h)
+
+
+def test_a_refused_limit_is_not_remembered(dev, kvx):
+    before = dev.lib.fake_live_allocations()
+    for n in range(3):
+        dev.lib.fake_fail_attribute(n)
+        rc, h = dev.create(4, 8, 2, 64)
+        assert rc == kvx.KVX_ERR_CUDA and not h.value and dev.lib.fake_live_allocations() == before
+    rc, h = dev.create(4, 8, 2, 64)
+    assert rc == kvx.KVX_OK and dev.attend(h, 4, 8, 2, 64, 1000, 100) == kvx.KVX_OK
+    dev.lib.kvx_batch_destroy(h)
