@@ -40,6 +40,7 @@
 // the ranges always agree there.)
 
 #include "attention.cuh"
+#include "host.cuh"
 #include "xkv_decode.cuh"
 
 namespace kvx {
@@ -1213,11 +1214,9 @@ __global__ void __launch_bounds__(1024) split_kernel(const FlatBlock *flat, int6
         for (int w2 = 1; w2 < nw; ++w2) range_begin[w2] = n;
 }
 
-template <int D, bool CP, bool BF16IN> void configure() {
-    static bool done = false;
-    if (done) return;
-    cudaFuncSetAttribute(attn_kernel<D, CP, BF16IN>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, CP>::SMEM);
-    done = true;
+template <int D, bool CP, bool BF16IN> cudaError_t configure() {
+    static SmemLimit limit;
+    return limit.allow(attn_kernel<D, CP, BF16IN>, Cfg<D, CP>::SMEM);
 }
 
 // ---- stage copy lists ------------------------------------------------------------------------------
@@ -1396,7 +1395,7 @@ __global__ void max_valid_kernel(const FlatBlock *flat, int64_t n, int *out) {
 
 template <int D, bool CP, bool BF16IN>
 cudaError_t launch_d(const AttnArgs &a, int grid, cudaStream_t s) {
-    configure<D, CP, BF16IN>();
+    if (cudaError_t e = configure<D, CP, BF16IN>(); e != cudaSuccess) return e;
     // programmatic dependent launch: the grid may be set up while the kernel before it in the
     // stream drains (the kernel waits for that grid before it reads anything)
     cudaLaunchConfig_t cfg = {};

@@ -12,6 +12,7 @@
 //  * enc_emit_kernel     writes header, bases, sign/mantissa bytes, packed residuals and escapes
 //                        (codec.cpp:105-161); byte-identical to encode_bf16.
 #include "codec.cuh"
+#include "host.cuh"
 
 namespace kvx {
 namespace {
@@ -800,12 +801,8 @@ cudaError_t launch_encode_analyze(const uint16_t *const *tensors, int n_tensors,
     const int nb = n_tensors * ((seq + block_tokens - 1) / block_tokens);
     if (nb <= 0) return cudaSuccess;
     const size_t sm = size_t(dim) * 128 * 4;
-    static bool configured = false;
-    if (!configured) {
-        cudaFuncSetAttribute(enc_analyze_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             int(kMaxHeadDim * 128 * 4));
-        configured = true;
-    }
+    static SmemLimit limit;
+    if (cudaError_t e = limit.allow(enc_analyze_kernel, int(kMaxHeadDim * 128 * 4)); e != cudaSuccess) return e;
     enc_analyze_kernel<<<nb, 256, sm, s>>>(tensors, seq, dim, block_tokens, code_bits, blocks, bases);
     return cudaGetLastError();
 }

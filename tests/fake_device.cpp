@@ -1,6 +1,6 @@
 // fake_device.cpp -- the CUDA runtime calls that the serving-step operators' host code makes, without a
 // device: memory is the host's, launches are recorded, and a call can be made to fail.  Linked with
-// batch.cu, rotate.cu, paged_stream.cu and prefix_attention.cu it shows what they ask of the runtime.
+// the sources of those operators and of the kernels beside them it shows what they ask of the runtime.
 #include <cuda.h>
 #include <cuda_runtime_api.h>
 
@@ -19,6 +19,7 @@ namespace {
 constexpr int kDefaultSmem = 48 * 1024;   // what a kernel may take a CTA without having been allowed more
 
 int device = 0;
+cudaError_t last = cudaSuccess;
 int fail_launch = -1, fail_attribute = -1;   // which one from now on fails (0: the next)
 std::vector<Launch> launches;
 std::map<const void *, std::string> &names() {  // (filled before this file's own objects are made)
@@ -27,6 +28,7 @@ std::map<const void *, std::string> &names() {  // (filled before this file's ow
 }
 std::map<std::pair<int, const void *>, int> smem;
 std::set<void *> memory;
+struct { dim3 grid, block; size_t bytes; } call;   // between a launch's <<<>>> and its stub
 
 bool hit(int &countdown) { return countdown >= 0 && countdown-- == 0; }
 
@@ -82,7 +84,11 @@ cudaError_t cudaMemset(void *p, int v, size_t n) {
 }
 cudaError_t cudaMemsetAsync(void *p, int v, size_t n, cudaStream_t) { return cudaMemset(p, v, n); }
 cudaError_t cudaDeviceSynchronize() { return cudaSuccess; }
-cudaError_t cudaGetLastError() { return cudaSuccess; }
+cudaError_t cudaGetLastError() {
+    const cudaError_t e = last;
+    last = cudaSuccess;
+    return e;
+}
 const char *cudaGetErrorString(cudaError_t) { return "an error"; }
 cudaError_t cudaFuncSetAttribute(const void *f, cudaFuncAttribute a, int v) {
     if (hit(fail_attribute)) return cudaErrorInvalidValue;
@@ -95,7 +101,7 @@ cudaError_t cudaGetDriverEntryPoint(const char *, void **p, unsigned long long, 
     return cudaSuccess;
 }
 cudaError_t cudaLaunchKernel(const void *f, dim3 grid, dim3 block, void **args, size_t bytes, cudaStream_t) {
-    return launched(f, grid, block, bytes, args);
+    return last = launched(f, grid, block, bytes, args);
 }
 cudaError_t cudaLaunchKernelExC(const cudaLaunchConfig_t *c, const void *f, void **args) {
     return launched(f, c->gridDim, c->blockDim, c->dynamicSmemBytes, args);
@@ -112,8 +118,15 @@ char __cudaInitModule(void **) { return 1; }
 void __cudaRegisterFunction(void **, const char *f, char *, const char *name, int, uint3 *, uint3 *, dim3 *, dim3 *, int *) {
     names()[f] = name;
 }
-unsigned __cudaPushCallConfiguration(dim3, dim3, size_t, struct CUstream_st *) { return 0; }
-cudaError_t __cudaPopCallConfiguration(dim3 *, dim3 *, size_t *, void *) { return cudaSuccess; }
+unsigned __cudaPushCallConfiguration(dim3 grid, dim3 block, size_t bytes, struct CUstream_st *) {
+    call = {grid, block, bytes};
+    return 0;
+}
+cudaError_t __cudaPopCallConfiguration(dim3 *grid, dim3 *block, size_t *bytes, void *stream) {
+    *grid = call.grid, *block = call.block, *bytes = call.bytes;
+    *static_cast<cudaStream_t *>(stream) = nullptr;
+    return cudaSuccess;
+}
 
 // ---- for the tests ---------------------------------------------------------------------------------------
 

@@ -1,5 +1,8 @@
 // fake_device.cu -- what the stand-in for the CUDA runtime (fake_device.cpp) needs to know of the library: an
-// attention call's arguments, a coded prefix's handle, and the helpers of host.cuh that api.cu defines.
+// attention call's arguments, a coded prefix's handle, the older kernels' launches, and the helpers of host.cuh
+// that api.cu defines.
+#include "../compressed-kv-attention_b200/csrc/attention.cuh"
+#include "../compressed-kv-attention_b200/csrc/codec.cuh"
 #include "../compressed-kv-attention_b200/csrc/host.cuh"
 #include "../compressed-kv-attention_b200/csrc/prefix.cuh"
 #include "fake_device.h"
@@ -34,6 +37,12 @@ void fake_paged(const void *args, Launch *l) {
 
 const char *fake_last_error() { return last_error.c_str(); }
 void fake_set_error(const char *s) { last_error = s; }
+
+// The decode attention kernel and the encoder's first one (their arguments are not looked at).
+int fake_decode_attention(int dim, int bf16, int compact) {
+    return kvx::launch_attention(dim, bf16 != 0, compact != 0, kvx::AttnArgs{}, 1, nullptr);
+}
+int fake_encode(int dim) { return kvx::launch_encode_analyze(nullptr, 1, 100, dim, 128, 0x14, nullptr, nullptr, nullptr); }
 
 // A coded prefix of so many tokens a head (nothing reads its table here).
 kvx_prefix fake_prefix(int heads, int dim, int seq) {

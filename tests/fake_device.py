@@ -8,7 +8,8 @@ import subprocess
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(os.path.dirname(HERE), "compressed-kv-attention_b200", "csrc")
 OUT = os.path.join(HERE, "_build")
-SOURCES = [os.path.join(CSRC, f) for f in ("batch.cu", "rotate.cu", "paged_stream.cu", "prefix_attention.cu")] + [
+SOURCES = [os.path.join(CSRC, f) for f in ("attention.cu", "codec.cu", "batch.cu", "rotate.cu", "paged_stream.cu",
+                                              "prefix_attention.cu")] + [
     os.path.join(HERE, "fake_device.cu"), os.path.join(HERE, "fake_device.cpp")]
 KINDS = ["rotate", "prefix", "stream", "combine", "other"]
 

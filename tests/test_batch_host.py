@@ -57,3 +57,22 @@ def test_a_refused_limit_is_not_remembered(dev, kvx):
     rc, h = dev.create(4, 8, 2, 64)
     assert rc == kvx.KVX_OK and dev.attend(h, 4, 8, 2, 64, 1000, 100) == kvx.KVX_OK
     dev.lib.kvx_batch_destroy(h)
+
+
+@pytest.mark.parametrize("dim", [32, 64, 128, 256])
+def test_older_kernels_launch_on_every_device(dev, kvx, dim):
+    """The decode attention kernel of every kind of plan and the encoder, whose limits are raised where they are
+    launched; a failure is not kept."""
+    calls = [lambda: dev.lib.fake_decode_attention(dim, 1, 0), lambda: dev.lib.fake_decode_attention(dim, 0, 1),
+             lambda: dev.lib.fake_decode_attention(dim, 0, 0), lambda: dev.lib.fake_encode(dim)]
+    for ordinal in (0, 1, 5):
+        dev.lib.fake_set_device(ordinal)
+        assert [c() for c in calls] == [0, 0, 0, 0], ordinal
+        assert [x.device for x in dev.launches()] == [ordinal] * 4
+        assert [c() for c in calls] == [0, 0, 0, 0]
+        dev.launches()
+    dev.lib.fake_set_device(10 + dim // 32)  # (no other test uses it)
+    for c in calls[:3]:
+        dev.lib.fake_fail_attribute(0)
+        assert c() != 0 and not dev.launches()
+        assert c() == 0 and len(dev.launches()) == 1
