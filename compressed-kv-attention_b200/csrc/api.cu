@@ -636,6 +636,7 @@ static int prefix_create_impl(const kvx_unit *heads, int n_kv_heads, int dim, kv
     p->n_kv_heads = n_kv_heads;
     p->dim = dim;
     p->seq = heads[0].seq;
+    KVX_CUDA(cudaGetDevice(&p->device));
     const int tpb = std::max(1, (plan->max_valid + kPrefixTile - 1) / kPrefixTile);
     XkvGroup *groups = nullptr;
     uint8_t *tokens = nullptr;

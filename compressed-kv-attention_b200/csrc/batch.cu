@@ -12,7 +12,7 @@ using namespace kvx;
 
 struct kvx_batch_s {
     int max_batch = 0, n_q_heads = 0, n_kv_heads = 0, group = 0, dim = 0, dtype = 0;
-    int sms = 0;
+    int device = 0, sms = 0;
     int64_t cap_rows = 0;   // partial-state rows of the scratch
     float *acc = nullptr;
     float2 *ml = nullptr;
@@ -160,6 +160,15 @@ RotSeg seg_of(const kvx_view *src, const kvx_view *dst, int heads, bool rotated,
     return s;
 }
 
+// Whether the current device is the handle's (its scratch and its kernels' limits are there).
+int on_device(const char *who, const kvx_batch_s *h) {
+    int dev = 0;
+    KVX_CUDA(cudaGetDevice(&dev));
+    if (dev == h->device) return KVX_OK;
+    return fail(KVX_ERR_INVALID_ARGUMENT, std::string(who) + ": the batch was made on device " + std::to_string(h->device) +
+                                              ", and device " + std::to_string(dev) + " is current");
+}
+
 bool view_ok(const kvx_view *v) { return v != nullptr && v->data != nullptr; }
 
 }  // namespace
@@ -182,8 +191,9 @@ int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int 
     h->dim = dim;
     h->dtype = dtype;
     h->sms = sm_count();
+    cudaError_t e = cudaGetDevice(&h->device);
     h->cap_rows = scratch_rows(h, max_batch);
-    cudaError_t e = cudaMalloc(&h->status, 2 * sizeof(int));
+    if (e == cudaSuccess) e = cudaMalloc(&h->status, 2 * sizeof(int));
     if (e == cudaSuccess) e = cudaMemset(h->status, 0, 2 * sizeof(int));
     if (e == cudaSuccess) e = cudaMalloc(&h->starts, (size_t(max_batch) + 2) * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMemset(h->starts, 0, (size_t(max_batch) + 2) * sizeof(int32_t));
@@ -204,6 +214,7 @@ void kvx_batch_destroy(kvx_batch h) { delete h; }
 
 int kvx_batch_check(kvx_batch h) {
     if (h == nullptr) return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_check: null batch");
+    if (int rc = on_device("kvx_batch_check", h)) return rc;
     KVX_CUDA(cudaDeviceSynchronize());
     if (int rc = read_status(h->status, true)) return rc;
     clear_error();
@@ -224,6 +235,7 @@ int kvx_batch_rotate(kvx_batch h, const kvx_view *x, const kvx_view *out, int n_
     if (h == nullptr || !view_ok(x) || !view_ok(out) || n_tokens < 0 || n_tokens > kMaxTokens || n_heads <= 0 ||
         n_heads > kMaxHeads || rope == nullptr)
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_rotate: bad argument");
+    if (int rc = on_device("kvx_batch_rotate", h)) return rc;
     RotArgs a{};
     if (int rc = rope_of("kvx_batch_rotate", h, rope, a)) return rc;
     a.seg[0] = seg_of(x, out, n_heads, true, 0);
@@ -243,6 +255,7 @@ int kvx_batch_append(kvx_batch h, const kvx_view *q, const kvx_view *k, const kv
     if (h == nullptr || !view_ok(k) || !view_ok(v) || n_tokens < 0 || n_tokens > kMaxTokens || slots == nullptr ||
         has_q != (q_out != nullptr && q_out->data != nullptr))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_append: bad argument");
+    if (int rc = on_device("kvx_batch_append", h)) return rc;
     RotArgs a{};
     if (int rc = pool_of("kvx_batch_append", pages, a.pool)) return rc;
     if (rope != nullptr)
@@ -266,6 +279,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
         !view_ok(&x->out) || x->prefix_len < 0 || x->max_len < 0 || x->prefix_len > kMaxTokens ||
         x->max_len > kMaxTokens || !(x->scale >= 0.f))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: bad argument");
+    if (int rc = on_device("kvx_batch_attend", h)) return rc;
     if (!attends(h->dim))
         return fail(KVX_ERR_UNSUPPORTED, "kvx_batch_attend: head_dim must be 32, 64, 128 or 256");
     const bool coded = x->prefix != nullptr, paged = !coded && x->prefix_table != nullptr && x->prefix_len > 0;
@@ -273,6 +287,8 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: one prefix, in pages or as blobs");
     if (coded && (h->dtype != KVX_DTYPE_BF16 || x->prefix->dim != h->dim || x->prefix->n_kv_heads != h->n_kv_heads))
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: the prefix is BF16 and of other heads or another head_dim");
+    if (coded && x->prefix->device != h->device)
+        return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: the prefix is on another device");
     if (!coded && x->prefix_len > 0 && x->prefix_table == nullptr)
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_attend: a prefix without its page table");
     if (x->max_len > 0 && (x->table == nullptr || x->lens == nullptr))

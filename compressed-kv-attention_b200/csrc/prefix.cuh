@@ -6,7 +6,7 @@
 #include "paged.cuh"
 
 struct kvx_prefix_s {
-    int n_kv_heads = 0, dim = 0, seq = 0;
+    int n_kv_heads = 0, dim = 0, seq = 0, device = 0;
     kvx::XkvDev dev{};
     std::vector<void *> owned;   // device arrays
     ~kvx_prefix_s() {

@@ -478,11 +478,15 @@ def exponent_report(kv, seq_len, head_dim, block_tokens=K_ENCODE_BLOCK, bit_widt
 DTYPES = {"bf16": (0, "bfloat16"), "fp16": (1, "float16")}
 
 
-def _device_tensor(x, name, dtype, ndim):
-    """Checks what the device code takes on trust: a CUDA tensor of this type and rank, its last
-    dimension contiguous.  Returns its strides."""
-    if not getattr(x, "is_cuda", False):
-        raise ValueError(f"{name} must be a CUDA tensor")
+def _device_tensor(x, name, dtype, ndim, device=None):
+    """Checks what the device code takes on trust: a CUDA tensor of this type and rank, on this device
+    if one is given, its last dimension contiguous.  Returns its strides."""
+    at = x.get_device() if hasattr(x, "get_device") else -1
+    if at != device:
+        if at < 0:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if device is not None:
+            raise ValueError(f"{name} is on device {at}, not on device {device}")
     if x.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, not {x.dtype}")
     st = x.stride()
@@ -499,12 +503,14 @@ class Rope:
 
     def __init__(self, cos, sin, axis=None, n_axes=1, interleaved=False):
         import torch
+        _device_tensor(cos, "cos", torch.float32, 2)
+        self.device = cos.get_device()
         for name, x in (("cos", cos), ("sin", sin)):
-            _device_tensor(x, name, torch.float32, 2)
+            _device_tensor(x, name, torch.float32, 2, self.device)
             if not x.is_contiguous() or x.shape != cos.shape:
                 raise ValueError("cos and sin must be contiguous and of one shape")
         if axis is not None:
-            _device_tensor(axis, "axis", torch.uint8, 1)
+            _device_tensor(axis, "axis", torch.uint8, 1, self.device)
             if axis.shape[0] != cos.shape[1]:
                 raise ValueError("axis must name one axis for each pair")
         elif n_axes != 1:
@@ -516,10 +522,12 @@ class Rope:
         self._axis = _addr(axis) or 0
         self._rest = int(cos.shape[0]), 2 * int(cos.shape[1]), self.n_axes, int(bool(interleaved))
 
-    def _at(self, pos, n_tokens):
-        """kvx_rope for positions [n_tokens] or [n_axes, n_tokens] int32."""
+    def _at(self, pos, n_tokens, device):
+        """kvx_rope for positions [n_tokens] or [n_axes, n_tokens] int32 on the device of a batch."""
+        if self.device != device:
+            raise ValueError(f"the rotation's tables are on device {self.device}, not on device {device}")
         shape = pos.shape
-        st = _device_tensor(pos, "pos", self._int32, len(shape))
+        st = _device_tensor(pos, "pos", self._int32, len(shape), device)
         if shape != (self.n_axes, n_tokens) and (shape != (n_tokens,) or self.n_axes != 1):
             raise ValueError("pos must be [n_tokens], or [n_axes, n_tokens]")
         return _pack_rope(*self._tables, pos.data_ptr(), self._axis, st[0] if len(st) == 2 else 0, *self._rest)
@@ -530,8 +538,10 @@ class Pages:
     same type and strides; heads outside tokens in memory is the transposed view of such a pool."""
 
     def __init__(self, k, v):
+        _device_tensor(k, "k", k.dtype, 4)
+        self.device = k.get_device()
         for name, x in (("k", k), ("v", v)):
-            _device_tensor(x, name, k.dtype, 4)
+            _device_tensor(x, name, k.dtype, 4, self.device)
             if x.shape != k.shape or x.stride() != k.stride():
                 raise ValueError("k and v must have one shape and one set of strides")
         self.k, self.v = k, v
@@ -563,7 +573,7 @@ class Prefix:
         """Encodes k and v (BF16 CUDA tensors [n_kv_heads, tokens, dim], contiguous) on the GPU."""
         import torch
         for name, x in (("k", k), ("v", v)):
-            _device_tensor(x, name, torch.bfloat16, 3)
+            _device_tensor(x, name, torch.bfloat16, 3, torch.cuda.current_device())
             if not x.is_contiguous() or x.shape != k.shape:
                 raise ValueError("k and v must be contiguous and of one shape")
         heads, seq, dim = (int(n) for n in k.shape)
@@ -615,10 +625,11 @@ class Batch:
         _check(_batch_create(int(max_batch), self.n_q_heads, self.n_kv_heads, self.dim, code,
                              C.byref(h)))
         self._h = h
+        self.device = torch.cuda.current_device()
 
     def _view(self, x, name, tokens, heads):
         """(address, token stride, head stride) of a [tokens, heads, dim] tensor."""
-        st = _device_tensor(x, name, self._type, 3)
+        st = _device_tensor(x, name, self._type, 3, self.device)
         if x.shape != (tokens, heads, self.dim):
             raise ValueError(f"{name} must be {(tokens, heads, self.dim)}, not {tuple(x.shape)}")
         return x.data_ptr(), st[0], st[1]
@@ -626,6 +637,8 @@ class Batch:
     def _pages(self, pages):
         if pages.n_heads != self.n_kv_heads or pages.dim != self.dim or pages.dtype is not self._type:
             raise ValueError("the page pools have other heads, another head_dim or another type")
+        if pages.device != self.device:
+            raise ValueError(f"the page pools are on device {pages.device}, not on device {self.device}")
         return pages
 
     def rotate(self, x, pos, rope, out, inverse=False, stream=None):
@@ -633,7 +646,7 @@ class Batch:
         gradient's rotation); out may be x."""
         n, heads = x.shape[:2]
         rc = _batch_rotate(self._h, _pack_view(*self._view(x, "x", n, heads)),
-                           _pack_view(*self._view(out, "out", n, heads)), n, heads, rope._at(pos, n),
+                           _pack_view(*self._view(out, "out", n, heads)), n, heads, rope._at(pos, n, self.device),
                            1 if inverse else 0, stream)
         if rc:
             _check(rc)
@@ -643,7 +656,7 @@ class Batch:
         page_tokens + place; negative: not stored), q rotated into q_out (both None: no queries).
         rope None: nothing is rotated."""
         n = k.shape[0]
-        if _device_tensor(slots, "slots", self._int64, 1) and slots.shape[0] != n:
+        if _device_tensor(slots, "slots", self._int64, 1, self.device) and slots.shape[0] != n:
             raise ValueError("slots must be one for each token")
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out go together")
@@ -652,7 +665,7 @@ class Batch:
             self._h, None if q is None else _pack_view(*self._view(q, "q", n, self.n_q_heads)),
             _pack_view(*self._view(k, "k", n, kv)), _pack_view(*self._view(v, "v", n, kv)),
             None if q is None else _pack_view(*self._view(q_out, "q_out", n, self.n_q_heads)), n,
-            None if rope is None else rope._at(pos, n), slots.data_ptr(), self._pages(pages)._c, stream)
+            None if rope is None else rope._at(pos, n, self.device), slots.data_ptr(), self._pages(pages)._c, stream)
         if rc:
             _check(rc)
 
@@ -666,20 +679,20 @@ class Batch:
         max_len, prefix_len = int(max_len), int(prefix_len)
         at_table = at_lens = at_prefix = at_lse = stride = 0
         if max_len > 0:
-            st = _device_tensor(table, "table", self._int32, 2)
-            _device_tensor(lens, "lens", self._int32, 1)
+            st = _device_tensor(table, "table", self._int32, 2, self.device)
+            _device_tensor(lens, "lens", self._int32, 1, self.device)
             if table.shape[0] != n or lens.shape[0] != n:
                 raise ValueError("table and lens must have one row for each sequence")
             if table.shape[1] * pages.page_tokens < max_len:
                 raise ValueError("table rows hold fewer than max_len tokens")
             at_table, at_lens, stride = table.data_ptr(), lens.data_ptr(), st[0]
         if prefix_table is not None and prefix_len > 0:
-            _device_tensor(prefix_table, "prefix_table", self._int32, 1)
+            _device_tensor(prefix_table, "prefix_table", self._int32, 1, self.device)
             if prefix_table.shape[0] * pages.page_tokens < prefix_len:
                 raise ValueError("prefix_table holds fewer than prefix_len tokens")
             at_prefix = prefix_table.data_ptr()
         if lse is not None:
-            _device_tensor(lse, "lse", self._float32, 2)
+            _device_tensor(lse, "lse", self._float32, 2, self.device)
             if lse.shape != (n, heads) or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous [batch, n_q_heads]")
             at_lse = lse.data_ptr()

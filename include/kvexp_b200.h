@@ -325,7 +325,8 @@ typedef struct kvx_attend {
  * takes 32, 64, 128 and 256.  The scratch does not grow with lengths (23 MB for 16 sequences of 14
  * heads of 64, 48 MB for 64 of 32 heads of 128).  One
  * handle serves every layer; like a plan's steps, its attention calls run one after another (calls
- * that overlap on two streams race on its scratch). */
+ * that overlap on two streams race on its scratch).  It belongs to the device that was current; its
+ * calls are refused while another one is, and their buffers are on that device. */
 KVX_API int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int dtype,
                              kvx_batch *batch);
 /* out = x rotated (inverse != 0: by the opposite angles, which is the gradient's rotation).  out

@@ -44,10 +44,11 @@ int fake_decode_attention(int dim, int bf16, int compact) {
 }
 int fake_encode(int dim) { return kvx::launch_encode_analyze(nullptr, 1, 100, dim, 128, 0x14, nullptr, nullptr, nullptr); }
 
-// A coded prefix of so many tokens a head (nothing reads its table here).
+// A coded prefix of so many tokens a head on the current device (nothing reads its table here).
 kvx_prefix fake_prefix(int heads, int dim, int seq) {
     auto *p = new kvx_prefix_s();
     p->n_kv_heads = heads, p->dim = dim, p->seq = seq;
+    cudaGetDevice(&p->device);
     p->dev.tiles = p->dev.head_tiles = (seq + kvx::kPrefixTile - 1) / kvx::kPrefixTile;
     return p;
 }

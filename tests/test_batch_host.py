@@ -76,3 +76,23 @@ def test_older_kernels_launch_on_every_device(dev, kvx, dim):
         dev.lib.fake_fail_attribute(0)
         assert c() != 0 and not dev.launches()
         assert c() == 0 and len(dev.launches()) == 1
+
+
+def test_a_batch_belongs_to_its_device(dev, kvx):
+    """Its calls are refused, with nothing launched, while another device is current; so is another device's prefix."""
+    dev.lib.fake_set_device(1)
+    _, h = dev.create(8, 8, 2, 64)
+    calls = [lambda: dev.attend(h, 8, 8, 2, 64, 1000, 100), lambda: dev.rotate(h, 5, 8, 64), lambda: dev.append(h, 5, 2, 64),
+             lambda: dev.lib.kvx_batch_check(h)]
+    assert [c() for c in calls] == [kvx.KVX_OK] * 4
+    assert {x.device for x in dev.launches()} == {1}
+    dev.lib.fake_set_device(0)
+    for c in calls:
+        assert c() == kvx.KVX_ERR_INVALID_ARGUMENT
+        assert dev.lib.fake_last_error().endswith(b"the batch was made on device 1, and device 0 is current")
+    p = dev.lib.fake_prefix(2, 64, 500)  # (made on device 0)
+    dev.lib.fake_set_device(1)
+    assert dev.attend(h, 8, 8, 2, 64, 0, 100, coded=p) == kvx.KVX_ERR_INVALID_ARGUMENT
+    assert b"another device" in dev.lib.fake_last_error() and not dev.launches()
+    dev.lib.fake_prefix_free(p)
+    dev.lib.kvx_batch_destroy(h)
