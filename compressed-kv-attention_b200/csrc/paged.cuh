@@ -100,7 +100,7 @@ struct PagedArgs {
     XkvDev xkv;             // the prefix when xkv.tiles > 0
     int32_t batch, n_q_heads, n_kv_heads, group;
     float scale_log2;       // scale * log2(e)
-    int32_t wait_us;        // limit of a wait in the tensor-core prefix kernel (0: none is waited for)
+    int32_t wait_us;        // limit of a wait in the tensor-core prefix kernel (0: nothing is computed)
     int *status;
     // Partial states: row r has dim accumulators at acc + r * dim and {m (log2 units), l} at ml[r].
     float *acc;

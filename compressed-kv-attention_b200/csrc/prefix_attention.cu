@@ -305,7 +305,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
     auto bar = [&](int b) { return bars + 8u * uint32_t(2 * C::NSLOT + b); };
     const Item it = item_of(a, int(blockIdx.x));
     auto wait = [&](uint32_t b, int phase) -> bool {
-        if (a.wait_us > 0 && mbar_wait_bounded(b, uint32_t(phase & 1), uint32_t(a.wait_us))) return true;
+        if (mbar_wait_bounded(b, uint32_t(phase & 1), uint32_t(a.wait_us))) return true;
         report(a.status, KVX_ERR_TIMEOUT, DERR_TIMEOUT);
         return false;
     };
@@ -570,7 +570,7 @@ prefix_kernel(const PagedArgs a, const __grid_constant__ PrefixMaps maps) {
             // descriptors of a tile are its base's plus steps of the start address
             const uint64_t q0 = smem_desc(sb + C::O_Q, 16, K8, C::LAYOUT), k0 = smem_desc(sb + C::O_RING, 16, K8, C::LAYOUT),
                            v0 = smem_desc(sb + C::O_RING, TT * C::ROWB, K8, C::LAYOUT);
-            bool ok = wait(bar(B_Q), 0);
+            bool ok = wait(bar(B_Q), 0) && a.wait_us > 0;  // (0: no S is begun, so that every row's wait runs out)
             for (int i = 0; ok && i <= it.tiles; ++i) {
                 if (i < it.tiles) {
                     const int x = Ring::k_item(i);
