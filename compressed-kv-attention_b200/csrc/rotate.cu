@@ -156,7 +156,9 @@ __global__ void __launch_bounds__(256, 4) rotate_many_kernel(const __grid_consta
     const int slot = r % a.head_slots, token = int(blockIdx.x) * a.tokens_per_cta + r / a.head_slots;
     if (r >= a.tokens_per_cta * a.head_slots || token >= a.n_tokens) return;
     float co[8], si[8];
-    const bool angles = 16 * c >= a.rot_dim || load_angles8<INTER>(a, token, c, co, si);
+    // (a padding token without queries turns nothing, and its position is not looked at)
+    const bool turns = a.seg[0].pool == 0 || __ldg(a.slots + token) >= 0;
+    const bool angles = 16 * c >= a.rot_dim || (turns && load_angles8<INTER>(a, token, c, co, si));
 #pragma unroll
     for (int g = 0; g < 3; ++g) {
         const RotSeg &sg = a.seg[g];

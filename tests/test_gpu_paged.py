@@ -160,6 +160,28 @@ def test_append(kvx, cuda, H, tokens, hq, hkv, dim, rot, axes, page, layout, dty
     assert torch.equal(kp, k1) and torch.equal(vp, v1)
 
 
+@pytest.mark.parametrize("tokens,hkv,dim,rot", [(1, 2, 64, 64), (300, 2, 128, 64), (9000, 16, 128, 128), (40, 1, 32, 24)])
+def test_padding_tokens_have_no_position(kvx, cuda, H, tokens, hkv, dim, rot):
+    """A padding token's position is a filler: in an append without queries it is not looked at, however many tokens the
+    call has (9000 of 2 x 16 heads of 128 are over a million pieces); where a query is rotated by it, it is reported."""
+    torch = cuda
+    cos, sin = H.tables(50, rot)
+    rope = kvx.Rope(cos, sin)
+    k, v = (torch.randn((tokens, hkv, dim), device="cuda").to(torch.bfloat16) for _ in range(2))
+    kp, vp = (torch.zeros((tokens, 1, hkv, dim), device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    pad = torch.arange(tokens, device="cuda") % 3 == 0
+    slots = torch.where(pad, -1, torch.arange(tokens, device="cuda"))
+    pos = torch.where(pad, -1, torch.arange(tokens, device="cuda") % 50).to(torch.int32)
+    b = kvx.Batch(1, hkv, hkv, dim)
+    b.append(None, k, v, pos, rope, slots, kvx.Pages(kp, vp), None)
+    b.check()
+    H.assert_rotated(kp[~pad, 0], k[~pad], pos[None, ~pad], cos, sin, None, False, "bf16")
+    assert torch.equal(vp[~pad, 0], v[~pad]) and not bool(kp[pad].any()) and not bool(vp[pad].any())
+    b.append(k, k, v, pos, rope, slots, kvx.Pages(kp, vp), torch.empty_like(k))
+    with pytest.raises(RuntimeError, match="position outside the rotation tables"):
+        b.check()
+
+
 def test_append_past_32_bits(kvx, cuda, H):
     """Elements whose offset in the pool passes 2^32."""
     torch = cuda
