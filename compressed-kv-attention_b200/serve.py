@@ -68,6 +68,7 @@ class Session:
         self.new_k, self.new_v = (draw(layers, steps, batch, n_kv_heads, dim) for _ in range(2))
         self.turned = torch.empty((batch, n_q_heads, dim), device="cuda", dtype=torch.bfloat16)
         self.out = torch.zeros((layers, batch, n_q_heads, dim), device="cuda", dtype=torch.bfloat16)
+        self.taken = 0               # steps since the beginning
         self._graph = None
 
     def _stream(self):
@@ -80,7 +81,10 @@ class Session:
 
     def step(self):
         """One token of every sequence through every layer, on the current stream."""
-        torch, page = self.torch, self.pages[0].page_tokens
+        if self.taken >= self.steps:  # (the sequences' pages are full)
+            raise ValueError(f"all {self.steps} steps have been taken: rewind()")
+        self.taken += 1
+        page = self.pages[0].page_tokens
         s = self._stream()
         pos = self.lens + self.prompt
         place = self.lens.long()
@@ -93,8 +97,14 @@ class Session:
             self.op.attend(self.turned, self.out[i], self.pages[i], self.table, self.lens, self.steps, stream=s, **kept)
         self.step_index += 1
 
+    def rewind(self):
+        """Back to the beginning: the prompt alone."""
+        self.lens.zero_()
+        self.step_index.zero_()
+        self.taken = 0
+
     def capture(self):
-        """The step as a graph.  A step before the capture loads the kernels; its advances are undone
+        """The next step as a graph.  A step before the capture loads the kernels; its advances are undone
         (the first replay writes the same tokens again)."""
         torch = self.torch
         side = torch.cuda.Stream()
@@ -102,17 +112,21 @@ class Session:
         with torch.cuda.stream(side):
             self.step()
         torch.cuda.current_stream().wait_stream(side)
-        self.lens.zero_()
-        self.step_index.zero_()
+        self.lens -= 1
+        self.step_index -= 1
+        self.taken -= 1
         self._graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self._graph):
             self.step()
+        self.taken -= 1              # (a captured step has not run)
 
     def run(self):
-        """Every step; returns the milliseconds they took on the device."""
+        """Every step from the beginning; returns the milliseconds they took on the device."""
         torch = self.torch
+        self.rewind()
         if self._graph is None:
             self.capture()
+        self.taken = self.steps
         t0, t1 = (torch.cuda.Event(enable_timing=True) for _ in range(2))
         t0.record()
         for _ in range(self.steps):

@@ -52,3 +52,31 @@ def test_prompt_in_pages_and_compressed_agree(cuda):
     tol = 3 * 2.0 ** -8 * max(x[1].abs().max().item() for x in a.prompts + [(None, a.new_v)])
     assert float((a.out.float() - b.out.float()).abs().max()) <= tol
     assert 0 < a.prompt_bytes < b.prompt_bytes
+
+
+@pytest.mark.parametrize("compressed", [True, False])
+@pytest.mark.parametrize("steps", [1, 17])
+def test_a_session_runs_again(cuda, steps, compressed):
+    """A second run begins again and gives the same outputs; a step past the last is refused on the host."""
+    import serve
+    torch = cuda
+    s = serve.Session(3, 4, 2, 64, 100, steps, layers=2, compressed=compressed, seed=1)
+    s.run()
+    first = s.out.clone()
+    s.run()
+    assert torch.equal(s.out, first) and int(s.lens.min()) == int(s.lens.max()) == steps
+    with pytest.raises(ValueError, match="steps have been taken"):
+        s.step()
+    s.rewind()
+    for _ in range(steps):  # without the graph
+        s.step()
+    s.op.check()
+    assert torch.equal(s.out, first)
+    with pytest.raises(ValueError, match="steps have been taken"):
+        s.capture()
+
+
+def test_a_session_of_no_steps(cuda):
+    import serve
+    with pytest.raises(ValueError, match="steps have been taken"):
+        serve.Session(3, 4, 2, 64, 100, 0).run()
