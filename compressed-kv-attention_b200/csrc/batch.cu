@@ -169,6 +169,11 @@ int on_device(const char *who, const kvx_batch_s *h) {
                                               ", and device " + std::to_string(dev) + " is current");
 }
 
+int done() {
+    clear_error();
+    return KVX_OK;
+}
+
 bool view_ok(const kvx_view *v) { return v != nullptr && v->data != nullptr; }
 
 }  // namespace
@@ -206,8 +211,7 @@ int kvx_batch_create(int max_batch, int n_q_heads, int n_kv_heads, int dim, int 
         return fail(KVX_ERR_CUDA, std::string("kvx_batch_create: ") + cudaGetErrorString(e));
     }
     *out = h;
-    clear_error();
-    return KVX_OK;
+    return done();
 }
 
 void kvx_batch_destroy(kvx_batch h) { delete h; }
@@ -217,21 +221,19 @@ int kvx_batch_check(kvx_batch h) {
     if (int rc = on_device("kvx_batch_check", h)) return rc;
     KVX_CUDA(cudaDeviceSynchronize());
     if (int rc = read_status(h->status, true)) return rc;
-    clear_error();
-    return KVX_OK;
+    return done();
 }
 
 int kvx_batch_wait_limit(kvx_batch h, int microseconds) {
     if (h == nullptr || microseconds < 0)
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_wait_limit: bad argument");
     h->wait_us = microseconds;
-    clear_error();
-    return KVX_OK;
+    return done();
 }
 
 int kvx_batch_rotate(kvx_batch h, const kvx_view *x, const kvx_view *out, int n_tokens, int n_heads,
                      const kvx_rope *rope, int inverse, void *stream) {
-    if (h != nullptr && n_tokens == 0) return KVX_OK;  // (an empty tensor's address is null)
+    if (h != nullptr && n_tokens == 0) return done();  // (an empty tensor's address is null)
     if (h == nullptr || !view_ok(x) || !view_ok(out) || n_tokens < 0 || n_tokens > kMaxTokens || n_heads <= 0 ||
         n_heads > kMaxHeads || rope == nullptr)
         return fail(KVX_ERR_INVALID_ARGUMENT, "kvx_batch_rotate: bad argument");
@@ -245,12 +247,12 @@ int kvx_batch_rotate(kvx_batch h, const kvx_view *x, const kvx_view *out, int n_
     a.dim = h->dim;
     a.heads = n_heads;
     KVX_CUDA(launch_rotate(h->dtype, vector_path(a, 1), a, static_cast<cudaStream_t>(stream)));
-    return KVX_OK;
+    return done();
 }
 
 int kvx_batch_append(kvx_batch h, const kvx_view *q, const kvx_view *k, const kvx_view *v, const kvx_view *q_out,
                      int n_tokens, const kvx_rope *rope, const int64_t *slots, const kvx_pages *pages, void *stream) {
-    if (h != nullptr && n_tokens == 0) return KVX_OK;
+    if (h != nullptr && n_tokens == 0) return done();
     const bool has_q = q != nullptr && q->data != nullptr;
     if (h == nullptr || !view_ok(k) || !view_ok(v) || n_tokens < 0 || n_tokens > kMaxTokens || slots == nullptr ||
         has_q != (q_out != nullptr && q_out->data != nullptr))
@@ -270,11 +272,11 @@ int kvx_batch_append(kvx_batch h, const kvx_view *q, const kvx_view *k, const kv
     a.dim = h->dim;
     a.heads = (has_q ? h->n_q_heads : 0) + 2 * h->n_kv_heads;
     KVX_CUDA(launch_rotate(h->dtype, vector_path(a, n), a, static_cast<cudaStream_t>(stream)));
-    return KVX_OK;
+    return done();
 }
 
 int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
-    if (h != nullptr && x != nullptr && x->batch == 0) return KVX_OK;
+    if (h != nullptr && x != nullptr && x->batch == 0) return done();
     if (h == nullptr || x == nullptr || x->batch < 0 || x->batch > h->max_batch || !view_ok(&x->q) ||
         !view_ok(&x->out) || x->prefix_len < 0 || x->max_len < 0 || x->prefix_len > kMaxTokens ||
         x->max_len > kMaxTokens || !(x->scale >= 0.f))
@@ -361,7 +363,7 @@ int kvx_batch_attend(kvx_batch h, const kvx_attend *x, void *stream) {
     KVX_CUDA(launch_paged_stream(h->dim, h->dtype, a, tensor, s));
     KVX_CUDA(launch_paged_combine(h->dim, h->dtype, a, s));
     if (a.shared_runs) h->runs_taken = false;
-    return KVX_OK;
+    return done();
 }
 
 }  // extern "C"

@@ -61,6 +61,7 @@ def load(kvx):
         C.c_int, C.POINTER(kvx.kvx_rope), C.c_void_p, C.POINTER(kvx.kvx_pages), C.c_void_p]
     lib.kvx_batch_rotate.argtypes = [C.c_void_p] + [C.POINTER(kvx.kvx_view)] * 2 + [
         C.c_int, C.c_int, C.POINTER(kvx.kvx_rope), C.c_int, C.c_void_p]
+    lib.kvx_batch_wait_limit.argtypes = [C.c_void_p, C.c_int]
     lib.kvx_batch_check.argtypes = [C.c_void_p]
     lib.fake_last_error.restype = C.c_char_p
     lib.fake_set_error.argtypes = [C.c_char_p]

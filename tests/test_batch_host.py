@@ -96,3 +96,13 @@ def test_a_batch_belongs_to_its_device(dev, kvx):
     assert b"another device" in dev.lib.fake_last_error() and not dev.launches()
     dev.lib.fake_prefix_free(p)
     dev.lib.kvx_batch_destroy(h)
+
+
+def test_a_success_clears_the_last_error(dev, kvx):
+    _, h = dev.create(8, 8, 2, 64)
+    for call in (lambda: dev.attend(h, 8, 8, 2, 64, 1000, 100), lambda: dev.attend(h, 0, 8, 2, 64), lambda: dev.rotate(h, 5, 8, 64),
+                 lambda: dev.rotate(h, 0, 8, 64), lambda: dev.append(h, 5, 2, 64), lambda: dev.append(h, 0, 2, 64),
+                 lambda: dev.lib.kvx_batch_wait_limit(h, 5), lambda: dev.lib.kvx_batch_check(h)):
+        dev.lib.fake_set_error(b"an earlier call's")
+        assert call() == kvx.KVX_OK and dev.lib.fake_last_error() == b""
+    dev.lib.kvx_batch_destroy(h)
