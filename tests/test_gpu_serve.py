@@ -80,3 +80,48 @@ def test_a_session_of_no_steps(cuda):
     import serve
     with pytest.raises(ValueError, match="steps have been taken"):
         serve.Session(3, 4, 2, 64, 100, 0).run()
+
+
+@pytest.mark.parametrize("compressed", [True, False])
+@pytest.mark.parametrize("batch,hq,hkv,dim,prompt,steps", [(3, 4, 2, 64, 333, 19), (34, 8, 2, 128, 700, 33), (2, 14, 2, 64, 2000, 1)])
+def test_the_newest_and_the_first_own_token(cuda, batch, hq, hkv, dim, prompt, steps, compressed):
+    """The last step's even heads look at its own token and its odd heads at the sequence's first, so that a length, a slot
+    or a position that is off by one shows.  The cache is where the table says, K rotated and V as it was; the outputs are
+    within attention64's bound of what 64 bits make of that cache, and outside of it without either token."""
+    import paged_helpers as H
+    import serve
+    torch = cuda
+    s = serve.Session(batch, hq, hkv, dim, prompt, steps, layers=2, compressed=compressed, seed=batch)
+    cos, sin = serve.rope_tables(prompt + steps, dim)
+    head = torch.arange(hq, device="cuda") // (hq // hkv)
+    apart = torch.tensor([[steps - 1]], device="cuda")
+    for layer in range(2):
+        newest, first = s.new_k[layer, -1][:, head], s.new_k[layer, 0][:, head]
+        # turned back by the places between them, the first token's key meets its own rotation
+        first = H.rotate64(first.transpose(0, 1), apart.expand(1, hq), cos, sin, None, False, inverse=True)[0].transpose(0, 1)
+        at = torch.where((torch.arange(hq, device="cuda") % 2 == 0)[:, None], newest.double(), first)
+        s.new_q[layer, -1] = (at * 30.0 * dim ** 0.5 / at.square().sum(-1, keepdim=True)).to(torch.bfloat16)
+    s.run()
+    per = s.pages[0].page_tokens
+    t = torch.arange(steps, device="cuda")
+    pos = (prompt + t).to(torch.int32)
+    last = torch.full((batch,), prompt + steps - 1, device="cuda", dtype=torch.int32)
+    for layer in range(2):
+        k, v = s.prompts[layer]
+        turned, q = torch.empty_like(k), torch.empty_like(s.new_q[layer, -1])
+        s.op.rotate(k, torch.arange(prompt, device="cuda", dtype=torch.int32), s.rope, turned)
+        s.op.rotate(s.new_q[layer, -1], last, s.rope, q)
+        kv = []
+        for b in range(batch):
+            page = s.table[b].long()[t // per]
+            own_k, own_v = s.pages[layer].k[page, t % per], s.pages[layer].v[page, t % per]
+            H.assert_rotated(own_k, s.new_k[layer, :, b], pos[None], cos, sin, None, False, "bf16")
+            assert torch.equal(own_v, s.new_v[layer, :, b])
+            kv.append((torch.cat((turned, own_k)), torch.cat((v, own_v))))
+        truth = H.attention64(q, kv, dim ** -0.5, "bf16")
+        H.assert_attends(s.out[layer], None, truth)
+        even = torch.arange(hq, device="cuda") % 2 == 0
+        for gone, heads in [(prompt + steps - 1, even), (prompt, ~even)]:
+            less = [(torch.cat((a[:gone], a[gone + 1:])), torch.cat((c[:gone], c[gone + 1:]))) for a, c in kv]
+            off = (H.attention64(q, less, dim ** -0.5, "bf16")[0] - truth[0]).abs() > 2 * truth[2]
+            assert float(off[:, heads].double().mean()) > 0.9
