@@ -1,8 +1,12 @@
 """Host side of the serving-step operators without a GPU: what they ask of the CUDA runtime, over a stand-in for it
 (fake_device)."""
+import math
+import random
+
 import pytest
 
 import fake_device
+import long_cases
 
 pytestmark = pytest.mark.skipif(fake_device.nvcc() is None, reason="no nvcc")
 
@@ -106,3 +110,55 @@ def test_a_success_clears_the_last_error(dev, kvx):
         dev.lib.fake_set_error(b"an earlier call's")
         assert call() == kvx.KVX_OK and dev.lib.fake_last_error() == b""
     dev.lib.kvx_batch_destroy(h)
+
+
+def test_long_cases_have_long_items(dev, kvx):
+    """The GPU test of the prefix kernel's steady state has items of as many tiles as it is meant to."""
+    for hq, hkv, dim, batch, prefix, page, dtype in long_cases.CASES:
+        rc, h = dev.create(batch, hq, hkv, dim, int(dtype == "fp16"))
+        coded = dev.lib.fake_prefix(hkv, dim, prefix) if page == 0 else None
+        paged = {} if page == 0 else dict(prefix_len=prefix, page_tokens=page)
+        assert rc == kvx.KVX_OK and dev.attend(h, batch, hq, hkv, dim, max_len=5, coded=coded, **paged) == kvx.KVX_OK
+        x = dev.launches()[0]
+        assert x.kind == "prefix" and x.split_tiles >= long_cases.LEAST_TILES
+        dev.lib.kvx_batch_destroy(h)
+        if coded:
+            dev.lib.fake_prefix_free(coded)
+    loaders = {(c[2], c[5] == 0, c[5] % 8 == 0, c[6]) for c in long_cases.CASES}
+    for dim in (32, 64, 128, 256):
+        assert (dim, True, True, "bf16") in loaders
+        assert {t for d, coded, tma, t in loaders if d == dim and not coded and not tma} == {"bf16", "fp16"}
+        assert any(d == dim and not coded and tma for d, coded, tma, t in loaders)
+
+
+def test_every_cut_covers_its_prefix_and_fits_the_scratch(dev, kvx):
+    """Random layouts and lengths over the accepted ranges: the items cover every tile once, and the partial states fit."""
+    rng = random.Random(5)
+
+    def upto(n):
+        return int(math.exp(rng.uniform(0.0, math.log(n))))
+
+    for _ in range(400):
+        hkv, group, dim, dtype = upto(200), upto(40), rng.choice([32, 64, 128, 256]), rng.choice([0, 1])
+        most = upto(min(2048, max(1, 60000 // (hkv * group))))
+        hq = hkv * group
+        rc, h = dev.create(most, hq, hkv, dim, dtype)
+        assert rc == kvx.KVX_OK
+        for _ in range(6):
+            batch, prefix, tail, page = upto(most), upto(1 << 21) if rng.random() < 0.8 else 0, upto(1 << 17) - 1, rng.choice([1, 7, 16, 64])
+            coded = dev.lib.fake_prefix(hkv, dim, prefix) if prefix and dtype == 0 and rng.random() < 0.4 else None
+            rc = dev.attend(h, batch, hq, hkv, dim, 0 if coded else prefix, tail, page, coded)
+            assert rc == kvx.KVX_OK, (hq, hkv, dim, most, batch, prefix, tail, page, dev.lib.fake_last_error())
+            ran = dev.launches()
+            kinds = [x.kind for x in ran]
+            streamed = tail > 0 or (prefix > 0 and coded is None and batch * group <= 8)
+            tensor = prefix > 0 and (coded is not None or batch * group > 8)
+            assert kinds == ["prefix"] * tensor + ["stream"] * streamed + ["combine"]
+            if tensor:
+                x = ran[0]
+                assert x.prefix_tiles == -(-prefix // 64) and x.row_groups == -(-batch * group // 128)
+                assert (x.n_split - 1) * x.split_tiles < x.prefix_tiles <= x.n_split * x.split_tiles
+                assert x.grid == hkv * x.n_split * x.row_groups
+            if coded:
+                dev.lib.fake_prefix_free(coded)
+        dev.lib.kvx_batch_destroy(h)
