@@ -365,6 +365,65 @@ def test_attend_in_a_graph_on_a_stream(kvx, cuda, H):
     b.check()
 
 
+@pytest.mark.parametrize("batch,hq,hkv,dim,prefix,longest,page,dtype", [
+    (129, 4, 2, 64, 0, 40, 16, "bf16"), (300, 2, 2, 128, 4000, 64, 16, "bf16"), (700, 2, 2, 256, 0, 33, 7, "fp16"),
+    (1500, 8, 1, 64, 1000, 20, 16, "fp16"), (2048, 2, 1, 32, 300, 50, 16, "bf16"), (2048, 4, 2, 128, 100, 70, 32, "bf16"),
+    (2048, 2, 2, 256, 100, 20, 16, "bf16"),
+])
+def test_attend_large_batches(kvx, cuda, H, batch, hq, hkv, dim, prefix, longest, page, dtype):
+    """More sequences than a CTA has threads, up to the handle's bound; ragged, many of them empty."""
+    lens = [(i * 7919) % (longest + 1) if i % 5 else 0 for i in range(batch)]
+    lens[3] = longest
+    c = H.Paged(batch, hq, hkv, dim, prefix, lens, page, dtype=dtype, seed=batch)
+    out, lse = _attend(kvx, cuda, H, c, hq, hkv, dim)
+    H.assert_attends(out, lse, c.truth())
+    again, _ = _attend(kvx, cuda, H, c, hq, hkv, dim)
+    assert cuda.equal(out.view(cuda.int16), again.view(cuda.int16))
+
+
+@pytest.mark.parametrize("batch,hq,hkv,dim,prefix,page,dtype", [
+    (3, 14, 2, 64, 0, 16, "bf16"), (1, 8, 8, 128, 500, 16, "bf16"), (20, 8, 2, 64, 3000, 16, "fp16"), (64, 8, 2, 128, 9000, 64, "bf16"),
+    (40, 16, 16, 32, 900, 48, "bf16"), (5, 32, 8, 256, 700, 128, "bf16"),
+])
+def test_attend_lengths_far_below_max_len(kvx, cuda, H, batch, hq, hkv, dim, prefix, page, dtype):
+    """max_len as a capacity: tables with room for 20000 tokens, of which a few are there."""
+    torch = cuda
+    lens = [(i * 31) % 90 for i in range(batch)]
+    c = H.Paged(batch, hq, hkv, dim, prefix, lens, page, dtype=dtype)
+    wide = torch.full((batch, -(-20000 // page)), -1, device="cuda", dtype=torch.int32)  # (never looked at)
+    wide[:, :c.table.shape[1]] = c.table
+    c.table, c.max_len = wide, 20000
+    out, lse = _attend(kvx, torch, H, c, hq, hkv, dim)
+    H.assert_attends(out, lse, c.truth())
+
+
+def test_attend_on_two_streams(kvx, cuda, H):
+    """Two handles of different shapes on two streams at once, each with its own scratch: the same bits as one after the
+    other."""
+    torch = cuda
+    shapes = [(64, 32, 8, 128, 9000, 300, "bf16"), (20, 14, 2, 64, 5000, 900, "fp16")]
+    made = []
+    for batch, hq, hkv, dim, prefix, longest, dtype in shapes:
+        c = H.Paged(batch, hq, hkv, dim, prefix, [(i * 37) % (longest + 1) for i in range(batch)], 16, dtype=dtype, seed=dim)
+        b, pages = kvx.Batch(batch, hq, hkv, dim, dtype=dtype), kvx.Pages(c.k_pool, c.v_pool)
+
+        def call(out, stream, b=b, c=c, pages=pages):
+            b.attend(c.q, out, pages, c.table, c.lens, c.max_len, prefix_table=c.prefix_table, prefix_len=c.prefix_len, stream=stream)
+
+        want = torch.empty((batch, hq, dim), device="cuda", dtype=c.q.dtype)
+        call(want, None)
+        b.check()
+        H.assert_attends(want, None, c.truth())
+        made.append((b, call, want, [torch.full_like(want, 7.0) for _ in range(40)], torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for i in range(40):
+        for b, call, want, outs, stream in made:
+            call(outs[i], stream.cuda_stream)
+    for b, call, want, outs, stream in made:
+        b.check()
+        assert all(torch.equal(x, want) for x in outs)
+
+
 # ---- a prefix kept as XKV blobs ---------------------------------------------------------------------
 
 def _modes(torch, seq, heads, dim, block, seed, special=0.01):
