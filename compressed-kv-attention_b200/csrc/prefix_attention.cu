@@ -28,7 +28,7 @@
 // What bounds it: per 64 tokens and 128 rows the SM's exponentials take 64 x 128 / 16 = 512 cycles, the
 // MMAs at D = 128 about 600 (measured alone; S rereads Q for every 64 tokens) and the bytes from HBM
 // 256 D / 23 (712 at D = 64, 1425 at D = 128, shared by all 128-row items of the head through L2).  On one
-// B200, with the combine pass: 7 x 32 heads of 128 (28 rows) behind 131072 FP16 tokens 89 us, 6.0 TB/s, HBM;
+// B200, with the combine pass: 7 x 32 heads of 128 (28 rows) behind 131072 FP16 tokens 90 us, 6.0 TB/s, HBM;
 // 64 x 32 heads (256 rows) behind 32768 BF16 tokens 51 us, 680 TFLOP/s, where copies alone take 38 and
 // MMAs with softmax 37: two CTAs a SM overlap the rest; 32 x 32 heads behind 32731 coded tokens 53 us,
 // where the decode alone takes 47 and the rest without it 44.

@@ -216,7 +216,9 @@ __global__ void __launch_bounds__(256) rotate_few_kernel(const __grid_constant__
     store_once(out + p.first + p.apart, y);
 }
 
-// The same for any even width, stride and alignment: one thread per (token, head, pair of values).
+// The same for any even width, stride and alignment: one thread per (token, head, pair of values), two
+// bytes an access.  32768 tokens of 32 heads of 128, 72 of them rotated: 418 us (1.3 TB/s), where 64 rotated
+// take 84 in the kernel above; 20000 of 9 heads of 32 with 24 rotated: 25 us.
 template <int DT>
 __global__ void __launch_bounds__(256) rotate_any_kernel(const __grid_constant__ RotArgs a) {
     asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -254,7 +254,8 @@ KVX_API int kvx_attention_decode_noalloc(const uint16_t *q, const uint8_t *k_xkv
 
 /* The operators of a batch's decode step beside the compressed cache: rotate queries and keys by
  * their positions, append new keys and values to a paged cache (rotated on the way), and attend
- * from every sequence of a batch to one shared prefix (read once for all of them) followed by the
+ * from every sequence of a batch to one shared prefix (read once for every 128 (sequence, query
+ * head) rows of a KV head; later ones find it in L2 where it fits) followed by the
  * sequence's own pages.  All calls are asynchronous on `stream`, allocate nothing and do not
  * synchronise, so they can be captured in a CUDA graph.  No counterpart in the reference. */
 #define KVX_DTYPE_BF16 0
@@ -314,7 +315,8 @@ typedef struct kvx_attend {
     const int32_t *lens;         /* [batch] tokens in each sequence's own pages */
     int64_t table_stride;
     int32_t prefix_len;
-    int32_t max_len;             /* >= every lens[b]; table rows hold that many tokens' pages */
+    int32_t max_len;             /* >= every lens[b]; table rows hold that many tokens' pages.  The
+                                  * device is shared out as if lengths were max_len / 2 on average */
     int32_t batch;
     float scale;                 /* of q . k; 0 means dim^-1/2 */
 } kvx_attend;
